@@ -419,6 +419,54 @@ int b200_mask_tiles(const void* mask, int64_t B, int64_t T, int64_t S, int64_t m
  * (few or very many keys, rows that are not 16-byte aligned): looking for them would be a launch for nothing. */
 int b200_attn_prefill_reads_tiles(const void* mask, int64_t S, int64_t mask_b, int64_t mask_t, int dtype);
 
+/* ------------------------------------------------------------------------- *
+ * Serving over a paged KV cache.  No counterpart in the reference, whose cache is one static
+ * tensor per layer with all sequences at one position.
+ *   k_pages, v_pages: pages of page_size rows of Hkv heads, at the element strides kv_strides = (page, head, row) of
+ *     both (head_dim contiguous), so [num_pages, Hkv, page_size, D] and [num_pages, page_size, Hkv, D] both work.
+ *   The tokens of a step lie behind one another in [n_tokens, heads, D], sequence after sequence.
+ * Pages, slots and lengths are read on the device: a captured call follows what the arrays hold when it is replayed.
+ * ------------------------------------------------------------------------- */
+/* Keys and values of a step's tokens into their pages, with the rotation of queries and keys on the way: beside
+ * b200_qkv_rope_cache, for sequences at positions of their own.
+ *   q [n_tokens, Hq, D], k, v [n_tokens, Hkv, D]: views with element strides (token, head); Hq = 0: no queries;
+ *   cos_t, sin_t [n_tokens, D] of the tokens' positions, in f32 or the activation type (table_dtype); both NULL: no rotation;
+ *   q_out [n_tokens, Hq, D] dense (may be q itself where that is dense); slots[n] = page * page_size + row, a
+ *   slot outside the pages writes nothing (padding; its query is rotated all the same).  Of equal slots any one may stay.
+ * y = x*cos + rotate_half(x)*sin in fp32, rounded once.  head_dim a multiple of 16. */
+int b200_paged_append(const void* q, const void* k, const void* v, const void* cos_t, const void* sin_t, void* q_out,
+                      void* k_pages, void* v_pages, const int64_t* slots, int64_t n_tokens, int Hq, int Hkv, int D,
+                      int64_t num_pages, int page_size, const int64_t q_strides[2], const int64_t k_strides[2],
+                      const int64_t v_strides[2], const int64_t kv_strides[3], int table_dtype, int dtype, void* stream);
+
+/* Attention of every sequence's new tokens over its pages (their keys and values appended before): beside
+ * b200_attn_decode and b200_attn_prefill, for decoding sequences, chunks of prompts and both in one batch.
+ *   sequence b: tokens q_start[b] .. q_start[b+1] - 1, at most max_q; kv_len[b] keys with them; key j lies in page
+ *   page_table[b * table_stride + j / page_size].  Token i of T sees the keys up to its own position p = kv_len[b] - T + i, with
+ *   window > 0 only the last `window` of them (p included).  A token without any key gives zeros.
+ *   q: element strides (token, head); out [n_tokens, Hq, D]; rows behind the last sequence are left as they were.
+ * head_dim 64 or 128, f16 / bf16, up to 128 query heads per KV head, page_size a multiple of 16.  Page ids outside the
+ * cache read as zeros; table entries of pages without an attended key are not looked at, and what lies in pages behind
+ * kv_len or ahead of the window does not matter, whatever it is.  Probabilities are rounded to the activation type for the second product.
+ * workspace: 16-byte aligned, b200_attn_paged_workspace_bytes bytes of any content; calls that may overlap need one each. */
+int b200_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* q_start,
+                    const int32_t* kv_len, const int32_t* page_table, int64_t B, int64_t n_tokens, int64_t max_q,
+                    int Hq, int Hkv, int D, int64_t num_pages, int page_size, int64_t table_stride,
+                    const int64_t q_strides[2], const int64_t kv_strides[3], int64_t window, float scale, int dtype,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+int64_t b200_attn_paged_workspace_bytes(int64_t max_q, int Hq, int Hkv, int D);
+
+/* One token per row of logits (f32, f16, bf16), drawn with the given random numbers: beside b200_argmax_rows.
+ * Per row r: temperature[r] (<= 0: the arg-max), top_k[r] (<= 0: off), top_p[r] (>= 1: off), min_p[r] (<= 0: off), uniform[r] in
+ * [0, 1); NULL: temperature 1, filter off.  With w = exp((x - max) / temperature), tokens ordered by x, of equal ones the lower
+ * index first: top-k keeps the first k; top-p of those the ones before which less than top_p of their sum lies (always the
+ * first); min-p those with w >= min(min_p, 1).  out[r] = the first index at which the sum of what is kept, taken in the
+ * order of the indices, passes uniform[r] times the whole.  Weights are whole multiples of 2^-40 (what weighs less is never
+ * drawn), so the result depends on the row and its numbers alone; NaN counts as -infinity, a row of nothing else gives 0.
+ * At most 4194304 columns and 65535 rows. */
+int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, int64_t cols, int64_t row_stride, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

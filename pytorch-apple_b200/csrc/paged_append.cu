@@ -1,0 +1,115 @@
+// Keys and values of a step's new tokens -> pages of the KV cache, with the position rotation of queries and keys on the way:
+//   x'[d] = x[d] cos[d] - x[d + D/2] sin[d],   x'[d + D/2] = x[d + D/2] cos[d + D/2] + x[d] sin[d + D/2]     (d < D/2)
+// in fp32 with one rounding, to the activation type.  (The rotation of the static-cache path rounds both products too, because
+// the unfused graph that it replaces does; this one replaces nothing, and the errors would be twice as large.)
+//
+// One thread per 8 dims of both halves of a (token, head): everything it reads it has read before it writes, so queries may be
+// rotated in place.  Bound by launch latency for a decode step, by memory for a long prompt.
+#include "common.cuh"
+
+namespace b200 {
+
+namespace {
+
+struct AppendParams {
+  const void* x[3];      // q, k, v: [token, head, D], D contiguous
+  int64_t xs[3][2];      // element strides over (token, head)
+  const void *cos_t, *sin_t;
+  void *q_out, *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t N, n_slots;
+  int64_t ps[3];         // element strides of the pages over (page, head, row)
+  int Hq, Hkv, D, page_size, table_dtype;
+};
+
+__device__ __forceinline__ void load_table(const void* t, int64_t i, int dtype, float (&f)[8]) {
+  if (dtype == B200_F32) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(t) + i)), b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(t) + i) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else if (dtype == B200_BF16) {
+    unpack8<__nv_bfloat16>(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(t) + i)), f);
+  } else {
+    unpack8<__half>(__ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(t) + i)), f);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant__ AppendParams p) {
+  const int hp = p.D >> 4, H = p.Hq + 2 * p.Hkv;   // pairs of packs per head
+  const int64_t gid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = gid / hp;
+  const int pk = static_cast<int>(gid - row * hp);
+  const int64_t n = row / H;
+  if (n >= p.N) return;
+  int h = static_cast<int>(row - n * H);
+  const int which = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);
+  if (which == 1) h -= p.Hq;
+  if (which == 2) h -= p.Hq + p.Hkv;
+  T* dst;
+  if (which == 0) {
+    dst = static_cast<T*>(p.q_out) + (n * p.Hq + h) * p.D;
+  } else {
+    const int64_t slot = __ldg(p.slots + n);
+    if (slot < 0 || slot >= p.n_slots) return;   // a row of padding
+    const int64_t page = slot / p.page_size, r = slot - page * p.page_size;
+    dst = static_cast<T*>(which == 1 ? p.k_pages : p.v_pages) + page * p.ps[0] + h * p.ps[1] + r * p.ps[2];
+  }
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x[which]) + n * p.xs[which][0] + h * p.xs[which][1]);
+  uint4 lo = src[pk], hi = src[pk + hp];
+  if (which != 2 && p.cos_t) {
+    float a[8], b[8], c[8], s[8], o[8];
+    unpack8<T>(lo, a);
+    unpack8<T>(hi, b);
+    const int64_t t = n * p.D + pk * 8;
+    load_table(p.cos_t, t, p.table_dtype, c);
+    load_table(p.sin_t, t, p.table_dtype, s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = a[k] * c[k] - b[k] * s[k];
+    lo = pack8<T>(o);
+    load_table(p.cos_t, t + (p.D >> 1), p.table_dtype, c);
+    load_table(p.sin_t, t + (p.D >> 1), p.table_dtype, s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = b[k] * c[k] + a[k] * s[k];
+    hi = pack8<T>(o);
+  }
+  reinterpret_cast<uint4*>(dst)[pk] = lo;
+  reinterpret_cast<uint4*>(dst)[pk + hp] = hi;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_paged_append(const void* q, const void* k, const void* v, const void* cos_t, const void* sin_t, void* q_out, void* k_pages,
+                                 void* v_pages, const int64_t* slots, int64_t n_tokens, int Hq, int Hkv, int D, int64_t num_pages, int page_size,
+                                 const int64_t q_strides[2], const int64_t k_strides[2], const int64_t v_strides[2], const int64_t kv_strides[3],
+                                 int table_dtype, int dtype, void* stream) {
+  B200_CHECK_ARG(k && v && k_pages && v_pages && slots && k_strides && v_strides && kv_strides && n_tokens >= 0 && Hq >= 0 && Hkv > 0 && num_pages > 0 &&
+                 page_size > 0, "b200_paged_append: bad arguments");
+  B200_CHECK_ARG(Hq == 0 || (q && q_out && q_strides), "b200_paged_append: query heads without queries, their strides or a place for them");
+  B200_CHECK_ARG(!cos_t == !sin_t, "b200_paged_append: cos and sin tables come together");
+  B200_CHECK_ARG(D > 0 && D % 16 == 0, "b200_paged_append: head_dim %d is not a multiple of 16", D);
+  if (cos_t && table_dtype != B200_F32 && table_dtype != dtype)
+    B200_FAIL(B200_ENOTSUP, "b200_paged_append: tables are f32 or of the activation type (got dtype %d)", table_dtype);
+  bool ok = aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages) && aligned16(cos_t) && aligned16(sin_t);
+  AppendParams p;
+  p.x[0] = q; p.x[1] = k; p.x[2] = v;
+  if (Hq > 0) ok = ok && aligned16(q) && aligned16(q_out);
+  for (int i = 0; i < 2; ++i) {
+    p.xs[0][i] = Hq > 0 ? q_strides[i] : 0; p.xs[1][i] = k_strides[i]; p.xs[2][i] = v_strides[i];
+    ok = ok && p.xs[0][i] % 8 == 0 && p.xs[1][i] % 8 == 0 && p.xs[2][i] % 8 == 0;
+  }
+  for (int i = 0; i < 3; ++i) { p.ps[i] = kv_strides[i]; ok = ok && kv_strides[i] % 8 == 0; }
+  if (!ok) B200_FAIL(B200_EALIGN, "b200_paged_append: operands must be 16-byte aligned with strides multiple of 8");
+  if (n_tokens == 0) return B200_OK;
+  p.cos_t = cos_t; p.sin_t = sin_t; p.q_out = q_out; p.k_pages = k_pages; p.v_pages = v_pages; p.slots = slots;
+  p.N = n_tokens; p.n_slots = num_pages * page_size; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.page_size = page_size; p.table_dtype = table_dtype;
+  const int64_t blocks = ceil_div(n_tokens * (Hq + 2 * static_cast<int64_t>(Hkv)) * (D >> 4), 128);
+  if (blocks >= (1ll << 31)) B200_FAIL(B200_ELIMIT, "b200_paged_append: too many tokens");
+  B200_DISPATCH_HALF(dtype, T, { launch_pdl(paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, static_cast<cudaStream_t>(stream), p); });
+  B200_CHECK_LAUNCH("paged_append_kernel");
+  return B200_OK;
+}

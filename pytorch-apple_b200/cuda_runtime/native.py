@@ -86,6 +86,10 @@ SIGNATURES = {
     "b200_attn_prefill_reads_tiles": (_i, [_vp, _i64, _i64, _i64, _i]),
     "b200_mask_tiles": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp]),
     "b200_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i64, _i, _I64P, _I64P, _I64P, _i64, _i64, _f, _i, _vp]),
+    "b200_paged_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _i, _I64P, _I64P, _I64P, _I64P, _i, _i, _vp]),
+    "b200_attn_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _i64, _i, _i64, _I64P, _I64P, _i64, _f, _i, _vp, _i64, _vp]),
+    "b200_attn_paged_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
+    "b200_sample_rows": (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
 }
 
 _lib = None

@@ -167,10 +167,11 @@ class QwenSession:
         m = np.where(j <= i, 0.0, neg).astype(np.float32).astype(np_dt)
         return np.ascontiguousarray(np.broadcast_to(m[None, None], (batch, 1, q_len, kv_len)))
 
-    def prefill(self, input_ids: np.ndarray, prompt_len: int | None = None) -> np.ndarray:
+    def prefill(self, input_ids: np.ndarray, prompt_len: int | None = None, sampler=None) -> np.ndarray:
         """Run the prompt; returns the first generated token per sequence ``[B, 1]``.  ``prompt_len``
         (<= the graph's length) is the number of real tokens when the ids are right-padded, as the
-        reference pads prompts to its fixed prefill length (examples/run_qwen.py:100-118)."""
+        reference pads prompts to its fixed prefill length (examples/run_qwen.py:100-118).  ``sampler``
+        (``sampling.Sampler``) draws the token instead of taking the arg-max."""
         B, T = self.batch, self.prompt_len
         n = T if prompt_len is None else int(prompt_len)
         ids = np.ascontiguousarray(input_ids, dtype=np.int64).reshape(B, T)
@@ -179,14 +180,22 @@ class QwenSession:
                 "cache_position": np.arange(T, dtype=np.int64)}
         out = self._pre.execute(feed)
         self.kv = hand_off_kv(out, self.mapping, self.decode_ir, self.backend, valid_rows=n)
+        if sampler is not None:
+            self.position = n
+            return self._draw(sampler, out[self.prefill_ir["graph_outputs"][0]["name"]], n - 1)
         if self._argmax_prefill is None:
             self._argmax_prefill = self._argmax_executor(B, T)
         tokens = self._argmax_prefill.execute({"logits": out[self.prefill_ir["graph_outputs"][0]["name"]]})["token"].to_numpy()
         self.position = n
         return tokens[:, n - 1:n].astype(np.int64)
 
-    def step(self, token_ids: np.ndarray) -> np.ndarray:
-        """Decode one token for each sequence at the current position; returns the next ids ``[B, 1]``."""
+    def _draw(self, sampler, logits, row: int) -> np.ndarray:
+        """Tokens ``[B, 1]`` drawn from row ``row`` of a device buffer of logits ``[B, T, vocab]``."""
+        return sampler(logits.native_handle.reshape(self.batch, -1, self.vocab)[:, row]).cpu().numpy().reshape(self.batch, 1)
+
+    def step(self, token_ids: np.ndarray, sampler=None) -> np.ndarray:
+        """Decode one token for each sequence at the current position; returns the next ids ``[B, 1]`` (drawn where there is a
+        ``sampler``, else the arg-max)."""
         if self.position >= self.cache_len:
             raise RuntimeError(f"the KV cache holds {self.cache_len} rows; position {self.position} does not fit")
         B, pos = self.batch, self.position
@@ -198,13 +207,15 @@ class QwenSession:
         self.kv = dict(zip(self._kv_in, [out[n] for n in self._kv_out]))
         self.last_logits = out[self._logits_name]
         self.position += 1
+        if sampler is not None:
+            return self._draw(sampler, self.last_logits, 0)
         return self._argmax.execute({"logits": self.last_logits})["token"].to_numpy().reshape(B, 1)
 
-    def generate(self, input_ids: np.ndarray, max_new_tokens: int, prompt_len: int | None = None) -> np.ndarray:
-        """``[B, max_new_tokens]`` greedy continuation of the prompt."""
-        tok = self.prefill(input_ids, prompt_len)
+    def generate(self, input_ids: np.ndarray, max_new_tokens: int, prompt_len: int | None = None, sampler=None) -> np.ndarray:
+        """``[B, max_new_tokens]`` continuation of the prompt, greedy or drawn by ``sampler``."""
+        tok = self.prefill(input_ids, prompt_len, sampler)
         toks = [tok]
         for _ in range(max_new_tokens - 1):
-            tok = self.step(tok)
+            tok = self.step(tok, sampler)
             toks.append(tok)
         return np.concatenate(toks, axis=1)

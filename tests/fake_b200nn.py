@@ -175,6 +175,29 @@ class FakeLibrary:
         _flat(out, 4, rows).copy_(X.argmax(-1))
         return 0
 
+    def b200_sample_rows(self, logits, out, rows, cols, row_stride, temperature, top_k, top_p, min_p, uniform, dtype, stream):
+        self.calls.append("sample_rows")
+        X = _raw(logits, _DT[dtype], [rows, cols], [row_stride, 1]).double()
+        X = torch.where(X.isnan(), torch.full_like(X, -math.inf), X)
+        row = lambda ptr, code, off: _flat(ptr, code, rows).double() if _addr(ptr) else torch.full([rows], off, dtype=torch.float64)
+        T, K, P, MP, U = row(temperature, 0, 1.0), row(top_k, 3, 0.0), row(top_p, 0, 1.0), row(min_p, 0, 0.0), row(uniform, 0, 0.0)
+        for r in range(rows):
+            top, order = torch.sort(X[r], descending=True, stable=True)
+            if not T[r] > 0 or top[0] == -math.inf:
+                _flat(out, 4, rows)[r] = order[0] if top[0] > -math.inf else 0
+                continue
+            w = torch.where(top == top[0], torch.ones_like(top), torch.exp((top - top[0]) / T[r]))
+            n = min(int(K[r]), cols) if K[r] > 0 else cols
+            if P[r] < 1:
+                before = w[:n].cumsum(0) - w[:n]
+                n = max(1, int((before < P[r] * w[:n].sum()).sum()))
+            keep = order[:n][w[:n] >= min(float(MP[r]), 1.0)]
+            by_index = torch.zeros_like(w).scatter_(0, order, w)
+            keep = keep.sort().values
+            sums = by_index[keep].cumsum(0)
+            _flat(out, 4, rows)[r] = keep[min(len(keep) - 1, int((sums <= U[r] * sums[-1]).sum()))]
+        return 0
+
     # -- indexing ---------------------------------------------------------------------
     def b200_embedding(self, table, ids, out, n_ids, vocab, row_bytes, ids_dtype, stream):
         self.calls.append("embedding")
@@ -419,6 +442,48 @@ class FakeLibrary:
         M = _raw(mask, dt, [B, 1, 1, S], [mask_bs, 0, 0, 1]).float() if _addr(mask) else None
         o = self._attn(Q, K, Vv, M, scale, dt)
         _raw(out, dt, [B, Hq, D], [Hq * D, D, 1]).copy_(o[:, :, 0, :].to(dt))
+        return 0
+
+    def b200_attn_paged_workspace_bytes(self, max_q, Hq, Hkv, D):
+        return 256
+
+    def b200_attn_paged(self, q, kp, vp, out, q_start, kv_len, table, B, N, max_q, Hq, Hkv, D, num_pages, page, table_stride, qs, ks, window, scale, dtype,
+                        ws, ws_bytes, stream):
+        self.calls.append("attn_paged")
+        dt = _DT[dtype]
+        Q, O = _raw(q, dt, [N, Hq, D], [*qs, 1]), _raw(out, dt, [N, Hq, D], [Hq * D, D, 1])
+        K, Vv = (_raw(p, dt, [num_pages, Hkv, page, D], [*ks, 1]) for p in (kp, vp))
+        start, lens, tab = _flat(q_start, 3, B + 1), _flat(kv_len, 3, B), _raw(table, torch.int32, [B, table_stride], [table_stride, 1])
+        for b in range(B):
+            s, T, n = int(start[b]), int(start[b + 1] - start[b]), int(lens[b])
+            for i in range(T):
+                p = n - T + i
+                j = torch.arange(max(0, p - window + 1) if window else 0, p + 1)
+                if len(j) == 0:
+                    O[s + i] = 0
+                    continue
+                pages = tab[b][j // page].long()
+                k, v = K[pages, :, j % page].float(), Vv[pages, :, j % page].float()   # [keys, Hkv, D]
+                O[s + i] = self._attn(Q[s + i].float()[None, :, None], k.transpose(0, 1)[None], v.transpose(0, 1)[None], None, scale, dt)[0, :, 0].to(dt)
+        return 0
+
+    def b200_paged_append(self, q, k, v, cos_t, sin_t, q_out, kp, vp, slots, N, Hq, Hkv, D, num_pages, page, qs, ks, vs, ps, table_dtype, dtype, stream):
+        self.calls.append("paged_append")
+        dt, half = _DT[dtype], D // 2
+        table = [_raw(t, _DT[table_dtype], [N, 1, D], [D, D, 1]).float() for t in (cos_t, sin_t)] if _addr(cos_t) else None
+
+        def rotate(x):
+            if table is None:
+                return x
+            f = x.float()
+            return (f * table[0] + torch.cat([-f[..., half:], f[..., :half]], -1) * table[1]).to(dt)
+
+        slot = _flat(slots, 4, N)
+        if Hq:
+            _raw(q_out, dt, [N, Hq, D], [Hq * D, D, 1]).copy_(rotate(_raw(q, dt, [N, Hq, D], [*qs, 1])))
+        there = (slot >= 0) & (slot < num_pages * page)
+        for pages, x in ((kp, rotate(_raw(k, dt, [N, Hkv, D], [*ks, 1]))), (vp, _raw(v, dt, [N, Hkv, D], [*vs, 1]))):
+            _raw(pages, dt, [num_pages, Hkv, page, D], [*ps, 1])[slot[there] // page, :, slot[there] % page] = x[there]
         return 0
 
     def b200_attn_prefill(self, q, k, v, mask, out, B, Hq, Hkv, T, S, D, qs, ks, vs, mask_b, mask_t, scale, dtype, stream):
