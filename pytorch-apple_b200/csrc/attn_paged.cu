@@ -1,5 +1,9 @@
-// Attention of every sequence's new tokens over the pages of its KV cache.
+// Attention of every sequence's new tokens over the pages of its KV cache: the kernel for few rows per KV head (decoding sequences, a few
+// drafted tokens), the one that joins partial results, and the entry point.  Chunks and prompts: attn_paged_tc5.cu.
 #include "attn_paged.cuh"
+#include "gemm_tc5.cuh"
+#include "mma.cuh"
+#include "tc5.cuh"
 
 namespace b200 {
 
@@ -7,9 +11,396 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// One warp per (token, query head), one key at a time.
+// ===========================================================================
+// Few rows: up to 8 NT rows (tokens times query heads) share each KV head.  The problem is transposed so that the rows lie on the
+// 8-wide side of the m16n8k16 MMA (mma.sync: at 4 flop per byte and row this is bound by memory):
+//   S^T[16 keys x 8 rows] = K[16 x D] Q^T,   O^T[D x 8 rows] += V^T[D x 16] P^T.
+// A block of eight warps walks through its pieces (attn_paged.cuh) with a warp per 16 keys; every warp has a ring of its own
+// in shared memory, filled by TMA (one box of 16 rows of a page each for K and V, 128-byte swizzle), so that nothing in the loop
+// waits for another warp.  At the end of a piece each warp parks its accumulators in the ring stage that it has just read (which is
+// refilled afterwards; the others are on their way meanwhile) and the block adds them up.
+// ===========================================================================
+constexpr int FEW_WARPS = 8, FEW_KEYS = 16;
+constexpr int FEW_OV = 4;          // what an item costs besides its 16-key blocks, in blocks
+constexpr int FEW_MIN_SHARE = 16;  // blocks (and OVs) of a CTA at least
+constexpr float FEW_STEP = 8.f;    // the stored maximum follows the true one when that has grown by more (log2)
+constexpr int FEW_RING = 24576;    // bytes of a warp's ring
+
+__device__ int g_few_error = 0;    // left by a bounded wait that ran out
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1)
+    attn_paged_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedParams p, const int tpt) {
+  constexpr int BLOCK = 2 * FEW_KEYS * D * 2, HALF = BLOCK / 2, STAGES = FEW_RING / BLOCK;   // 16 keys of K and of V
+  constexpr int ROWS = 8 * NT, KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ __align__(8) uint64_t full[FEW_WARPS][STAGES];
+  __shared__ __align__(16) PagedPiece s_piece[PAGED_MAX_PIECES];
+  __shared__ int s_first[PAGED_MAX_PIECES + 1];   // blocks ahead of each piece of the list
+  __shared__ float s_m[FEW_WARPS][ROWS], s_l[FEW_WARPS][ROWS];
+  __shared__ int s_park[FEW_WARPS];               // where a warp has parked its accumulators (ring stage, -1: it has none)
+  __shared__ int64_t s_next, s_total[FEW_WARPS];
+  __shared__ int s_count;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
+  uint8_t* const ring = smem + warp * FEW_RING;
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) tc5::mbar_init(&full[warp][s], 1);
+    tc5::fence_barrier_init();
+  }
+  if (threadIdx.x == 0) { tc5::prefetch_tensormap(&map_k); tc5::prefetch_tensormap(&map_v); }
+  pdl_trigger();
+  pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
+  int64_t* const pre = reinterpret_cast<int64_t*>(smem);   // (nothing has been copied into the rings yet)
+  int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, pre, s_total);
+  const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > FEW_MIN_SHARE ? even : FEW_MIN_SHARE;
+  int64_t u0 = cta * share;
+  const int64_t u1 = u0 + share < total ? u0 + share : total;
+  int4 head = make_int4(0, 0, 0, 0);
+  const float sl = p.scale * LOG2E;
+  uint32_t phase = 0;   // parity of each stage's next completion
+  int st = 0;           // stage of the next block to be read
+  uint32_t patience = 1u << 22;
+
+  // ldmatrix: lane supplies one row address of 8x8 matrix (lane >> 3); a panel holds 64 dims of 16 rows, chunk c of row r at c ^ (r & 7)
+  const int mi = lane >> 3, mr = lane & 7;
+  const uint32_t ring_addr = smem_u32(ring);
+  const uint32_t k_row = (8 * (mi & 1) + mr) * 128, v_row = (8 * (mi >> 1) + mr) * 128;
+
+  while (u0 < u1) {
+    if (warp == 0) {
+      int count;
+      const int64_t next = paged_pieces<FEW_KEYS, FEW_OV>(p, tpt, pre, u0, u1, share, s_piece, count, head);
+      __syncwarp();
+      if (lane == 0) {
+        s_next = next;
+        s_count = count;
+        int run = 0;
+        for (int f = 0; f < count; ++f) { s_first[f] = run; run += s_piece[f].cnt; }
+        s_first[count] = run;
+      }
+    }
+    __syncthreads();
+    const int F = s_count, X = s_first[F];
+    u0 = s_next;
+
+    // Copies: block x of the list is warp x % 8's; its page and row are looked up 32 blocks ahead, one per lane
+    int id_page = 0, id_row = 0, id_hk = 0, next_page = 0, next_row = 0, next_hk = 0;
+    auto look = [&](int x, int& page, int& row, int& hk) {
+      page = row = hk = 0;
+      if (x < X) {
+        int f = 0;
+        while (x >= s_first[f + 1]) ++f;
+        const int key = (s_piece[f].j0 + x - s_first[f]) * FEW_KEYS, i = key / p.page_size;
+        row = key - i * p.page_size;
+        hk = s_piece[f].hk;
+        const int hi = s_piece[f].p0 + s_piece[f].rows / p.G;
+        page = key < hi ? __ldg(p.table + s_piece[f].b * p.table_stride + i) : -1;   // (an item without keys has no page either)
+        if (page < 0 || page >= p.num_pages) page = static_cast<int>(p.num_pages);   // outside the tensor: zeros
+      }
+    };
+    int x_copy = warp, st_copy = st;   // next block to be copied, and into which stage
+    auto copy = [&]() {
+      const int i = (x_copy / FEW_WARPS) & 31;
+      if (i == 0 && x_copy >= FEW_WARPS * 32) { id_page = next_page; id_row = next_row; id_hk = next_hk; }
+      if (i == 0) look(x_copy + FEW_WARPS * (32 + lane), next_page, next_row, next_hk);
+      const int page = __shfl_sync(0xffffffffu, id_page, i), row = __shfl_sync(0xffffffffu, id_row, i), hk = __shfl_sync(0xffffffffu, id_hk, i);
+      if (lane == 0 && x_copy < X) {
+        uint64_t* const bar = &full[warp][st_copy];
+        tc5::mbar_arrive_expect_tx(bar, BLOCK);
+        tc5::tma_load_5d(ring + st_copy * BLOCK, &map_k, bar, 0, row, 0, hk, page);
+        tc5::tma_load_5d(ring + st_copy * BLOCK + HALF, &map_v, bar, 0, row, 0, hk, page);
+      }
+      x_copy += FEW_WARPS;
+      st_copy = st_copy + 1 == STAGES ? 0 : st_copy + 1;
+    };
+    look(warp + FEW_WARPS * lane, id_page, id_row, id_hk);
+    tc5::fence_proxy_async();
+    __syncthreads();   // (the running costs lie in the rings: everybody is through with them)
+    for (int s = 0; s < STAGES; ++s) copy();
+
+    int x = warp;   // this warp's next block
+#pragma unroll 1
+    for (int f = 0; f < F; ++f) {
+      const PagedPiece c = s_piece[f];
+      const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
+      const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
+      const int x_end = s_first[f + 1], key_base = (c.j0 - s_first[f]) * FEW_KEYS;
+      float m[NT][2], l[NT][2], o[KS][NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.f;
+      int parked = -1;
+      if (x < x_end) {
+        // rows 8 j + 2 t, + 1 are this lane's columns of S^T; their keys end before see and begin at from
+        int see[NT][2], from[NT][2], see_min = hi, from_max = lo;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * j + 2 * t + e;
+            see[j][e] = r < c.rows ? c.p0 + r / p.G + 1 : hi;
+            from[j][e] = p.window > 0 && see[j][e] - p.window > 0 ? static_cast<int>(see[j][e] - p.window) : 0;
+            see_min = min(see_min, see[j][e]);
+            from_max = max(from_max, from[j][e]);
+          }
+        // Q^T fragments: row 8 j + g, dims 16 ks + 2 t, +1 and 16 ks + 2 t + 8, +9
+        uint32_t qf[KS][NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int r = 8 * j + g;
+          const T* qr = static_cast<const T*>(p.q) + (static_cast<int64_t>(c.token) + r / p.G) * p.qs[0] + (c.hk * p.G + r % p.G) * p.qs[1] + 2 * t;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            qf[ks][j][0] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks) : 0u;
+            qf[ks][j][1] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8) : 0u;
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) o[ks][j][0] = o[ks][j][1] = o[ks][j][2] = o[ks][j][3] = 0.f;
+
+#pragma unroll 1
+        while (true) {
+          const int key0 = key_base + x * FEW_KEYS;
+          const uint32_t sk = ring_addr + st * BLOCK, sv = sk + HALF;
+          if (!tc5::mbar_wait(&full[warp][st], (phase >> st) & 1u, patience)) {   // (a copy that never comes: the result is void, nothing hangs)
+            patience = 1u << 10;
+            if (lane == 0) atomicExch(&g_few_error, 60);
+          }
+          phase ^= 1u << st;
+          if (key0 + FEW_KEYS > hi || key0 < lo) {   // clear the rows of V that no row sees
+            const int row = lane >> 1, key = key0 + row;
+            if (key >= hi || key < lo) {
+              uint4* const v = reinterpret_cast<uint4*>(ring + st * BLOCK + HALF + (D == 128 ? (lane & 1) * 2048 + row * 128 : row * 128 + (lane & 1) * 64));
+#pragma unroll
+              for (int e = 0; e < D / 16; ++e) v[e] = make_uint4(0, 0, 0, 0);
+            }
+            tc5::fence_proxy_async();   // before the stage is copied into again
+            __syncwarp();
+          }
+          // ---- S^T = K Q^T (two accumulators halve the dependent chain) ----
+          float sa[NT][4], sb[NT][4];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sa[j][e] = sb[j][e] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ks += 2) {
+            uint32_t a0[4], a1[4];
+            ldmatrix_x4(a0, sk + (ks >> 2) * 2048 + k_row + (((2 * (ks & 3) + (mi >> 1)) ^ mr) << 4));
+            ldmatrix_x4(a1, sk + (ks >> 2) * 2048 + k_row + (((2 * (ks & 3) + 2 + (mi >> 1)) ^ mr) << 4));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              MmaType<T>::mma(sa[j], a0, qf[ks][j]);
+              MmaType<T>::mma(sb[j], a1, qf[ks + 1][j]);
+            }
+          }
+          float v[NT][4];   // keys g (0, 1) and g + 8 (2, 3) x rows 8 j + 2 t (0, 2) and + 1 (1, 3)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = (sa[j][e] + sb[j][e]) * sl;
+          if (key0 + FEW_KEYS > see_min || key0 < from_max) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = key0 + g + (e >> 1) * 8;
+                if (key >= see[j][e & 1] || key < from[j][e & 1]) v[j][e] = -INFINITY;
+              }
+          }
+          // ---- the running maximum moves only when some score has outgrown it ----
+          bool grown = false;
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) grown = grown || v[j][e] > m[j][e & 1] + FEW_STEP || (m[j][e & 1] == -INFINITY && v[j][e] > -INFINITY);
+          if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              float mx[2] = {fmaxf(v[j][0], v[j][2]), fmaxf(v[j][1], v[j][3])};
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) {
+                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float mn = fmaxf(m[j][e], mx[e]), f_ = ex2_approx(m[j][e] - (mn == -INFINITY ? 0.f : mn));
+                m[j][e] = mn;
+                l[j][e] *= f_;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) { o[ks][j][e] *= f_; o[ks][j][e + 2] *= f_; }
+              }
+            }
+          }
+          // ---- O^T += V^T P^T ----
+          uint32_t pb[NT][2];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const float u0_ = m[j][0] == -INFINITY ? 0.f : m[j][0], u1_ = m[j][1] == -INFINITY ? 0.f : m[j][1];
+            const float p0 = ex2_approx(v[j][0] - u0_), p1 = ex2_approx(v[j][1] - u1_), p2 = ex2_approx(v[j][2] - u0_), p3 = ex2_approx(v[j][3] - u1_);
+            l[j][0] += p0 + p2;
+            l[j][1] += p1 + p3;
+            pb[j][0] = movmatrix_trans(pack2<T>(p0, p1));
+            pb[j][1] = movmatrix_trans(pack2<T>(p2, p3));
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(a, sv + (ks >> 2) * 2048 + v_row + (((2 * (ks & 3) + (mi & 1)) ^ mr) << 4));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) MmaType<T>::mma(o[ks][j], a, pb[j]);
+          }
+          __syncwarp();   // every lane has read the stage
+          x += FEW_WARPS;
+          const int was = st;
+          st = st + 1 == STAGES ? 0 : st + 1;
+          if (x >= x_end) { parked = was; break; }
+          copy();
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            l[j][0] += __shfl_xor_sync(0xffffffffu, l[j][0], off);
+            l[j][1] += __shfl_xor_sync(0xffffffffu, l[j][1], off);
+          }
+        // [row][D] floats, dim d of row r at d ^ (r's 2 t and j) * 8: lanes that differ in t store to other banks
+        float* const slab = reinterpret_cast<float*>(ring + parked * BLOCK);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 8 * j + 2 * t + (e & 1);
+              slab[r * D + ((16 * ks + g + (e >> 1) * 8) ^ (t << 3))] = o[ks][j][e];
+            }
+        if (g == 0) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { s_m[warp][8 * j + 2 * t + e] = m[j][e]; s_l[warp][8 * j + 2 * t + e] = l[j][e]; }
+        }
+      }
+      if (lane == 0) s_park[warp] = parked;
+      __syncthreads();
+      // ---- the block's sums: a thread per dim, the rows dealt to FEW_WARPS * 32 / D of them ----
+      {
+        const int d = threadIdx.x % D;
+        const bool whole = c.flags == 3;
+        const int64_t slot = paged_slot(cta, c.flags & 1, ROWS);
+        for (int r = threadIdx.x / D; r < c.rows; r += FEW_WARPS * 32 / D) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < FEW_WARPS; ++w)
+            if (s_park[w] >= 0) top = fmaxf(top, s_m[w][r]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          float acc = 0.f, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < FEW_WARPS; ++w)
+            if (s_park[w] >= 0) {
+              const float f_ = ex2_approx(s_m[w][r] - ref);
+              acc += reinterpret_cast<const float*>(smem + w * FEW_RING + s_park[w] * BLOCK)[r * D + (d ^ (((r & 7) >> 1) << 3))] * f_;
+              sum += s_l[w][r] * f_;
+            }
+          if (whole) {   // (a row without keys gives zeros)
+            static_cast<T*>(p.out)[((static_cast<int64_t>(c.token) + r / p.G) * p.Hq + c.hk * p.G + r % p.G) * D + d] = from_f32<T>(sum > 0.f ? acc / sum : 0.f);
+          } else {
+            p.acc[(slot + r) * D + d] = acc;
+            if (d == 0) p.ml[slot + r] = make_float2(top, sum);
+          }
+        }
+      }
+      tc5::fence_proxy_async();   // what was parked, ahead of the copies into the same stages
+      __syncthreads();
+      if (parked >= 0) copy();
+    }
+    if (u0 < u1) total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, pre, s_total);   // (the rings lay over the running costs)
+  }
+  if (threadIdx.x == 0) p.head[cta] = head;
+}
+
+// ===========================================================================
+// Joins the pieces of items that several blocks had a part in, in the order of the blocks.  RB rows of an item at a time, a thread per four dims;
+// every block goes through the list of such items (at most one begins in each block of the kernel before).
+// ===========================================================================
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int RB = 256 / (D / 4);
+  __shared__ int s_upto[PAGED_CTAS + 1], s_sum[8];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int4 h = make_int4(0, 0, 0, 0);
+  if (threadIdx.x < PAGED_CTAS) h = __ldg(p.head + threadIdx.x);
+  const int mine = h.x > 0 ? (h.w + RB - 1) / RB : 0;   // tasks of this item
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) s_sum[warp] = upto;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += s_sum[w];
+  if (threadIdx.x < PAGED_CTAS) s_upto[threadIdx.x + 1] = upto;
+  if (threadIdx.x == 0) s_upto[0] = 0;
+  __syncthreads();
+  const int tasks = s_upto[PAGED_CTAS];
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    int lo = 0, hi = PAGED_CTAS;   // the item: the last one whose tasks begin at or before this one
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_upto[mid] <= task) lo = mid; else hi = mid;
+    }
+    const int4 it = __ldg(p.head + lo);
+    const int r = (task - s_upto[lo]) * RB + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    if (r >= it.w) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int BATCH = 8;
+    for (int i0 = 0; i0 < it.x; i0 += BATCH) {
+      float2 ml[BATCH];
+      float4 a[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + i < it.x) {
+          const int64_t slot = paged_slot(lo + i0 + i, i0 + i == 0, ROWS) + r;
+          ml[i] = __ldg(p.ml + slot);
+          a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float c = ex2_approx(m - ref);
+      l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float f = ex2_approx(ml[i].x - ref);
+        l += ml[i].y * f;
+        acc.x += a[i].x * f; acc.y += a[i].y * f; acc.z += a[i].z * f; acc.w += a[i].w * f;
+      }
+      m = top;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T* const o = static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D + d;
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  }
+}
+
+// ===========================================================================
+// Where the tensor-core kernels are switched off (or a tensor map cannot be made): one warp per (token, query head), one key at a time.
+// ===========================================================================
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_paged_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(128) attn_paged_plain_kernel(const __grid_constant__ PagedParams p) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), n = w / p.Hq;
@@ -49,13 +440,61 @@ __global__ void __launch_bounds__(128) attn_paged_kernel(const __grid_constant__
   for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l > 0.f ? o[e] / l : 0.f);
 }
 
+template <typename T, int D, int NT> int launch_few(const PagedParams& p, int dtype, cudaStream_t st) {
+  constexpr int smem = FEW_WARPS * FEW_RING + 1024;
+  static PerDevice<bool> configured_on;
+  bool* configured = configured_on.slot();
+  if (!configured) return B200_ENOTSUP;
+  if (!*configured) {
+    if (cudaFuncSetAttribute(attn_paged_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+      cudaGetLastError();
+      return B200_ENOTSUP;
+    }
+    *configured = true;
+  }
+  CUtensorMap mk, mv;
+  auto bytes = [](int64_t elems) { return elems > 0 ? static_cast<uint64_t>(elems) * 2 : static_cast<uint64_t>(D) * 2; };   // (0: an axis of length one)
+  const uint64_t dims[5] = {64, static_cast<uint64_t>(p.page_size), D / 64, static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.num_pages)};
+  const uint64_t str[4] = {bytes(p.ks[2]), 128, bytes(p.ks[1]), bytes(p.ks[0])};
+  const uint32_t box[5] = {64, FEW_KEYS, D / 64, 1, 1};
+  if (!tma_encode_sw128(&mk, dtype, 5, p.k_pages, dims, str, box) || !tma_encode_sw128(&mv, dtype, 5, p.v_pages, dims, str, box)) return B200_ENOTSUP;
+  return launch_pdl(attn_paged_few_kernel<T, D, NT>, dim3(PAGED_CTAS), dim3(FEW_WARPS * 32), smem, st, mk, mv, p, 8 * NT / p.G) == cudaSuccess ? B200_OK : B200_ELAUNCH;
+}
+
+// rows per KV head of the kernel that takes a call
+int rows_of(int64_t max_q, int G) {
+  if (G <= 8 && max_q * G <= 8) return 8;
+  if (G <= 16 && max_q * G <= 16) return 16;
+  return PAGED_TC5_ROWS;
+}
+
+int64_t workspace_parts(int rows, int D, int64_t* ml, int64_t* acc) {   // byte offsets of the arrays; returns the size
+  *ml = PAGED_CTAS * 16;
+  *acc = *ml + static_cast<int64_t>(PAGED_CTAS) * 2 * rows * 8;
+  return *acc + static_cast<int64_t>(PAGED_CTAS) * 2 * rows * D * 4;
+}
+
 }  // namespace
+
+int attn_paged_error(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_few_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_few_error, &zero, sizeof(int));
+  }
+  const int other = attn_paged_tc5_error(clear);
+  return v ? v : other;
+}
+
 }  // namespace b200
 
 using namespace b200;
 
 extern "C" int64_t b200_attn_paged_workspace_bytes(int64_t max_q, int Hq, int Hkv, int D) {
-  return 0;
+  if (max_q <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
+  int64_t ml, acc;
+  return workspace_parts(rows_of(max_q, Hq / Hkv), D, &ml, &acc);
 }
 
 extern "C" int b200_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* q_start, const int32_t* kv_len,
@@ -67,21 +506,51 @@ extern "C" int b200_attn_paged(const void* q, const void* k_pages, const void* v
   B200_CHECK_ARG(D == 64 || D == 128, "b200_attn_paged: head_dim %d not supported (64 and 128 only)", D);
   B200_CHECK_ARG(Hq % Hkv == 0 && Hq / Hkv <= 128, "b200_attn_paged: query heads per KV head must divide and be <= 128");
   B200_CHECK_ARG(page_size > 0 && page_size % 16 == 0, "b200_attn_paged: page size %d is not a multiple of 16", page_size);
-  if (!(table_stride * page_size < (1ll << 31) && n_tokens < (1ll << 31) && B < (1ll << 31)))
-    B200_FAIL(B200_ELIMIT, "b200_attn_paged: more than 2^31 - 1 tokens, sequences or keys of a sequence");
-  bool ok = aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out);
+  if (!(table_stride < (1ll << 30) && table_stride * page_size < (1ll << 30) && n_tokens * Hq < (1ll << 31) && B <= PAGED_MAX_SEQS))
+    B200_FAIL(B200_ELIMIT, "b200_attn_paged: more than %d sequences, 2^30 keys of one or 2^31 rows of queries", PAGED_MAX_SEQS);
+  bool ok = aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace);
   PagedParams p;
   for (int i = 0; i < 2; ++i) { p.qs[i] = q_strides[i]; ok = ok && q_strides[i] % 8 == 0 && q_strides[i] >= 0; }
   for (int i = 0; i < 3; ++i) { p.ks[i] = kv_strides[i]; ok = ok && kv_strides[i] % 8 == 0 && kv_strides[i] >= 0; }
   if (!ok) B200_FAIL(B200_EALIGN, "b200_attn_paged: operands must be 16-byte aligned with strides multiple of 8");
+  if (dtype != B200_BF16 && dtype != B200_F16) B200_FAIL(B200_ENOTSUP, "b200_attn_paged: dtype %d is not f16/bf16", dtype);
   if (B == 0 || n_tokens == 0 || max_q == 0) return B200_OK;
+  const int G = Hq / Hkv, rows = rows_of(max_q, G);
+  int64_t ml, acc;
+  const int64_t need = workspace_parts(rows, D, &ml, &acc);
+  if (!workspace || workspace_bytes < need)
+    B200_FAIL(B200_EINVAL, "b200_attn_paged: workspace of %lld bytes required (got %lld)", (long long)need, (long long)workspace_bytes);
   p.q = q; p.k_pages = k_pages; p.v_pages = v_pages; p.out = out; p.q_start = q_start; p.kv_len = kv_len; p.table = page_table;
-  p.B = B; p.N = n_tokens; p.num_pages = num_pages; p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.page_size = page_size;
+  p.B = B; p.N = n_tokens; p.num_pages = num_pages; p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.page_size = page_size;
   p.window = window; p.scale = scale;
-  const unsigned grid = static_cast<unsigned>(ceil_div(n_tokens * Hq, 4));
-  B200_DISPATCH_HALF(dtype, T, {
-    launch_pdl(D == 128 ? attn_paged_kernel<T, 128> : attn_paged_kernel<T, 64>, dim3(grid), dim3(128), 0, static_cast<cudaStream_t>(stream), p);
-  });
-  B200_CHECK_LAUNCH("attn_paged_kernel");
+  p.head = static_cast<int4*>(workspace);
+  p.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + ml);
+  p.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + acc);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = B200_ENOTSUP;
+  if (tc5_enabled()) {
+    if (rows == PAGED_TC5_ROWS) {
+      rc = attn_paged_tc5(p, D, dtype, st);
+    } else {
+      B200_DISPATCH_HALF(dtype, T, {
+        rc = rows == 8 ? (D == 128 ? launch_few<T, 128, 1>(p, dtype, st) : launch_few<T, 64, 1>(p, dtype, st))
+                       : (D == 128 ? launch_few<T, 128, 2>(p, dtype, st) : launch_few<T, 64, 2>(p, dtype, st));
+      });
+    }
+  }
+  if (rc == B200_ENOTSUP) {
+    B200_DISPATCH_HALF(dtype, T, {
+      launch_pdl(D == 128 ? attn_paged_plain_kernel<T, 128> : attn_paged_plain_kernel<T, 64>, dim3(static_cast<unsigned>(ceil_div(n_tokens * Hq, 4))),
+                 dim3(128), 0, st, p);
+    });
+  } else {
+    B200_DISPATCH_HALF(dtype, T, {
+      const auto merge = [&](auto kernel, int blocks) { launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p); };
+      if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8>, PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 8>, PAGED_CTAS); }
+      else if (rows == 16) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 16>, 2 * PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 16>, 2 * PAGED_CTAS); }
+      else { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 128>, 8 * PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 128>, 8 * PAGED_CTAS); }
+    });
+  }
+  B200_CHECK_LAUNCH("attn_paged");
   return B200_OK;
 }

@@ -1,4 +1,4 @@
-// Shared between the kernels of attention over a paged KV cache.
+// Shared between the kernels of attention over a paged KV cache: arguments, how the work is dealt to blocks, and the partial results.
 #pragma once
 #include "common.cuh"
 
@@ -13,7 +13,15 @@ struct PagedParams {
   int Hq, Hkv, G, page_size;
   int64_t window;                  // keys a token sees back from its own (0: all)
   float scale;
+  // partial results (paged_workspace)
+  int4* head;                      // [PAGED_CTAS]: {pieces, first token, KV head, rows} of the item that begins in a block and ends in a later one
+  float2* ml;                      // [PAGED_CTAS][2][rows]: (maximum in the log2 domain, sum)
+  float* acc;                      // [PAGED_CTAS][2][rows][D]
 };
+
+constexpr int PAGED_CTAS = 148;        // blocks that share the work (fixed, so that the workspace does not depend on the device)
+constexpr int PAGED_MAX_SEQS = 4096;   // of a call: their running costs are kept in shared memory
+constexpr int PAGED_MAX_PIECES = 32;   // of a block at a time
 
 // A sequence's first token, how many it has and how many keys.  What the device arrays hold is cut to what the buffers hold, so that
 // no value in them leads outside a buffer.
@@ -26,5 +34,159 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int64_t b) {
   n = n < 0 ? 0 : n > room ? room : n;
   return {lo, static_cast<int>(hi - lo), n};
 }
+
+// ---- how the work is dealt out --------------------------------------------------------------------------------
+// An item is (sequence, KV head, tile of `tpt` tokens): the tokens' G query heads of that KV head are the rows of one tile, row = token * G + head, so
+// that keys and values are read once for all of them.  It costs its key tiles of KT keys plus OV for what it does once.  All items, one behind
+// the other, are cut into equal ranges, one per block; a block's piece of an item that it does not have alone becomes a partial
+// result.  Lengths are read on the device (a captured call follows them), every block works the cuts out for itself, and sequences
+// of any lengths load all blocks alike.
+struct PagedPiece {
+  int32_t b, hk, token, rows;   // sequence, KV head, first token (index into q), rows = tokens * G
+  int32_t p0, j0, cnt, flags;   // position of the first token, first key tile and number of them, 1: the item begins here, 2: it ends here
+};
+
+struct PagedTile { int t0, t1, j0, cnt; int64_t p0; };
+template <int KT> __device__ __forceinline__ PagedTile paged_tile(const PagedParams& p, int T, int64_t n, int i, int tpt) {
+  PagedTile t;
+  t.t0 = i * tpt;
+  t.t1 = min(T, t.t0 + tpt);
+  t.p0 = n - T + t.t0;
+  const int64_t hi = n - T + t.t1, lo = p.window > 0 && t.p0 - p.window + 1 > 0 ? t.p0 - p.window + 1 : 0;
+  t.j0 = hi > lo ? static_cast<int>(lo / KT) : 0;
+  t.cnt = hi > lo ? static_cast<int>((hi + KT - 1) / KT) - t.j0 : 1;   // no key: one tile in which everything is masked
+  return t;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// pre[b] = cost of the sequences before b, b = 0..B (shared memory); returns pre[B].  All THREADS threads; ends with a barrier.
+template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const PagedParams& p, int tpt, int64_t* pre, int64_t* warp_total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = static_cast<int>(p.B);
+  const int chunk = (B + THREADS - 1) / THREADS;
+  int64_t run = 0;
+  for (int c = 0; c < chunk; ++c) {
+    const int b = threadIdx.x * chunk + c;
+    PagedSeq s = {0, 0, 0};
+    if (b < B) s = paged_seq(p, b);
+    const int tiles = (s.T + tpt - 1) / tpt;
+    int64_t cost = 0;
+    if (tiles <= 2)
+      for (int i = 0; i < tiles; ++i) cost += paged_tile<KT>(p, s.T, s.n, i, tpt).cnt + OV;
+    // a prompt's many tiles: the whole warp adds them up
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 2); many; many &= many - 1) {
+      const int src = __ffs(many) - 1, T = __shfl_sync(0xffffffffu, s.T, src), nt = (T + tpt - 1) / tpt;
+      const int64_t n = __shfl_sync(0xffffffffu, s.n, src);
+      int64_t sum = 0;
+      for (int i = lane; i < nt; i += 32) sum += paged_tile<KT>(p, T, n, i, tpt).cnt + OV;
+      sum = warp_sum64(sum);
+      if (lane == src) cost = sum;
+    }
+    run += cost * p.Hkv;
+    if (b < B) pre[b + 1] = run;
+  }
+  int64_t upto = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) warp_total[warp] = upto;
+  __syncthreads();
+  int64_t before = upto - run, total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_total[w];
+    total += warp_total[w];
+  }
+  for (int c = 0; c < chunk; ++c) {
+    const int b = threadIdx.x * chunk + c;
+    if (b < B) pre[b + 1] += before;
+  }
+  if (threadIdx.x == 0) pre[0] = 0;
+  __syncthreads();
+  return total;
+}
+
+// The pieces of items in the costs [u0, u1), at most PAGED_MAX_PIECES; returns where to go on (u1: that was all).  One whole warp.
+// head is written where an item begins in this block and does not end in it: how many blocks have pieces of it, and whose rows they are.
+template <int KT, int OV>
+__device__ int64_t paged_pieces(const PagedParams& p, int tpt, const int64_t* pre, int64_t u0, int64_t u1, int64_t share, PagedPiece* list, int& count, int4& head) {
+  const int lane = threadIdx.x & 31, B = static_cast<int>(p.B);
+  count = 0;
+  int lo = 0, hi = B;   // the last sequence that begins at or before u0 (and so is not empty)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u0) lo = mid; else hi = mid;
+  }
+  for (int b = lo; b < B && pre[b] < u1; ++b) {
+    if (pre[b + 1] <= u0 || pre[b + 1] == pre[b]) continue;
+    const PagedSeq s = paged_seq(p, b);
+    const int tiles = (s.T + tpt - 1) / tpt;
+    const int64_t per_head = (pre[b + 1] - pre[b]) / p.Hkv;
+    const int64_t skip = u0 > pre[b] ? (u0 - pre[b]) / per_head : 0;
+    int64_t base = pre[b] + skip * per_head;
+    const int64_t items = static_cast<int64_t>(p.Hkv) * tiles;
+    for (int64_t e0 = skip * tiles; e0 < items && base < u1; e0 += 32) {
+      const int64_t e = e0 + lane;
+      PagedTile t = {0, 0, 0, 0, 0};
+      if (e < items) t = paged_tile<KT>(p, s.T, s.n, static_cast<int>(e % tiles), tpt);
+      const int64_t cost = e < items ? t.cnt + OV : 0;
+      int64_t upto = cost;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const int64_t start = base + upto - cost + OV, end = base + upto, a = max(u0, start), z = min(u1, end);
+      const unsigned mine = __ballot_sync(0xffffffffu, e < items && a < z);
+      const int at = count + __popc(mine & ((1u << lane) - 1u));
+      const bool taken = ((mine >> lane) & 1u) && at < PAGED_MAX_PIECES;
+      if (taken) {
+        PagedPiece f;
+        f.b = b;
+        f.hk = static_cast<int>(e / tiles);
+        f.token = static_cast<int>(s.first) + t.t0;
+        f.rows = (t.t1 - t.t0) * p.G;
+        f.p0 = static_cast<int>(t.p0);
+        f.j0 = t.j0 + static_cast<int>(a - start);
+        f.cnt = static_cast<int>(z - a);
+        f.flags = (a == start ? 1 : 0) | (z == end ? 2 : 0);
+        list[at] = f;
+      }
+      // (at most one per block, and the last of its pieces)
+      const unsigned opens = __ballot_sync(0xffffffffu, taken && a == start && z < end);
+      if (opens) {
+        const int src = __ffs(opens) - 1;
+        head.x = __shfl_sync(0xffffffffu, static_cast<int>((end - 1) / share - start / share) + 1, src);
+        head.y = __shfl_sync(0xffffffffu, static_cast<int>(s.first) + t.t0, src);
+        head.z = __shfl_sync(0xffffffffu, static_cast<int>(e / tiles), src);
+        head.w = __shfl_sync(0xffffffffu, (t.t1 - t.t0) * p.G, src);
+      }
+      count += __popc(mine);
+      if (count > PAGED_MAX_PIECES) {   // go on behind the last one taken
+        const unsigned last = __ballot_sync(0xffffffffu, taken && at == PAGED_MAX_PIECES - 1);
+        count = PAGED_MAX_PIECES;
+        return last ? __shfl_sync(0xffffffffu, z, __ffs(last) - 1) : base;   // (none of this round was taken: they begin at base or later)
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  return u1;
+}
+
+// Where a piece's partial result goes: slot 1 for the one that an item begins with, slot 0 for the others.
+__device__ __forceinline__ int64_t paged_slot(int cta, bool begins, int rows_max) { return (static_cast<int64_t>(cta) * 2 + (begins ? 1 : 0)) * rows_max; }
+
+// tcgen05 kernel (attn_paged_tc5.cu); B200_ENOTSUP where a tensor map cannot be made
+int attn_paged_tc5(const PagedParams& p, int D, int dtype, cudaStream_t stream);
+int attn_paged_tc5_error(bool clear);
+// code left by a bounded wait of either kernel that ran out (0 = none); optionally cleared
+int attn_paged_error(bool clear);
+
+constexpr int PAGED_TC5_ROWS = 128;
 
 }  // namespace b200

@@ -1,0 +1,436 @@
+// Attention over a paged KV cache on the 5th-generation tensor cores (tcgen05.mma, accumulators in tensor memory, operands by TMA): chunks
+// of prompts, whole prompts, and batches in which some sequences decode.
+//
+// The rows of a tile are up to 128 / G tokens times the G query heads that share a KV head (row = token * G + head), so that a key tile is
+// fetched once for all of them; one TMA box per 64 dims brings them in that order.  Keys and values come in tiles of 128 keys, one box per
+// piece of a page (the largest power of two that divides the page size, at most 128 rows), through rings of two stages each.
+// What is attended follows from positions alone: a tile that reaches past a row's last key or ahead of its window is masked in
+// registers, rows of V that no row of the tile may see are cleared in shared memory (0 times what lies there need not be 0).
+//
+// Within a tile as in the attention over static prompts: two groups of four softmax warps share a tile, group g on its keys
+// 64 g .. 64 g + 63 with running maxima and an accumulator of its own, one thread per row; the stored maximum follows the true one when that
+// has grown by more than RESCALE_STEP.  A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
+// next item's first tile are computed while the last one's rows are written.
+//
+// Warp roles: warps 0-3 and 4-7 the softmax groups, warp 8 MMA issuer and owner of the tensor memory, warp 9 TMA producer, a box per lane.  Every
+// barrier wait is bounded; on a time-out the block records a code, stops issuing, waits for its copies, frees its tensor memory and returns.
+#include "attn_paged.cuh"
+#include "gemm_tc5.cuh"
+#include "tc5.cuh"
+
+namespace b200 {
+
+__device__ int g_attn_paged_error = 0;
+
+namespace {
+
+constexpr int BKV = 128;
+constexpr int PANEL = 128 * 128;               // [128 rows][128 bytes]: 64 columns of an operand tile
+constexpr int THREADS = 320;
+constexpr int OV = 1;                          // what an item costs besides its tiles, in tiles
+constexpr int MIN_SHARE = 2;                   // tiles (and OVs) of a block at least
+constexpr float LOG2E_F = 1.4426950408889634f;
+constexpr float RESCALE_STEP = 8.f;
+constexpr int TMEM_COLS = 512;                 // two buffers of S (128 columns each), O of both groups
+
+template <typename T> struct Fmt;
+template <> struct Fmt<__half> { static constexpr int value = 0; };
+template <> struct Fmt<__nv_bfloat16> { static constexpr int value = 1; };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc5::smem_addr(bar)) : "memory");
+}
+
+constexpr int smem_bytes(int D) { return (5 * (D / 64) + 4) * PANEL + 1024; }   // Q, K x 2, V x 2, P x 2 (two panels each), alignment
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+    attn_paged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          const __grid_constant__ PagedParams p, const int tpt, const int box) {
+  constexpr int NP = D / 64, TILE = NP * PANEL;   // panels and bytes of a K, V or Q tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_s = smem;
+  uint8_t* k_s = smem + TILE;
+  uint8_t* v_s = smem + 3 * TILE;
+  uint8_t* p_s = smem + 5 * TILE;
+  // tile n of the block lives in stage / buffer n & 1
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ __align__(16) PagedPiece s_piece[PAGED_MAX_PIECES];
+  __shared__ int64_t s_next, s_total[THREADS / 32];
+  __shared__ int s_count, failed;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+  if (warp == 9 && lane == 0) {
+    failed = 0;
+    tc5::mbar_init(&q_full, 1);
+    tc5::mbar_init(&q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      tc5::mbar_init(&k_full[s], 1);
+      tc5::mbar_init(&k_empty[s], 1);
+      tc5::mbar_init(&v_full[s], 1);
+      tc5::mbar_init(&v_empty[s], 1);
+      tc5::mbar_init(&s_full[s], 1);
+      tc5::mbar_init(&p_ready[s], 256);
+      tc5::mbar_init(&o_full[s], 1);
+    }
+    tc5::fence_barrier_init();
+    tc5::prefetch_tensormap(&map_q);
+    tc5::prefetch_tensormap(&map_k);
+    tc5::prefetch_tensormap(&map_v);
+  }
+  if (warp == 8) { tc5::tmem_alloc(&tmem_holder, TMEM_COLS); tc5::tmem_relinquish(); }
+  pdl_trigger();
+  pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
+  int64_t* const pre = reinterpret_cast<int64_t*>(p_s);
+  tc5::tc_fence_before();
+  int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, pre, s_total);
+  tc5::tc_fence_after();
+  const uint32_t tmem_base = tmem_holder;
+  const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > MIN_SHARE ? even : MIN_SHARE;
+  int64_t u0 = cta * share;
+  const int64_t u1 = u0 + share < total ? u0 + share : total;
+  int4 head = make_int4(0, 0, 0, 0);
+  int n = 0, fg = 0;   // tiles and pieces behind this block, the same in every role
+
+  while (u0 < u1) {
+    if (warp == 0) {
+      int count;
+      const int64_t next = paged_pieces<BKV, OV>(p, tpt, pre, u0, u1, share, s_piece, count, head);
+      if (lane == 0) { s_next = next; s_count = count; }
+    }
+    __syncthreads();
+    const int F = s_count;
+    u0 = s_next;
+
+    if (warp == 9) {   // ---- TMA producer: lane l brings rows [l * box, (l + 1) * box) of a tile ----
+      bool ok = true;
+      int q_at = fg, kv_at = n;   // copies issued
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        bool got = tc5::mbar_wait(bar, parity);
+        got = __all_sync(0xffffffffu, got) && !*reinterpret_cast<volatile int*>(&failed);
+        if (!got && lane == 0 && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, code); }
+        return __all_sync(0xffffffffu, got);
+      };
+      int at = n;
+      for (int f = 0; f < F && ok; ++f) {
+        const PagedPiece c = s_piece[f];
+        const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
+        const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
+        const int32_t* const pages = p.table + c.b * p.table_stride;
+        for (int k = 0; k < c.cnt && ok; ++k, ++at) {
+          const int st = at & 1, key = (c.j0 + k) * BKV + lane * box;
+          const bool there = lane * box < BKV && key < hi && key + box > lo;
+          const unsigned present = __ballot_sync(0xffffffffu, there);
+          int page = 0, row = 0;
+          if (there) {
+            const int i = key / p.page_size;
+            row = key - i * p.page_size;
+            page = __ldg(pages + i);
+            if (page < 0 || page >= p.num_pages) page = static_cast<int>(p.num_pages);   // outside the tensor: zeros
+          }
+          const uint32_t bytes = static_cast<uint32_t>(__popc(present)) * box * 128 * NP, parity = ((at >> 1) & 1) ^ 1;
+          if (at >= 2 && !(ok = wait(&k_empty[st], parity, 50))) break;
+          if (k == 0) {
+            if (fg + f >= 1 && !(ok = wait(&q_empty, (fg + f - 1) & 1, 51))) break;
+            if (lane == 0) {
+              tc5::mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.G) * tpt * 128 * NP);
+              for (int h = 0; h < NP; ++h) tc5::tma_load_4d(q_s + h * PANEL, &map_q, &q_full, 0, c.hk * p.G, c.token, h);
+            }
+            ++q_at;
+          }
+          if (lane == 0) tc5::mbar_arrive_expect_tx(&k_full[st], bytes);
+          __syncwarp();
+          if (there)
+            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(k_s + st * TILE + h * PANEL + lane * box * 128, &map_k, &k_full[st], 0, row, h, c.hk, page);
+          if (at >= 2 && !(ok = wait(&v_empty[st], parity, 52))) {
+            tc5::mbar_wait(&k_full[st], (at >> 1) & 1, 1u << 16);   // the copies just issued
+            break;
+          }
+          if (lane == 0) tc5::mbar_arrive_expect_tx(&v_full[st], bytes);
+          __syncwarp();
+          if (there)
+            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(v_s + st * TILE + h * PANEL + lane * box * 128, &map_v, &v_full[st], 0, row, h, c.hk, page);
+          kv_at = at + 1;
+        }
+      }
+      // on a failure elsewhere the copies in flight must land before the block leaves
+      if (*reinterpret_cast<volatile int*>(&failed)) {
+        if (q_at > 0) tc5::mbar_wait(&q_full, (q_at - 1) & 1, 1u << 16);
+        for (int i = kv_at > 2 ? kv_at - 2 : 0; i < kv_at; ++i) {
+          tc5::mbar_wait(&k_full[i & 1], (i >> 1) & 1, 1u << 16);
+          tc5::mbar_wait(&v_full[i & 1], (i >> 1) & 1, 1u << 16);
+        }
+      }
+    } else if (warp == 8) {
+      if (lane == 0) {   // ---- MMA issuer ----
+        constexpr uint32_t idesc_s = tc5::umma_idesc(128, BKV, Fmt<T>::value);
+        constexpr uint32_t idesc_o = tc5::umma_idesc(128, D, Fmt<T>::value) | (1u << 16);   // B operand MN-major
+        const uint32_t q_lo = tc5::desc_sw128_lo(tc5::smem_addr(q_s));
+        bool ok = true;
+        // scores run up to two tiles ahead of the products with V: (sf, sk) is the next tile whose scores are to be issued
+        int sf = 0, sk = 0, sn = n;
+        auto issue_s = [&](bool look) {   // look: the K tile has not been looked for by the softmax threads
+          const int st = sn & 1;
+          if (sk == 0 && !tc5::mbar_wait(&q_full, (fg + sf) & 1)) return false;
+          if (look && !tc5::mbar_wait(&k_full[st], (sn >> 1) & 1)) return false;
+          tc5::tc_fence_after();
+          const uint32_t k_lo = tc5::desc_sw128_lo(tc5::smem_addr(k_s + st * TILE));
+#pragma unroll
+          for (int h = 0; h < NP; ++h) tc5::umma_f16_kblock(tmem_base + 128 * st, q_lo + h * (PANEL >> 4), k_lo + h * (PANEL >> 4), idesc_s, h > 0);
+          tc5::umma_commit(&s_full[st]);
+          tc5::umma_commit(&k_empty[st]);
+          if (++sk == s_piece[sf].cnt) {
+            tc5::umma_commit(&q_empty);
+            ++sf;
+            sk = 0;
+          }
+          ++sn;
+          return true;
+        };
+        for (int i = 0; i < 2 && ok && sf < F; ++i) ok = issue_s(true);
+        int at = n;
+        for (int f = 0; f < F && ok; ++f) {
+          const int cnt = s_piece[f].cnt;
+          for (int k = 0; k < cnt && ok; ++k, ++at) {
+            const int st = at & 1;
+            const uint32_t v_addr = tc5::smem_addr(v_s + st * TILE), p_addr = tc5::smem_addr(p_s + st * 2 * PANEL);
+            if (!(ok = tc5::mbar_wait(&p_ready[st], (at >> 1) & 1))) break;
+            tc5::tc_fence_after();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {     // 16 keys per instruction = two 8-key groups of the V panels
+              const uint64_t da = tc5::umma_desc_sw128(p_addr + (e >> 2) * PANEL) + 2 * (e & 3);
+              const uint64_t db = tc5::umma_desc_sw128_mn(v_addr + e * 2048, PANEL, 1024);
+              tc5::umma_f16(tmem_base + 256 + 128 * (e >> 2), da, db, idesc_o, k > 0 || (e & 3) != 0);
+            }
+            tc5::umma_commit(&o_full[st]);
+            tc5::umma_commit(&v_empty[st]);
+            if (sf < F) ok = issue_s(false);
+          }
+        }
+        if (!ok && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, 53); }
+      }
+      __syncwarp();
+    } else {
+      // ---- softmax: one thread per row and group, group g on keys 64 g .. of a tile ----
+      const int g = warp >> 2, quarter = warp & 3;
+      const int r = 32 * quarter + lane;   // the tensor-memory lane this thread may read
+      const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(32 * quarter) << 16);
+      const uint32_t t_o = t_lane + 256 + 128 * g;
+      const float c = p.scale * LOG2E_F;   // scores in the log2 domain
+      bool alive = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+        bool got = tc5::mbar_try_wait(bar, parity);
+        if (!__all_sync(0xffffffffu, got)) got = __all_sync(0xffffffffu, tc5::mbar_wait(bar, parity));
+        if (!got && lane == 0 && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, code); }
+        return got;
+      };
+      int at = n, left = 0;   // tiles of this list still to come
+      for (int f = 0; f < F; ++f) left += s_piece[f].cnt;
+#pragma unroll 1
+      for (int f = 0; f < F; ++f) {   // (a thread that has given up still meets the others at the end of every piece)
+        const PagedPiece pc = s_piece[f];
+        const int tokens = pc.rows / p.G;
+        const bool row_live = r < pc.rows, warp_live = 32 * quarter < pc.rows;
+        const int see = row_live ? pc.p0 + r / p.G + 1 : 0;   // keys from here on this row does not see
+        const int from = p.window > 0 && see - p.window > 0 ? static_cast<int>(see - p.window) : 0;   // nor those ahead of this one
+        const int hi = pc.p0 + tokens, lo = p.window > 0 && pc.p0 - p.window + 1 > 0 ? static_cast<int>(pc.p0 - p.window + 1) : 0;   // nor any row
+        float m_run = -INFINITY, l_run = 0.f;   // maximum that the row's sums are relative to, sum of the probabilities
+#pragma unroll 1
+        for (int k = 0; k < pc.cnt && alive; ++k, ++at, --left) {
+          const int st = at & 1, key0 = (pc.j0 + k) * BKV;
+          uint8_t* const p_own = p_s + st * 2 * PANEL + g * PANEL + r * 128;
+          // S of this tile: its barrier also says that every product issued before it, that of this buffer's last probabilities among them, is complete
+          if (!wait_all(&s_full[st], (at >> 1) & 1, 54)) { alive = false; break; }
+          tc5::tc_fence_after();
+          if (warp_live) {
+            float u[64];
+            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g, *reinterpret_cast<float(*)[32]>(&u[0]));
+            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g + 32, *reinterpret_cast<float(*)[32]>(&u[32]));
+            tc5::tmem_ld_wait();
+            float to_log2 = c;
+            if (c <= 0.f) {   // (with the factor left for later the maximum would be the minimum, and 0 times a masked key's -infinity no number)
+#pragma unroll
+              for (int e = 0; e < 64; e += 2) tc5::mul2(u[e], u[e + 1], c);
+              to_log2 = 1.f;
+            }
+            const int end = see - key0 - 64 * g, begin = from - key0 - 64 * g;
+            if (end < 64 || begin > 0) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (e >= end || e < begin) u[e] = -INFINITY;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(u[e + 2 * q], u[e + 2 * q + 1]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+            const bool moved = top > m_run + RESCALE_STEP || (m_run == -INFINITY && top > m_run);
+            const float m_new = moved ? top : m_run;
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            if (k > 0 && __any_sync(0xffffffffu, moved)) {   // rescale this warp's rows, once the product before has finished
+              if (!wait_all(&o_full[st ^ 1], ((at - 1) >> 1) & 1, 55)) { alive = false; break; }
+              const float alpha = moved ? ex2(m_run - m_use) : 1.f;   // 0 for the first maximum of a row
+              tc5::tc_fence_after();
+#pragma unroll 1
+              for (int q = 0; q < D; q += 16) {
+                float t[16];
+                tc5::tmem_ld_32x16(t_o + q, t);
+                tc5::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) tc5::mul2(t[e], t[e + 1], alpha);
+                tc5::tmem_st_32x16(t_o + q, t);
+              }
+              tc5::tmem_st_wait();
+              l_run *= alpha;
+            }
+            m_run = m_new;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              float pr[8];
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) {
+                float a = u[8 * q + e], d = u[8 * q + e + 1];
+                tc5::fma2(a, d, to_log2, -m_use, -m_use);
+                pr[e] = ex2(a);
+                pr[e + 1] = ex2(d);
+                tc5::add2(sum[e & 2], sum[(e & 2) + 1], pr[e], pr[e + 1]);
+              }
+              *reinterpret_cast<uint4*>(p_own + ((q ^ (r & 7)) << 4)) = pack8<T>(pr);
+            }
+            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          }
+          if (key0 + BKV > hi || key0 < lo) {   // clear the rows of V that no row sees
+            if (!wait_all(&v_full[st], (at >> 1) & 1, 56)) { alive = false; break; }
+            const int row = threadIdx.x >> 1, half = threadIdx.x & 1, key = key0 + row;
+            if (key >= hi || key < lo) {
+              uint8_t* const at_v = v_s + st * TILE + (NP == 2 ? half * PANEL + row * 128 : row * 128 + half * 64);
+#pragma unroll
+              for (int e = 0; e < 4 * NP; ++e) reinterpret_cast<uint4*>(at_v)[e] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          tc5::fence_proxy_async();   // the probabilities are read by the tensor core (async proxy)
+          tc5::tc_fence_before();     // this thread's tcgen05.ld / st are complete before S and O are touched again
+          // what the products of this tile and the scores of the one after next read has landed: looked for by one warp per group
+          if (quarter == 0) {
+            if (g == 0 ? !wait_all(&v_full[st], (at >> 1) & 1, 57) : left > 2 && !wait_all(&k_full[st], ((at + 2) >> 1) & 1, 58)) { alive = false; break; }
+          }
+          mbar_arrive1(&p_ready[st]);
+        }
+        // ---- the piece's rows: the half of the head dimension that this group writes, from both accumulators ----
+        if (alive) alive = wait_all(&o_full[(at - 1) & 1], ((at - 1) >> 1) & 1, 59);
+        float* const ml = reinterpret_cast<float*>(p_s + g * PANEL);   // (the probabilities have been read)
+        ml[r] = m_run;
+        ml[128 + r] = l_run;
+        tc5::tc_fence_before();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        tc5::tc_fence_after();
+        const float *ml_0 = reinterpret_cast<const float*>(p_s) + r, *ml_1 = reinterpret_cast<const float*>(p_s + PANEL) + r;
+        const float m_0 = ml_0[0], m_1 = ml_1[0], l_0 = ml_0[128], l_1 = ml_1[128];
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (alive && warp_live) {
+          const float m_all = fmaxf(m_0, m_1), m_ref = m_all == -INFINITY ? 0.f : m_all;
+          float w_0 = ex2(m_0 - m_ref), w_1 = ex2(m_1 - m_ref);
+          const float l_all = l_0 * w_0 + l_1 * w_1;
+          const bool whole = pc.flags == 3;
+          if (whole) {
+            const float inv = l_all > 0.f ? 1.f / l_all : 0.f;   // a row without keys gives zeros
+            w_0 *= inv;
+            w_1 *= inv;
+          }
+          const int64_t slot = paged_slot(cta, pc.flags & 1, PAGED_TC5_ROWS) + r;
+          float* const part = p.acc + slot * D + g * (D / 2);
+          T* const orow = static_cast<T*>(p.out) + ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
+          if (!whole && g == 0 && row_live) p.ml[slot] = make_float2(m_all, l_all);
+#pragma unroll 1
+          for (int q = 0; q < D / 2; q += 16) {
+            float t0[16], t1[16];
+            tc5::tmem_ld_32x16(t_lane + 256 + g * (D / 2) + q, t0);
+            tc5::tmem_ld_32x16(t_lane + 384 + g * (D / 2) + q, t1);
+            tc5::tmem_ld_wait();
+            float o[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(t1[e], w_1, t0[e] * w_0);
+            if (row_live) {
+              if (whole) {
+                reinterpret_cast<uint4*>(orow + q)[0] = pack8<T>(*reinterpret_cast<float(*)[8]>(&o[0]));
+                reinterpret_cast<uint4*>(orow + q)[1] = pack8<T>(*reinterpret_cast<float(*)[8]>(&o[8]));
+              } else {
+                tc5::st_global_f8(part + q, o);
+                tc5::st_global_f8(part + q + 8, o + 8);
+              }
+            }
+          }
+          tc5::tc_fence_before();
+        }
+      }
+    }
+    for (int f = 0; f < F; ++f) n += s_piece[f].cnt;
+    fg += F;
+    if (__syncthreads_or(*reinterpret_cast<volatile int*>(&failed))) break;   // (what the threads see may differ: they agree)
+    if (u0 < u1) total = paged_prefix<BKV, OV, THREADS>(p, tpt, pre, s_total);   // (the probabilities lay over the running costs)
+  }
+  if (threadIdx.x == 0) p.head[cta] = head;
+  tc5::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) { tc5::tc_fence_after(); tc5::tmem_dealloc(tmem_base, TMEM_COLS); }
+}
+
+template <typename T, int D> int launch(const PagedParams& p, int dtype, cudaStream_t st) {
+  static PerDevice<bool> configured_on;
+  bool* configured = configured_on.slot();
+  if (!configured) return B200_ENOTSUP;
+  if (!*configured) {
+    if (cudaFuncSetAttribute(attn_paged_tc5_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D)) != cudaSuccess) {
+      cudaGetLastError();
+      return B200_ENOTSUP;
+    }
+    *configured = true;
+  }
+  const int tpt = 128 / p.G;
+  int box = 16;
+  while (box < 128 && p.page_size % (2 * box) == 0) box *= 2;
+  CUtensorMap mq, mk, mv;
+  auto bytes = [](int64_t elems) { return elems > 0 ? static_cast<uint64_t>(elems) * 2 : static_cast<uint64_t>(D) * 2; };   // (0: an axis of length one)
+  {
+    const uint64_t dims[4] = {64, static_cast<uint64_t>(p.Hq), static_cast<uint64_t>(p.N), D / 64};
+    const uint64_t str[3] = {bytes(p.qs[1]), bytes(p.qs[0]), 128};
+    const uint32_t b[4] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(tpt), 1};
+    if (!tma_encode_sw128(&mq, dtype, 4, p.q, dims, str, b)) return B200_ENOTSUP;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[5] = {64, static_cast<uint64_t>(p.page_size), D / 64, static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.num_pages)};
+    const uint64_t str[4] = {bytes(p.ks[2]), 128, bytes(p.ks[1]), bytes(p.ks[0])};
+    const uint32_t b[5] = {64, static_cast<uint32_t>(box), 1, 1, 1};
+    if (!tma_encode_sw128(i ? &mv : &mk, dtype, 5, i ? p.v_pages : p.k_pages, dims, str, b)) return B200_ENOTSUP;
+  }
+  return launch_pdl(attn_paged_tc5_kernel<T, D>, dim3(PAGED_CTAS), dim3(THREADS), smem_bytes(D), st, mq, mk, mv, p, tpt, box) == cudaSuccess ? B200_OK : B200_ELAUNCH;
+}
+
+}  // namespace
+
+int attn_paged_tc5_error(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_paged_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_attn_paged_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+int attn_paged_tc5(const PagedParams& p, int D, int dtype, cudaStream_t st) {
+  if (p.num_pages >= (1ll << 31) - 1) return B200_ENOTSUP;
+  if (dtype == B200_BF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, dtype, st) : launch<__nv_bfloat16, 64>(p, dtype, st);
+  return D == 128 ? launch<__half, 128>(p, dtype, st) : launch<__half, 64>(p, dtype, st);
+}
+
+}  // namespace b200

@@ -11,6 +11,7 @@
 // apply the epilogue in fp32 and store.  Every barrier wait is bounded: on a timeout the
 // CTA records an error code in `g_tc5_error`, drains its own copies and exits.
 #include "attention.cuh"
+#include "attn_paged.cuh"
 #include "gemm_epilogue.cuh"
 #include "tc5.cuh"
 
@@ -1904,8 +1905,8 @@ extern "C" int b200_debug_device_error(int* code, int clear) {
   cudaError_t e = cudaMemcpyFromSymbol(&v, b200::g_tc5_error, sizeof(int));
   if (e != cudaSuccess) B200_FAIL(B200_ELAUNCH, "b200_debug_device_error: %s", cudaGetErrorString(e));
   const int att = b200::attn_prefill_tc5_error(clear != 0), stem = b200::conv_stem_error(clear != 0),
-            rows = b200::conv_rows_error(clear != 0), pair = b200::gemm_pair_error(clear != 0);
-  if (code) *code = v ? v : att > 0 ? att : stem > 0 ? stem : rows > 0 ? rows : pair > 0 ? pair : 0;
+            rows = b200::conv_rows_error(clear != 0), pair = b200::gemm_pair_error(clear != 0), paged = b200::attn_paged_error(clear != 0);
+  if (code) *code = v ? v : att > 0 ? att : stem > 0 ? stem : rows > 0 ? rows : pair > 0 ? pair : paged > 0 ? paged : 0;
   if (clear && v) {
     v = 0;
     cudaMemcpyToSymbol(b200::g_tc5_error, &v, sizeof(int));
