@@ -426,6 +426,7 @@ int b200_attn_prefill_reads_tiles(const void* mask, int64_t S, int64_t mask_b, i
  *     both (head_dim contiguous), so [num_pages, Hkv, page_size, D] and [num_pages, page_size, Hkv, D] both work.
  *   The tokens of a step lie behind one another in [n_tokens, heads, D], sequence after sequence.
  * Pages, slots and lengths are read on the device: a captured call follows what the arrays hold when it is replayed.
+ * The calls take their many arguments as a struct, which is read before they return.
  * ------------------------------------------------------------------------- */
 /* Keys and values of a step's tokens into their pages, with the rotation of queries and keys on the way: beside
  * b200_qkv_rope_cache, for sequences at positions of their own.
@@ -434,10 +435,15 @@ int b200_attn_prefill_reads_tiles(const void* mask, int64_t S, int64_t mask_b, i
  *   q_out [n_tokens, Hq, D] dense (may be q itself where that is dense); slots[n] = page * page_size + row, a
  *   slot outside the pages writes nothing (padding; its query is rotated all the same).  Of equal slots any one may stay.
  * y = x*cos + rotate_half(x)*sin in fp32, rounded once.  head_dim a multiple of 16. */
-int b200_paged_append(const void* q, const void* k, const void* v, const void* cos_t, const void* sin_t, void* q_out,
-                      void* k_pages, void* v_pages, const int64_t* slots, int64_t n_tokens, int Hq, int Hkv, int D,
-                      int64_t num_pages, int page_size, const int64_t q_strides[2], const int64_t k_strides[2],
-                      const int64_t v_strides[2], const int64_t kv_strides[3], int table_dtype, int dtype, void* stream);
+typedef struct b200_paged_append_args {
+  const void *q, *k, *v, *cos_t, *sin_t;
+  void *q_out, *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t n_tokens, num_pages;
+  int64_t q_strides[2], k_strides[2], v_strides[2], kv_strides[3];
+  int32_t Hq, Hkv, D, page_size, table_dtype, dtype;
+} b200_paged_append_args;
+int b200_paged_append(const b200_paged_append_args* args, void* stream);
 
 /* Attention of every sequence's new tokens over its pages (their keys and values appended before): beside
  * b200_attn_decode and b200_attn_prefill, for decoding sequences, chunks of prompts and both in one batch.
@@ -449,11 +455,17 @@ int b200_paged_append(const void* q, const void* k, const void* v, const void* c
  * cache read as zeros; table entries of pages without an attended key are not looked at, and what lies in pages behind
  * kv_len or ahead of the window does not matter, whatever it is.  Probabilities are rounded to the activation type for the second product.
  * workspace: 16-byte aligned, b200_attn_paged_workspace_bytes bytes of any content; calls that may overlap need one each. */
-int b200_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* q_start,
-                    const int32_t* kv_len, const int32_t* page_table, int64_t B, int64_t n_tokens, int64_t max_q,
-                    int Hq, int Hkv, int D, int64_t num_pages, int page_size, int64_t table_stride,
-                    const int64_t q_strides[2], const int64_t kv_strides[3], int64_t window, float scale, int dtype,
-                    void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct b200_attn_paged_args {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  const int32_t *q_start, *kv_len, *page_table;
+  void* workspace;
+  int64_t workspace_bytes, B, n_tokens, max_q, num_pages, table_stride;
+  int64_t q_strides[2], kv_strides[3], window;
+  int32_t Hq, Hkv, D, page_size, dtype;
+  float scale;
+} b200_attn_paged_args;
+int b200_attn_paged(const b200_attn_paged_args* args, void* stream);
 int64_t b200_attn_paged_workspace_bytes(int64_t max_q, int Hq, int Hkv, int D);
 
 /* One token per row of logits (f32, f16, bf16), drawn with the given random numbers: beside b200_argmax_rows.

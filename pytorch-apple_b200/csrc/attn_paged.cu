@@ -497,35 +497,36 @@ extern "C" int64_t b200_attn_paged_workspace_bytes(int64_t max_q, int Hq, int Hk
   return workspace_parts(rows_of(max_q, Hq / Hkv), D, &ml, &acc);
 }
 
-extern "C" int b200_attn_paged(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* q_start, const int32_t* kv_len,
-                               const int32_t* page_table, int64_t B, int64_t n_tokens, int64_t max_q, int Hq, int Hkv, int D, int64_t num_pages,
-                               int page_size, int64_t table_stride, const int64_t q_strides[2], const int64_t kv_strides[3], int64_t window, float scale,
-                               int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-  B200_CHECK_ARG(q && k_pages && v_pages && out && q_start && kv_len && page_table && q_strides && kv_strides && B >= 0 && n_tokens >= 0 && max_q >= 0 &&
-                 Hq > 0 && Hkv > 0 && num_pages > 0 && table_stride > 0 && window >= 0, "b200_attn_paged: bad arguments");
+extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
+  B200_CHECK_ARG(args, "b200_attn_paged: bad arguments");
+  const b200_attn_paged_args& a = *args;
+  const int Hq = a.Hq, Hkv = a.Hkv, D = a.D, dtype = a.dtype;
+  B200_CHECK_ARG(a.q && a.k_pages && a.v_pages && a.out && a.q_start && a.kv_len && a.page_table && a.B >= 0 && a.n_tokens >= 0 && a.max_q >= 0 &&
+                 Hq > 0 && Hkv > 0 && a.num_pages > 0 && a.table_stride > 0 && a.window >= 0, "b200_attn_paged: bad arguments");
   B200_CHECK_ARG(D == 64 || D == 128, "b200_attn_paged: head_dim %d not supported (64 and 128 only)", D);
   B200_CHECK_ARG(Hq % Hkv == 0 && Hq / Hkv <= 128, "b200_attn_paged: query heads per KV head must divide and be <= 128");
-  B200_CHECK_ARG(page_size > 0 && page_size % 16 == 0, "b200_attn_paged: page size %d is not a multiple of 16", page_size);
-  if (!(table_stride < (1ll << 30) && table_stride * page_size < (1ll << 30) && n_tokens * Hq < (1ll << 31) && B <= PAGED_MAX_SEQS))
+  B200_CHECK_ARG(a.page_size > 0 && a.page_size % 16 == 0, "b200_attn_paged: page size %d is not a multiple of 16", a.page_size);
+  if (!(a.table_stride < (1ll << 30) && a.table_stride * a.page_size < (1ll << 30) && a.n_tokens * Hq < (1ll << 31) && a.B <= PAGED_MAX_SEQS))
     B200_FAIL(B200_ELIMIT, "b200_attn_paged: more than %d sequences, 2^30 keys of one or 2^31 rows of queries", PAGED_MAX_SEQS);
-  bool ok = aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace);
+  bool ok = aligned16(a.q) && aligned16(a.k_pages) && aligned16(a.v_pages) && aligned16(a.out) && aligned16(a.workspace);
   PagedParams p;
-  for (int i = 0; i < 2; ++i) { p.qs[i] = q_strides[i]; ok = ok && q_strides[i] % 8 == 0 && q_strides[i] >= 0; }
-  for (int i = 0; i < 3; ++i) { p.ks[i] = kv_strides[i]; ok = ok && kv_strides[i] % 8 == 0 && kv_strides[i] >= 0; }
-  if (!ok) B200_FAIL(B200_EALIGN, "b200_attn_paged: operands must be 16-byte aligned with strides multiple of 8");
+  const int64_t q_len[2] = {a.n_tokens, Hq}, kv_len[3] = {a.num_pages, Hkv, a.page_size};
+  for (int i = 0; i < 2; ++i) { p.qs[i] = a.q_strides[i]; ok = ok && a.q_strides[i] % 8 == 0 && (a.q_strides[i] > 0 || q_len[i] <= 1); }
+  for (int i = 0; i < 3; ++i) { p.ks[i] = a.kv_strides[i]; ok = ok && a.kv_strides[i] % 8 == 0 && (a.kv_strides[i] > 0 || kv_len[i] <= 1); }
+  if (!ok) B200_FAIL(B200_EALIGN, "b200_attn_paged: operands must be 16-byte aligned with positive strides that are multiples of 8");
   if (dtype != B200_BF16 && dtype != B200_F16) B200_FAIL(B200_ENOTSUP, "b200_attn_paged: dtype %d is not f16/bf16", dtype);
-  if (B == 0 || n_tokens == 0 || max_q == 0) return B200_OK;
-  const int G = Hq / Hkv, rows = rows_of(max_q, G);
+  if (a.B == 0 || a.n_tokens == 0 || a.max_q == 0) return B200_OK;
+  const int G = Hq / Hkv, rows = rows_of(a.max_q, G);
   int64_t ml, acc;
   const int64_t need = workspace_parts(rows, D, &ml, &acc);
-  if (!workspace || workspace_bytes < need)
-    B200_FAIL(B200_EINVAL, "b200_attn_paged: workspace of %lld bytes required (got %lld)", (long long)need, (long long)workspace_bytes);
-  p.q = q; p.k_pages = k_pages; p.v_pages = v_pages; p.out = out; p.q_start = q_start; p.kv_len = kv_len; p.table = page_table;
-  p.B = B; p.N = n_tokens; p.num_pages = num_pages; p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.page_size = page_size;
-  p.window = window; p.scale = scale;
-  p.head = static_cast<int4*>(workspace);
-  p.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + ml);
-  p.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + acc);
+  if (!a.workspace || a.workspace_bytes < need)
+    B200_FAIL(B200_EINVAL, "b200_attn_paged: workspace of %lld bytes required (got %lld)", (long long)need, (long long)a.workspace_bytes);
+  p.q = a.q; p.k_pages = a.k_pages; p.v_pages = a.v_pages; p.out = a.out; p.q_start = a.q_start; p.kv_len = a.kv_len; p.table = a.page_table;
+  p.B = a.B; p.N = a.n_tokens; p.num_pages = a.num_pages; p.table_stride = a.table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.page_size = a.page_size;
+  p.window = a.window; p.scale = a.scale;
+  p.head = static_cast<int4*>(a.workspace);
+  p.ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + ml);
+  p.acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + acc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = B200_ENOTSUP;
   if (tc5_enabled()) {
@@ -538,9 +539,10 @@ extern "C" int b200_attn_paged(const void* q, const void* k_pages, const void* v
       });
     }
   }
+  if (rc == B200_ELAUNCH) B200_CHECK_LAUNCH("attn_paged");
   if (rc == B200_ENOTSUP) {
     B200_DISPATCH_HALF(dtype, T, {
-      launch_pdl(D == 128 ? attn_paged_plain_kernel<T, 128> : attn_paged_plain_kernel<T, 64>, dim3(static_cast<unsigned>(ceil_div(n_tokens * Hq, 4))),
+      launch_pdl(D == 128 ? attn_paged_plain_kernel<T, 128> : attn_paged_plain_kernel<T, 64>, dim3(static_cast<unsigned>(ceil_div(a.n_tokens * Hq, 4))),
                  dim3(128), 0, st, p);
     });
   } else {

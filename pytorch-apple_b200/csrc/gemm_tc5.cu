@@ -1905,8 +1905,9 @@ extern "C" int b200_debug_device_error(int* code, int clear) {
   cudaError_t e = cudaMemcpyFromSymbol(&v, b200::g_tc5_error, sizeof(int));
   if (e != cudaSuccess) B200_FAIL(B200_ELAUNCH, "b200_debug_device_error: %s", cudaGetErrorString(e));
   const int att = b200::attn_prefill_tc5_error(clear != 0), stem = b200::conv_stem_error(clear != 0),
-            rows = b200::conv_rows_error(clear != 0), pair = b200::gemm_pair_error(clear != 0), paged = b200::attn_paged_error(clear != 0);
-  if (code) *code = v ? v : att > 0 ? att : stem > 0 ? stem : rows > 0 ? rows : pair > 0 ? pair : paged > 0 ? paged : 0;
+            rows = b200::conv_rows_error(clear != 0), pair = b200::gemm_pair_error(clear != 0), paged = b200::attn_paged_error(clear != 0),
+            draw = b200::sample_error(clear != 0);
+  if (code) *code = v ? v : att > 0 ? att : stem > 0 ? stem : rows > 0 ? rows : pair > 0 ? pair : paged > 0 ? paged : draw > 0 ? draw : 0;
   if (clear && v) {
     v = 0;
     cudaMemcpyToSymbol(b200::g_tc5_error, &v, sizeof(int));

@@ -60,6 +60,7 @@ int conv_tc5(const Tc5Args& a, const Tc5Conv& g, cudaStream_t stream);
 // B200_ENOTSUP for other geometries and for shapes that the im2col route with tiles of im2col_bn columns serves better.
 int conv_rows(const Tc5Args& a, const Tc5Conv& g, int im2col_bn, cudaStream_t stream);
 int conv_rows_error(bool clear);
+int sample_error(bool clear);    // sample.cu
 // code left by a bounded wait of the stem + pooling kernel (conv_stem.cu) that ran out (0 = none); optionally cleared
 int conv_stem_error(bool clear);
 

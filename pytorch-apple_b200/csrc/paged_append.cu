@@ -83,33 +83,31 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
 
 using namespace b200;
 
-extern "C" int b200_paged_append(const void* q, const void* k, const void* v, const void* cos_t, const void* sin_t, void* q_out, void* k_pages,
-                                 void* v_pages, const int64_t* slots, int64_t n_tokens, int Hq, int Hkv, int D, int64_t num_pages, int page_size,
-                                 const int64_t q_strides[2], const int64_t k_strides[2], const int64_t v_strides[2], const int64_t kv_strides[3],
-                                 int table_dtype, int dtype, void* stream) {
-  B200_CHECK_ARG(k && v && k_pages && v_pages && slots && k_strides && v_strides && kv_strides && n_tokens >= 0 && Hq >= 0 && Hkv > 0 && num_pages > 0 &&
-                 page_size > 0, "b200_paged_append: bad arguments");
-  B200_CHECK_ARG(Hq == 0 || (q && q_out && q_strides), "b200_paged_append: query heads without queries, their strides or a place for them");
-  B200_CHECK_ARG(!cos_t == !sin_t, "b200_paged_append: cos and sin tables come together");
-  B200_CHECK_ARG(D > 0 && D % 16 == 0, "b200_paged_append: head_dim %d is not a multiple of 16", D);
-  if (cos_t && table_dtype != B200_F32 && table_dtype != dtype)
-    B200_FAIL(B200_ENOTSUP, "b200_paged_append: tables are f32 or of the activation type (got dtype %d)", table_dtype);
-  bool ok = aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages) && aligned16(cos_t) && aligned16(sin_t);
+extern "C" int b200_paged_append(const b200_paged_append_args* a, void* stream) {
+  B200_CHECK_ARG(a && a->k && a->v && a->k_pages && a->v_pages && a->slots && a->n_tokens >= 0 && a->Hq >= 0 && a->Hkv > 0 && a->num_pages > 0 &&
+                 a->page_size > 0, "b200_paged_append: bad arguments");
+  B200_CHECK_ARG(a->Hq == 0 || (a->q && a->q_out), "b200_paged_append: query heads without queries or a place for them");
+  B200_CHECK_ARG(!a->cos_t == !a->sin_t, "b200_paged_append: cos and sin tables come together");
+  B200_CHECK_ARG(a->D > 0 && a->D % 16 == 0, "b200_paged_append: head_dim %d is not a multiple of 16", a->D);
+  if (a->cos_t && a->table_dtype != B200_F32 && a->table_dtype != a->dtype)
+    B200_FAIL(B200_ENOTSUP, "b200_paged_append: tables are f32 or of the activation type (got dtype %d)", a->table_dtype);
+  bool ok = aligned16(a->k) && aligned16(a->v) && aligned16(a->k_pages) && aligned16(a->v_pages) && aligned16(a->cos_t) && aligned16(a->sin_t);
   AppendParams p;
-  p.x[0] = q; p.x[1] = k; p.x[2] = v;
-  if (Hq > 0) ok = ok && aligned16(q) && aligned16(q_out);
+  p.x[0] = a->q; p.x[1] = a->k; p.x[2] = a->v;
+  if (a->Hq > 0) ok = ok && aligned16(a->q) && aligned16(a->q_out);
   for (int i = 0; i < 2; ++i) {
-    p.xs[0][i] = Hq > 0 ? q_strides[i] : 0; p.xs[1][i] = k_strides[i]; p.xs[2][i] = v_strides[i];
+    p.xs[0][i] = a->Hq > 0 ? a->q_strides[i] : 0; p.xs[1][i] = a->k_strides[i]; p.xs[2][i] = a->v_strides[i];
     ok = ok && p.xs[0][i] % 8 == 0 && p.xs[1][i] % 8 == 0 && p.xs[2][i] % 8 == 0;
   }
-  for (int i = 0; i < 3; ++i) { p.ps[i] = kv_strides[i]; ok = ok && kv_strides[i] % 8 == 0; }
+  for (int i = 0; i < 3; ++i) { p.ps[i] = a->kv_strides[i]; ok = ok && a->kv_strides[i] % 8 == 0; }
   if (!ok) B200_FAIL(B200_EALIGN, "b200_paged_append: operands must be 16-byte aligned with strides multiple of 8");
-  if (n_tokens == 0) return B200_OK;
-  p.cos_t = cos_t; p.sin_t = sin_t; p.q_out = q_out; p.k_pages = k_pages; p.v_pages = v_pages; p.slots = slots;
-  p.N = n_tokens; p.n_slots = num_pages * page_size; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.page_size = page_size; p.table_dtype = table_dtype;
-  const int64_t blocks = ceil_div(n_tokens * (Hq + 2 * static_cast<int64_t>(Hkv)) * (D >> 4), 128);
+  if (a->n_tokens == 0) return B200_OK;
+  p.cos_t = a->cos_t; p.sin_t = a->sin_t; p.q_out = a->q_out; p.k_pages = a->k_pages; p.v_pages = a->v_pages; p.slots = a->slots;
+  p.N = a->n_tokens; p.n_slots = a->num_pages * a->page_size; p.Hq = a->Hq; p.Hkv = a->Hkv; p.D = a->D; p.page_size = a->page_size;
+  p.table_dtype = a->table_dtype;
+  const int64_t blocks = ceil_div(a->n_tokens * (a->Hq + 2 * static_cast<int64_t>(a->Hkv)) * (a->D >> 4), 128);
   if (blocks >= (1ll << 31)) B200_FAIL(B200_ELIMIT, "b200_paged_append: too many tokens");
-  B200_DISPATCH_HALF(dtype, T, { launch_pdl(paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, static_cast<cudaStream_t>(stream), p); });
+  B200_DISPATCH_HALF(a->dtype, T, { launch_pdl(paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, static_cast<cudaStream_t>(stream), p); });
   B200_CHECK_LAUNCH("paged_append_kernel");
   return B200_OK;
 }

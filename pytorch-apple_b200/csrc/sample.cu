@@ -5,13 +5,16 @@
 // first always), min-p what weighs at least min_p.  The token drawn is the first one, by index, at which the running sum of what is kept
 // passes u times the whole sum.
 //
-// Weights are whole numbers in units of 2^-40 (their sums over a row stay below 2^62), good to about 2^-31 of themselves: integer sums
+// Weights are whole numbers in units of 2^-40 (their sums over a row stay below 2^62), good to about 2^-31 of the largest: integer sums
 // do not depend on the order of the additions, so the same row gives the same token however it is dealt to blocks, and a sum over
 // 150 000 tokens is as exact as its terms (in fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a
 // rare token is wide).  Thresholds are found on the logits themselves, never on weights.
 //
-// A row belongs to the CTAs of a cluster, each with a contiguous range of columns; what they find out they tell one another through
-// distributed shared memory.
+// A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once (a bulk copy per warp)
+// and then goes through several times: for the maximum; for counts or weights in 16 intervals of z, then in 16 parts of the interval in which the k-th token or
+// the top_p-th part of the sum lies, and so on (private counters per lane: no atomics) until few enough tokens are left to be
+// sorted; for the tokens to be sorted.  Mostly all that is kept is in that list, and its CTA finishes alone; where more is kept than a list
+// holds, the list gives the last token kept and the row is drawn from by sums over ranges.
 #include "common.cuh"
 #include "tc5.cuh"
 
@@ -24,6 +27,11 @@ constexpr int ST = 512, SW = ST / 32;        // threads and warps of a CTA
 constexpr int MAX_CTAS = 8;                  // of a row
 constexpr int64_t MAX_COLS = 1 << 22;        // sums of weights stay below 2^62
 constexpr u64 ONE = 1ull << 40;              // weight of the row's maximum
+constexpr int BINS = 16;
+constexpr int CAP = 2048;                    // tokens of a list
+constexpr int BIN_BYTES = SW * BINS * 32 * 8;   // a counter per warp, bin and lane; later the lists
+constexpr int STAGE_BYTES = 152 * 1024;      // of a CTA's columns at most
+static_assert(BIN_BYTES >= 3 * CAP * 8, "the lists lie over the counters");
 
 struct SampleParams {
   const void* logits;
@@ -32,7 +40,11 @@ struct SampleParams {
   const float *temperature, *top_p, *min_p, *uniform;
   const int32_t* top_k;
   int cols, seg;   // columns of the row and of a CTA's range
+  int staged;      // the range is brought into shared memory
 };
+
+// code left by a bounded wait that ran out
+__device__ int g_sample_error = 0;
 
 // Keys order like the logits they come from: equal keys, equal values (-0 counts as 0); NaN comes last, like -infinity.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -40,7 +52,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-constexpr uint32_t KEY_NEG_INF = 0x007fffffu;   // key_of(-infinity)
 
 // exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T, by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a table for
 // the first eight, a cubic for the rest (its next term is below 2^-38).  The difference and its product with log2(e) / T are carried as
@@ -52,9 +63,14 @@ struct Weigher {
     if (z == m) return ONE;
     const float dh = m - z, bv = m - dh, dl = (m - (dh + bv)) + (bv - z);
     const float p = __fmul_rn(dh, c_hi);
-    if (!(p < 60.f)) return 0;   // (a NaN or an infinite difference as well)
+    if (!(p < 41.f)) return 0;   // (a NaN or an infinite difference as well)
     const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, dl * c_hi);
     const float ip = floorf(p);
+    if (p >= 16.f) {   // most tokens: below 2^24 units, where the fast exponential of the fraction (2^-22 of itself) is as good
+      float y;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((ip - p) - e));
+      return __float2uint_rz(y * __int_as_float((167 - static_cast<int>(ip)) << 23));   // 2^(40 - ip)
+    }
     int64_t t = (static_cast<int64_t>(ip) << 32) + static_cast<int64_t>(__float2uint_rz((p - ip) * 4294967296.f)) + static_cast<int64_t>(__float2int_rn(e * 4294967296.f));
     t = t < 0 ? 0 : t;
     const uint32_t f = static_cast<uint32_t>(t);
@@ -69,29 +85,41 @@ struct Weigher {
 struct Shared {
   uint32_t table[256];
   u64 part[SW];
-  u64 total;
   u64 told[2][MAX_CTAS];   // values of all CTAs of the row, two exchanges deep
+  u64 bin_mass[SW][BINS], told_mass[2][MAX_CTAS][BINS];
+  uint32_t bin_count[SW][BINS], told_count[2][MAX_CTAS][BINS];
+  u64 cut_last;            // from the list: key << 32 | index of the last token kept
+  int listed;
+  int pick[2];
+  __align__(8) uint64_t full[SW];
 };
 
 // A thread's share of the CTA's columns: warp w has a contiguous range, 256 columns at a time, eight per lane.
 template <typename T> struct Row {
   const T* x;
-  int begin, end;   // of this warp
+  const T* copy;             // of this warp's range, or nullptr
+  int begin, end, copied;    // columns begin .. copied - 1 are in the copy
   bool vec;
   __device__ __forceinline__ void load(int c, float (&f)[8]) const {   // columns c .. c + 7; those past the end as NaN
-    if (vec && c + 8 <= end) {
-      if constexpr (sizeof(T) == 2) {
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(x + c)), f);
-      } else {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(x + c)), b = __ldg(reinterpret_cast<const float4*>(x + c) + 1);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-      }
+    if (c + 8 <= copied) {
+      unpack(copy + (c - begin), f);
+    } else if (vec && c + 8 <= end) {
+      unpack(x + c, f);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = c + k < end ? to_f32<T>(x[c + k]) : __uint_as_float(0x7fffffffu);
     }
   }
+  static __device__ __forceinline__ void unpack(const T* at, float (&f)[8]) {
+    if constexpr (sizeof(T) == 2) {
+      unpack8<T>(*reinterpret_cast<const uint4*>(at), f);
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(at), b = *(reinterpret_cast<const float4*>(at) + 1);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+  }
   template <typename F> __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll 2
     for (int c = begin + (threadIdx.x & 31) * 8; c < end; c += 256) {
       float v[8];
       load(c, v);
@@ -137,16 +165,60 @@ template <bool TOP> __device__ u64 row_reduce(u64 v, Shared& sh, int ctas, int& 
   return r;
 }
 
+// list[0 .. n) in descending order; n a power of two.  All threads; begins and ends with a barrier.
+__device__ void sort_list(u64* list, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += ST) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const u64 a = list[lo], b = list[hi];
+        if ((a < b) == ((lo & size) == 0)) { list[lo] = b; list[hi] = a; }
+      }
+    }
+  __syncthreads();
+}
+
+// sums[i] = val(0) + .. + val(i) for i < n <= CAP (four to a thread).  All threads; ends with a barrier.
+template <typename F> __device__ void scan_list(u64* sums, int n, Shared& sh, F&& val) {
+  constexpr int PER = CAP / ST;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 v[PER], run = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    run += i < n ? val(i) : 0;
+    v[e] = run;
+  }
+  u64 upto = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  __syncthreads();
+  if (lane == 31) sh.part[warp] = upto;
+  __syncthreads();
+  u64 before = upto - run;
+  for (int w = 0; w < warp; ++w) before += sh.part[w];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = threadIdx.x * PER + e;
+    if (i < n) sums[i] = before + v[e];
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
 template <typename T>
-__global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constant__ SampleParams p) {
+  extern __shared__ __align__(16) uint8_t dsm[];
   __shared__ Shared sh;
+  u64* const bins = reinterpret_cast<u64*>(dsm);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = gridDim.x, rank = blockIdx.x;
   const int64_t r = blockIdx.y;
   int turn = 0;
-  if (threadIdx.x < 256) sh.table[threadIdx.x] = static_cast<uint32_t>(exp2(-static_cast<double>(threadIdx.x) / 256.) * 2147483648. + 0.5);
-  pdl_trigger();
-  if (ctas > 1) tc5::cluster_sync();   // every CTA of the row runs before anyone writes into a peer
-  pdl_wait();
   const T* x = static_cast<const T*>(p.logits) + r * p.row_stride;
   const int c0 = min(p.cols, rank * p.seg), c1 = min(p.cols, c0 + p.seg);
   const int span = (((c1 - c0 + SW - 1) / SW) + 255) & ~255;   // columns of a warp
@@ -155,33 +227,216 @@ __global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__
   row.begin = min(c1, c0 + warp * span);
   row.end = min(c1, row.begin + span);
   row.vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+  row.copied = row.begin;
+  row.copy = reinterpret_cast<const T*>(dsm + BIN_BYTES) + (row.begin - c0);
+  if (lane == 0) tc5::mbar_init(&sh.full[warp], 1);
+  if (threadIdx.x == 0) sh.listed = 0;
+  tc5::fence_barrier_init();
+  __syncwarp();
+  pdl_trigger();
+  pdl_wait();
+  if (p.staged && row.vec) {
+    const uint32_t bytes = static_cast<uint32_t>(row.end - row.begin) * sizeof(T) & ~15u;
+    row.copied = row.begin + bytes / sizeof(T);
+    if (bytes && lane == 0) {
+      tc5::mbar_arrive_expect_tx(&sh.full[warp], bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(tc5::smem_addr(row.copy)), "l"(x + row.begin), "r"(bytes), "r"(tc5::smem_addr(&sh.full[warp])) : "memory");
+    }
+  }
+  if (threadIdx.x < 256) sh.table[threadIdx.x] = static_cast<uint32_t>(exp2(-static_cast<double>(threadIdx.x) / 256.) * 2147483648. + 0.5);
+  const float T_ = p.temperature ? __ldg(p.temperature + r) : 1.f, tp = p.top_p ? __ldg(p.top_p + r) : 1.f, mp = p.min_p ? __ldg(p.min_p + r) : 0.f;
+  const int k = p.top_k ? __ldg(p.top_k + r) : 0;
+  const float uniform = __ldg(p.uniform + r);
+  if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer; the table is there
+  if (row.copied > row.begin && !tc5::mbar_wait(&sh.full[warp], 0) && lane == 0) atomicExch(&g_sample_error, 70);
 
   // ---- the maximum, and of equal ones the lowest index ----
   u64 best = 0;
-  row.each([&](float z, int c) {
-    const u64 v = static_cast<u64>(key_of(z)) << 32 | static_cast<uint32_t>(~c);
-    if (v > best && c < row.end) best = v;
-  });
+  {
+    float top = -INFINITY;   // (a lane's columns come in rising order: of equal ones the first stays)
+    int at = -1;
+    row.each([&](float z, int c) {
+      if (z > top) { top = z; at = c; }
+    });
+    if (at >= 0) best = static_cast<u64>(key_of(top)) << 32 | static_cast<uint32_t>(~at);
+  }
   best = row_reduce<true>(best, sh, ctas, turn);
-  const uint32_t top = static_cast<uint32_t>(best >> 32);
-  const int first = static_cast<int>(~static_cast<uint32_t>(best));
-  const float T_ = p.temperature ? __ldg(p.temperature + r) : 1.f;
-  if (!(T_ > 0.f) || top <= KEY_NEG_INF) {   // greedy; a row without any weight gives its first token
-    if (rank == 0 && threadIdx.x == 0) p.out[r] = top <= KEY_NEG_INF ? 0 : first;
+  if (!(T_ > 0.f) || best == 0) {   // greedy; a row without any weight gives its first token
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = best == 0 ? 0 : static_cast<int>(~static_cast<uint32_t>(best));
     return;
   }
-  const double c = 1.4426950408889634074 / static_cast<double>(T_);
+  const double c_ = 1.4426950408889634074 / static_cast<double>(T_);
   Weigher weight;
-  weight.m = __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
-  weight.c_hi = static_cast<float>(c);
-  weight.c_lo = static_cast<float>(c - static_cast<double>(weight.c_hi));
+  weight.m = value_of(static_cast<uint32_t>(best >> 32));
+  weight.c_hi = static_cast<float>(c_);
+  weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
   weight.table = sh.table;
+  const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;
+  auto target_of = [&](u64 total) -> u64 {
+    const double d = static_cast<double>(uniform) * static_cast<double>(total);
+    const u64 t = d > 0. ? (d < static_cast<double>(total) ? static_cast<u64>(d) : total - 1) : 0;
+    return t < total ? t : total - 1;
+  };
 
   // What is kept: keys above `cut`, and of those equal to it the indices up to `last`
   uint32_t cut = 0;
   int last = p.cols;
-  // the (need)th lowest index among the columns whose key is `cut`
-  auto index_limit = [&](u64 need) {
+  auto stays = [&](float z, int i) {
+    const uint32_t key = key_of(z);
+    return i < row.end && (key > cut || (key == cut && i <= last));
+  };
+
+  // The place of a logit in [0, 2^32) below the maximum, 2^32 where weights end; not below 2^32 for those that weigh nothing and for NaN.  It
+  // falls as logits rise (every step of its arithmetic does), equal places need not mean equal logits.
+  const float to_place = weight.c_hi * (4294967296.f / 41.f);
+  auto place = [&](float z) { return z == weight.m ? 0.f : (weight.m - z) * to_place; };
+  constexpr float END = 4294967040.f;
+
+  // Looks for the token that the filter ends with: the k-th (count), or the one at which the running sum reaches `limit`.  Result: 0 nothing is cut off,
+  // 1 all that is kept is in the list of CTA 0, 2 (cut, last) are found, 3 they are to be found bit by bit.
+  u64 whole = 0;         // sum of what is kept before top-p
+  auto limit_of = [&](u64 sum) { return fmax(static_cast<double>(tp) * static_cast<double>(sum), 0.5); };
+  const bool restricted_by_k = k > 0 && k < p.cols;
+  auto collect = [&](uint32_t lo, uint32_t hi) {   // tokens with places in [lo, hi], to CTA 0
+    const uint32_t to_count = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(&sh.listed), 0) : tc5::smem_addr(&sh.listed);
+    const uint32_t to_list = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(bins), 0) : tc5::smem_addr(bins);
+    row.each([&](float z, int i) {
+      const float pl = place(z);
+      if (pl < END && i < row.end) {
+        const uint32_t X = __float2uint_rz(pl);
+        if (X >= lo && X <= hi && stays(z, i)) {
+          uint32_t at;
+          asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(to_count) : "memory");
+          if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to_list + at * 8), "l"(static_cast<u64>(key_of(z)) << 32 | static_cast<uint32_t>(~i)) : "memory");
+        }
+      }
+    });
+    if (ctas > 1) tc5::cluster_sync(); else __syncthreads();
+  };
+  auto sorted = [&]() {   // CTA 0: its list in order; the number of tokens
+    const int n = min(sh.listed, CAP);
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += ST) bins[i] = 0;
+    sort_list(bins, size);
+    return n;
+  };
+  auto search = [&](const bool by_mass) -> int {
+    uint32_t prefix = 0, above = 0;
+    u64 above_mass = 0;
+    double limit = 0.;
+#pragma unroll 1
+    for (int shift = 28; ; shift -= 4) {
+      u64* const own = bins + warp * BINS * 32 + lane;
+#pragma unroll
+      for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
+      row.each([&](float z, int i) {
+        const float pl = place(z);
+        if (pl < END && i < row.end) {
+          const uint32_t X = __float2uint_rz(pl);
+          if (shift == 28 || (X >> (shift + 4)) == prefix) {
+            u64 add = 1ull << 52;   // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1)
+            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight(z) : 0;
+            own[((X >> shift) & 15u) * 32] += add;
+          }
+        }
+      });
+      __syncwarp();
+      {
+        const int b = lane >> 1;
+        uint32_t count = 0;
+        u64 mass = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const u64 v = bins[(warp * BINS + b) * 32 + (lane & 1) * 16 + ((e + b) & 15)];
+          count += static_cast<uint32_t>(v >> 52);
+          mass += v & ((1ull << 52) - 1);
+        }
+        count += __shfl_xor_sync(0xffffffffu, count, 1);
+        mass += __shfl_xor_sync(0xffffffffu, mass, 1);
+        if (!(lane & 1)) { sh.bin_count[warp][b] = count; sh.bin_mass[warp][b] = mass; }
+      }
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < BINS * ctas) {
+        const int b = threadIdx.x & (BINS - 1), to = threadIdx.x / BINS;
+        uint32_t count = 0;
+        u64 mass = 0;
+        for (int w = 0; w < SW; ++w) { count += sh.bin_count[w][b]; mass += sh.bin_mass[w][b]; }
+        if (ctas == 1) {
+          sh.told_count[turn][0][b] = count;
+          sh.told_mass[turn][0][b] = mass;
+        } else {
+          const uint32_t me = tc5::cluster_ctarank();
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.told_count[turn][me][b]), to)), "r"(count) : "memory");
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.told_mass[turn][me][b]), to)), "l"(mass) : "memory");
+        }
+      }
+      if (ctas == 1) __syncthreads(); else tc5::cluster_sync();
+      // lane b of every warp: bin b over all CTAs, then running sums
+      uint32_t count = 0;
+      u64 mass = 0;
+      for (int i = 0; i < ctas; ++i) { count += sh.told_count[turn][i][lane & 15]; mass += sh.told_mass[turn][i][lane & 15]; }
+      turn ^= 1;
+      uint32_t n = count;
+      u64 s = mass;
+#pragma unroll
+      for (int o = 1; o < BINS; o <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xffffffffu, n, o);
+        const u64 t = __shfl_up_sync(0xffffffffu, s, o);
+        if ((lane & 15) >= o) { n += a; s += t; }
+      }
+      if (shift == 28 && by_mass) {
+        whole = __shfl_sync(0xffffffffu, s, 15);
+        limit = limit_of(whole);
+      }
+      const bool reached = by_mass ? static_cast<double>(above_mass + s) >= limit : above + n >= static_cast<uint32_t>(k);
+      const unsigned hit = __ballot_sync(0xffffffffu, reached && lane < BINS);
+      if (!hit) return 0;   // (fewer than k tokens weigh anything)
+      const int b = __ffs(hit) - 1;
+      const uint32_t here = __shfl_sync(0xffffffffu, count, b);
+      above += __shfl_sync(0xffffffffu, n, b) - here;
+      above_mass += __shfl_sync(0xffffffffu, s, b) - __shfl_sync(0xffffffffu, mass, b);
+      prefix = prefix << 4 | static_cast<uint32_t>(b);
+      const uint32_t first = prefix << shift, end = first + ((1u << shift) - 1u);
+      if (above + here <= CAP) { collect(0, end); return 1; }
+      if (here <= CAP && (above > CAP - CAP / 8 || shift == 0)) {   // the last token kept is among these
+        collect(first, end);
+        if (rank == 0) {
+          const int n_ = sorted();
+          u64* const sums = bins + CAP;
+          int want;
+          if (by_mass) {
+            scan_list(sums, n_, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
+            int mine = n_;   // the first at which the running sum reaches the limit
+            for (int i = threadIdx.x; i < n_; i += ST)
+              if (static_cast<double>(above_mass + sums[i]) >= limit) { mine = i; break; }
+            if (threadIdx.x == 0) sh.pick[0] = n_ - 1;
+            __syncthreads();
+            atomicMin(&sh.pick[0], mine);
+            __syncthreads();
+            want = sh.pick[0];
+          } else {
+            want = static_cast<int>(static_cast<uint32_t>(k) - above) - 1;
+          }
+          if (static_cast<int>(threadIdx.x) < ctas) {
+            const u64 v = bins[want];
+            if (ctas == 1) sh.cut_last = v;
+            else asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.cut_last), threadIdx.x)), "l"(v) : "memory");
+          }
+          if (threadIdx.x == 0) sh.listed = 0;
+        }
+        if (ctas == 1) __syncthreads(); else tc5::cluster_sync();
+        cut = static_cast<uint32_t>(sh.cut_last >> 32);
+        last = static_cast<int>(~static_cast<uint32_t>(sh.cut_last));
+        return 2;
+      }
+      if (shift == 0) return 3;   // more equal places than a list holds
+    }
+  };
+
+  // The thresholds bit by bit, a pass over the row for each bit of key and index: for rows with thousands of equal logits at the border
+  auto index_limit = [&](u64 need) {   // the (need)th lowest index among the columns whose key is `cut`
     int at = 0;
 #pragma unroll 1
     for (int bit = 1 << 21; bit > 0; bit >>= 1) {
@@ -192,9 +447,7 @@ __global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__
     }
     return at;
   };
-
-  const int k = p.top_k ? __ldg(p.top_k + r) : 0;
-  if (k > 0 && k < p.cols) {
+  auto top_k_by_bits = [&]() {
 #pragma unroll 1
     for (uint32_t bit = 0x80000000u; bit > 0; bit >>= 1) {
       u64 n = 0;
@@ -205,34 +458,73 @@ __global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__
     row.each([&](float z, int i) { above += (i < row.end && key_of(z) > cut) ? 1 : 0; });
     above = row_reduce<false>(above, sh, ctas, turn);
     last = index_limit(static_cast<u64>(k) - above);
-  }
-  const float tp = p.top_p ? __ldg(p.top_p + r) : 1.f;
-  if (tp < 1.f) {
+  };
+  auto top_p_by_bits = [&]() {
     auto mass_from = [&](uint32_t from) {   // of what is kept so far, with keys of at least `from`
       u64 s = 0;
       row.each([&](float z, int i) {
-        const uint32_t key = key_of(z);
-        if (i < row.end && key >= from && (key > cut || (key == cut && i <= last))) s += weight(z);
+        if (stays(z, i) && key_of(z) >= from) s += weight(z);
       });
       return row_reduce<false>(s, sh, ctas, turn);
     };
-    const double limit = fmax(static_cast<double>(tp) * static_cast<double>(mass_from(0)), 0.5);
+    const double limit = limit_of(whole);
     uint32_t at = 0;
 #pragma unroll 1
     for (uint32_t bit = 0x80000000u; bit > 0; bit >>= 1)
       if (static_cast<double>(mass_from(at | bit)) >= limit) at |= bit;
     const u64 above = at == 0xffffffffu ? 0 : mass_from(at + 1);
     if (at != cut) { cut = at; last = p.cols; }
-    const u64 w = weight(__uint_as_float(at & 0x80000000u ? at & 0x7fffffffu : ~at));
-    last = min(last, index_limit(static_cast<u64>(ceil((limit - static_cast<double>(above)) / static_cast<double>(w)))));
-  }
-  const float mp = p.min_p ? __ldg(p.min_p + r) : 0.f;
-  const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;
+    last = min(last, index_limit(static_cast<u64>(ceil((limit - static_cast<double>(above)) / static_cast<double>(weight(value_of(at)))))));
+  };
 
-  // ---- the draw: sums of the warps' ranges, then the range in which the running sum passes the target ----
+  int found = 0;
+  bool all_k = false;    // the list holds the k tokens themselves
+  if (restricted_by_k) {
+    found = search(false);
+    all_k = found == 1;
+    if (found == 3) top_k_by_bits();
+  }
+  if (tp < 1.f && found != 1) {
+    found = search(true);
+    if (found == 3) top_p_by_bits();
+  }
+
+  if (found == 1) {
+    // ---- everything that can be kept is in the list of CTA 0: cut it off there, and draw in the order of the indices ----
+    if (rank != 0) return;
+    const int n = sorted();
+    u64 *const sums = bins + CAP, *const order = bins + 2 * CAP;
+    scan_list(sums, n, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
+    int kept = all_k && k < n ? k : n;
+    const double limit = tp < 1.f ? limit_of(all_k ? sums[kept - 1] : whole) : 0.;
+    if (threadIdx.x == 0) sh.pick[0] = sh.pick[1] = kept;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kept; i += ST) {
+      const u64 before = i > 0 ? sums[i - 1] : 0;
+      if ((tp < 1.f && i > 0 && static_cast<double>(before) >= limit) || sums[i] - before < least) { atomicMin(&sh.pick[0], i); break; }
+    }
+    __syncthreads();
+    kept = sh.pick[0];
+    int size = 2;
+    while (size < kept) size <<= 1;
+    for (int i = threadIdx.x; i < size; i += ST) order[i] = i < kept ? (bins[i] << 32 | static_cast<uint32_t>(i)) : 0;   // ~index, place in the list
+    sort_list(order, size);
+    const u64 total = sums[kept - 1];
+    scan_list(bins, kept, sh, [&](int i) {   // (the keys are not needed any more: weights come from the sums)
+      const uint32_t j = static_cast<uint32_t>(order[i]);
+      return sums[j] - (j > 0 ? sums[j - 1] : 0);
+    });
+    const u64 target = target_of(total);
+    for (int i = threadIdx.x; i < kept; i += ST)
+      if (bins[i] > target) { atomicMin(&sh.pick[1], i); break; }
+    __syncthreads();
+    if (threadIdx.x == 0) p.out[r] = static_cast<int>(~static_cast<uint32_t>(order[min(sh.pick[1], kept - 1)] >> 32));
+    return;
+  }
+
+  // ---- the draw: sums of the warps' ranges, then of parts of the one in which the running sum passes the target ----
   auto kept = [&](float z, int i) -> u64 {
-    const uint32_t key = key_of(z);
-    if (i >= row.end || key < cut || (key == cut && i > last)) return 0;
+    if (!stays(z, i)) return 0;
     const u64 w = weight(z);
     return w >= least ? w : 0;
   };
@@ -241,20 +533,46 @@ __global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
-  const double d = static_cast<double>(p.uniform ? __ldg(p.uniform + r) : 0.f) * static_cast<double>(total);
-  u64 target = d > 0. ? (d < static_cast<double>(total) ? static_cast<u64>(d) : total - 1) : 0;
-  target = target < total ? target : total - 1;
+  const u64 target = target_of(total);
   u64 before = 0;
   for (int i = 0; i < rank; ++i) before += sh.told[slot][i];
+  if (target < before || target >= before + sh.told[slot][rank]) return;   // another CTA's
+  int w_ = 0;
+  while (before + sh.part[w_] <= target) before += sh.part[w_++];
+  // all warps take equal parts of warp w_'s range, in whole steps of 256 columns
+  const int b_ = min(c1, c0 + w_ * span), e_ = min(c1, b_ + span), step = ((e_ - b_ + 255) / 256 + SW - 1) / SW * 256;
+  const int from = min(e_, b_ + warp * step), upto_ = min(e_, from + step);
+  Row<T> part = row;
+  part.begin = b_;
+  part.end = e_;
+  part.copy = reinterpret_cast<const T*>(dsm + BIN_BYTES) + (b_ - c0);
+  part.copied = p.staged && row.vec ? b_ + static_cast<int>((static_cast<uint32_t>(e_ - b_) * sizeof(T) & ~15u) / sizeof(T)) : b_;
+  auto kept_at = [&](float z, int i) -> u64 {
+    const uint32_t key = key_of(z);
+    if (i >= upto_ || key < cut || (key == cut && i > last)) return 0;
+    const u64 w = weight(z);
+    return w >= least ? w : 0;
+  };
+  u64 sum = 0;
+  for (int c = from + lane * 8; c < upto_; c += 256) {
+    float v[8];
+    part.load(c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += kept_at(v[e], c + e);
+  }
+  sum = warp_add(sum);
+  __syncthreads();   // (the ranges' sums have been read)
+  if (lane == 0) sh.part[warp] = sum;
+  __syncthreads();
   for (int i = 0; i < warp; ++i) before += sh.part[i];
-  if (target < before || target >= before + mine) return;
-  for (int c = row.begin + lane * 8; ; c += 256) {   // (the whole warp goes round together)
+  if (target < before || target >= before + sum) return;
+  for (int c = from + lane * 8; ; c += 256) {   // (the whole warp goes round together, and the target lies in its part)
     float v[8];
     u64 w[8], s = 0;
-    if (c < row.end) row.load(c, v);
+    if (c < upto_) part.load(c, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = c < row.end ? kept(v[e], c + e) : 0;
+      w[e] = c < upto_ ? kept_at(v[e], c + e) : 0;
       s += w[e];
     }
     u64 upto = s;
@@ -277,26 +595,21 @@ __global__ void __launch_bounds__(ST) sample_rows_kernel(const __grid_constant__
   }
 }
 
-}  // namespace
-}  // namespace b200
-
-using namespace b200;
-
-extern "C" int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, int64_t cols, int64_t row_stride, const float* temperature,
-                                const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int dtype, void* stream) {
-  B200_CHECK_ARG(logits && out && uniform && rows >= 0 && cols > 0 && row_stride >= 0, "b200_sample_rows: bad arguments");
-  if (cols > MAX_COLS || rows > 65535) B200_FAIL(B200_ELIMIT, "b200_sample_rows: more than %lld columns or 65535 rows", (long long)MAX_COLS);
-  if (rows == 0) return B200_OK;
-  SampleParams p;
-  p.logits = logits; p.out = out; p.row_stride = row_stride; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
-  p.uniform = uniform; p.cols = static_cast<int>(cols);
-  int ctas = 1;
-  while (ctas < MAX_CTAS && 2 * ctas * rows <= 148 && cols > 4096 * ctas) ctas *= 2;
-  p.seg = static_cast<int>(ceil_div(ceil_div(cols, ctas), 256) * 256);
+template <typename T> int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st) {
+  constexpr int smem = BIN_BYTES + STAGE_BYTES;
+  static PerDevice<bool> configured_on;
+  bool* configured = configured_on.slot();
+  if (!configured) B200_FAIL(B200_ELAUNCH, "sample_rows_kernel: no current device");
+  if (!*configured) {
+    const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) B200_FAIL(B200_ELAUNCH, "sample_rows_kernel attribute: %s", cudaGetErrorString(e));
+    *configured = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(rows));
   cfg.blockDim = dim3(ST);
-  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.dynamicSmemBytes = BIN_BYTES + (p.staged ? static_cast<size_t>(p.seg) * sizeof(T) : 0);
+  cfg.stream = st;
   cudaLaunchAttribute attrs[2];
   int n = 0;
   attrs[n].id = cudaLaunchAttributeClusterDimension;
@@ -309,7 +622,42 @@ extern "C" int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, 
   }
   cfg.attrs = attrs;
   cfg.numAttrs = n;
-  B200_DISPATCH_FLOAT(dtype, T, { cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, p); });
+  cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, p);
   B200_CHECK_LAUNCH("sample_rows_kernel");
+  return B200_OK;
+}
+
+}  // namespace
+
+int sample_error(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_sample_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_sample_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, int64_t cols, int64_t row_stride, const float* temperature,
+                                const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int dtype, void* stream) {
+  B200_CHECK_ARG(logits && out && uniform && rows >= 0 && cols > 0 && row_stride >= 0, "b200_sample_rows: bad arguments");
+  if (cols > MAX_COLS || rows > 65535) B200_FAIL(B200_ELIMIT, "b200_sample_rows: more than %lld columns or 65535 rows", (long long)MAX_COLS);
+  if (rows == 0) return B200_OK;
+  SampleParams p;
+  p.logits = logits; p.out = out; p.row_stride = row_stride; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
+  p.uniform = uniform; p.cols = static_cast<int>(cols);
+  // as many CTAs per row as there are SMs for, at least as many as hold the row in shared memory (longer rows are read anew in each pass)
+  const int64_t esize = dtype == B200_F32 ? 4 : 2;
+  const auto seg_of = [&](int ctas) { return ceil_div(ceil_div(cols, ctas), 256) * 256; };
+  int ctas = 1;
+  while (ctas < MAX_CTAS && cols > 2048 * ctas && (2 * ctas * rows <= 148 || seg_of(ctas) * esize > STAGE_BYTES)) ctas *= 2;
+  p.seg = static_cast<int>(seg_of(ctas));
+  p.staged = p.seg * esize <= STAGE_BYTES ? 1 : 0;
+  B200_DISPATCH_FLOAT(dtype, T, { return launch_sample<T>(p, rows, ctas, static_cast<cudaStream_t>(stream)); });
   return B200_OK;
 }

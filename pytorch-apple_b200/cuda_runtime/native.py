@@ -41,6 +41,27 @@ class EwOp(C.Structure):
     _fields_ = [("opcode", C.c_int32), ("a", C.c_int32), ("b", C.c_int32), ("round_dtype", C.c_int32), ("imm", C.c_float)]
 
 
+class PagedAppendArgs(C.Structure):
+    """``b200_paged_append_args``."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "cos_t", "sin_t", "q_out", "k_pages", "v_pages", "slots")] + \
+               [("n_tokens", C.c_int64), ("num_pages", C.c_int64), ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2),
+                ("kv_strides", C.c_int64 * 3)] + [(n, C.c_int32) for n in ("Hq", "Hkv", "D", "page_size", "table_dtype", "dtype")]
+
+
+class AttnPagedArgs(C.Structure):
+    """``b200_attn_paged_args``."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_pages", "v_pages", "out", "q_start", "kv_len", "page_table", "workspace")] + \
+               [(n, C.c_int64) for n in ("workspace_bytes", "B", "n_tokens", "max_q", "num_pages", "table_stride")] + \
+               [("q_strides", C.c_int64 * 2), ("kv_strides", C.c_int64 * 3), ("window", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("Hq", "Hkv", "D", "page_size", "dtype")] + [("scale", C.c_float)]
+
+
+# the same structures for struct.Struct, whose packing costs a tenth of filling a ctypes.Structure
+PAGED_APPEND_FORMAT = "@9P11q6i"
+ATTN_PAGED_FORMAT = "@8P12q5if"
+
 _vp, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
 _TP = C.POINTER(Tensor)
 _I64P = C.POINTER(C.c_int64)
@@ -86,8 +107,8 @@ SIGNATURES = {
     "b200_attn_prefill_reads_tiles": (_i, [_vp, _i64, _i64, _i64, _i]),
     "b200_mask_tiles": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp]),
     "b200_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i64, _i, _I64P, _I64P, _I64P, _i64, _i64, _f, _i, _vp]),
-    "b200_paged_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _i, _I64P, _I64P, _I64P, _I64P, _i, _i, _vp]),
-    "b200_attn_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i, _i, _i64, _i, _i64, _I64P, _I64P, _i64, _f, _i, _vp, _i64, _vp]),
+    "b200_paged_append": (_i, [_vp, _vp]),   # PagedAppendArgs (or its bytes), stream
+    "b200_attn_paged": (_i, [_vp, _vp]),     # AttnPagedArgs (or its bytes), stream
     "b200_attn_paged_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
     "b200_sample_rows": (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
 }
@@ -139,6 +160,19 @@ def install_test_library(lib, device: str = "cpu") -> None:
     exercise the host logic without a GPU).  Never used by the product."""
     global _test_override
     _test_override = None if lib is None else (lib, device)
+
+
+def on_stream(device, what: str, name: str, *args) -> None:
+    """Entry point ``name`` with ``args`` and the current stream of ``device`` (a ``torch.device``), with that device current."""
+    import torch
+
+    fn = getattr(_lib or load(), name) if _test_override is None else getattr(_test_override[0], name)
+    if device.type != "cuda":
+        return check(fn(*args, 0), what)
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    return check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
 
 
 def check(rc: int, what: str = "") -> None:

@@ -12,7 +12,8 @@ Work is enqueued on the current stream of the tensors' device.
 
 from __future__ import annotations
 
-import ctypes as C
+import functools
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -21,42 +22,18 @@ import torch
 from cuda_runtime import native
 
 _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_S2, _S3 = C.c_int64 * 2, C.c_int64 * 3
+_pack_append, _pack_attention = struct.Struct(native.PAGED_APPEND_FORMAT).pack, struct.Struct(native.ATTN_PAGED_FORMAT).pack
 
 
-def _call(device: torch.device, what: str, name: str, *args) -> None:
-    """The library's call on the current stream of ``device``, with that device current."""
-    fn = getattr(native.load(), name)
-    if device.type != "cuda":
-        return native.check(fn(*args, 0), what)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return native.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
-    return native.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+# The checks of the two calls run in a few microseconds as long as they pass; what is wrong is looked for when they fail.
+def _seen(**tensors) -> str:
+    return ", ".join(f"{n} {tuple(t.shape)} {str(t.dtype)[6:]} strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}"
+                     for n, t in tensors.items())
 
 
-def _same(what: str, device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
-
-
-def _heads(what: str, name: str, x: torch.Tensor, dtype, tokens: int | None = None) -> None:
-    if x.dim() != 3 or x.dtype != dtype or (x.shape[2] > 1 and x.stride(2) != 1) or (tokens is not None and x.shape[0] != tokens):
-        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim] of {dtype} with head_dim contiguous, got {tuple(x.shape)} {x.dtype} "
-                         f"strides {x.stride()}" + (f" for {tokens} tokens" if tokens is not None else ""))
-
-
-def _pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, dim: int) -> None:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.dtype != dtype or v_pages.dtype != dtype or \
-            k_pages.shape[3] != dim or k_pages.stride(3) != 1:
-        raise ValueError(f"{what}: pages must be [pages, heads, page_size, {dim}] of {dtype}, keys and values alike with head_dim contiguous, got "
-                         f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
-
-
-def _index(what: str, name: str, x: torch.Tensor, dtype, *shape) -> None:
-    if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}, got {tuple(x.shape)} {x.dtype}")
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(max_q: int, Hq: int, Hkv: int, D: int, _lib) -> int:
+    return _lib.b200_attn_paged_workspace_bytes(max_q, Hq, Hkv, D)
 
 
 def paged_append(q, k, v, cos, sin, k_pages, v_pages, slots, q_out=None):
@@ -65,41 +42,38 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, slots, q_out=None):
     ``q`` ``[N, Hq, D]`` (or None), ``k``, ``v`` ``[N, Hkv, D]``: any strides over tokens and heads (columns of a merged projection); ``cos``, ``sin``
     ``[N, D]`` in fp32 or the activation type (both None: no rotation); ``k_pages``, ``v_pages`` ``[pages, Hkv, page_size, D]``; ``slots`` int64 ``[N]``
     (page * page_size + row, negative: written nowhere).  ``q_out`` may be a dense ``q`` itself."""
-    what = "paged_append"
-    N, Hkv, D = k.shape if k.dim() == 3 else (0, 0, 0)
-    _heads(what, "k", k, k.dtype)
-    _heads(what, "v", v, k.dtype, N)
-    _pages(what, k_pages, v_pages, k.dtype, D)
-    if v.shape != k.shape or k_pages.shape[1] != Hkv:
-        raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)} and pages of {k_pages.shape[1]} heads do not belong together")
-    if k.dtype not in _CODES:
-        raise ValueError(f"{what}: {k.dtype} is not supported")
-    _index(what, "slots", slots, torch.int64, N)
-    Hq, qs = 0, None
-    if q is not None:
-        _heads(what, "q", q, k.dtype, N)
-        Hq, qs = q.shape[1], _S2(q.stride(0), q.stride(1))
-        if q.shape[2] != D:
-            raise ValueError(f"{what}: queries of {q.shape[2]} dims, keys of {D}")
+    dt, at = k.dtype, k.get_device()
+    ks, vs, ps, shape, pages = k.stride(), v.stride(), k_pages.stride(), k.shape, k_pages.shape
+    ok = len(shape) == 3 and len(pages) == 4 and dt in _CODES and v.shape == shape and v.dtype is dt and ks[2] == 1 and vs[2] == 1 and v.get_device() == at
+    ok = ok and pages == v_pages.shape and ps == v_pages.stride() and k_pages.dtype is dt and v_pages.dtype is dt and ps[3] == 1 and \
+        pages[1] == shape[1] and pages[3] == shape[2] and k_pages.get_device() == at and v_pages.get_device() == at
+    ok = ok and slots.dtype is torch.int64 and slots.shape == shape[:1] and slots.is_contiguous() and slots.get_device() == at
+    qs, Hq, q_at, out_at, c_at, s_at, table = (0, 0, 0), 0, 0, 0, 0, 0, 0
+    if ok and q is not None:
+        q_shape, qs = q.shape, q.stride()
+        ok = len(q_shape) == 3 and q.dtype is dt and qs[2] == 1 and q_shape[0] == shape[0] and q_shape[2] == shape[2] and q.get_device() == at
         if q_out is None:
-            q_out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
-            raise ValueError(f"{what}: q_out must be a contiguous {tuple(q.shape)} tensor of {q.dtype}")
-    if (cos is None) != (sin is None):
-        raise ValueError(f"{what}: cos and sin come together")
-    table = 0
-    if cos is not None:
-        _index(what, "cos", cos, cos.dtype, N, D)
-        _index(what, "sin", sin, cos.dtype, N, D)
-        if cos.dtype not in _CODES:
-            raise ValueError(f"{what}: tables of {cos.dtype} are not supported")
-        table = _CODES[cos.dtype]
-    _same(what, k.device, q=q, v=v, cos=cos, sin=sin, k_pages=k_pages, v_pages=v_pages, slots=slots, q_out=q_out)
-    p = lambda t: None if t is None else t.data_ptr()
-    if N:
-        _call(k.device, what, "b200_paged_append", p(q), k.data_ptr(), v.data_ptr(), p(cos), p(sin), p(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
-              slots.data_ptr(), N, Hq, Hkv, D, k_pages.shape[0], k_pages.shape[2], qs, _S2(k.stride(0), k.stride(1)), _S2(v.stride(0), v.stride(1)),
-              _S3(*k_pages.stride()[:3]), table, _CODES[k.dtype])
+            q_out = k.new_empty(q_shape)
+        else:
+            ok = ok and q_out.shape == q_shape and q_out.dtype is dt and q_out.is_contiguous() and q_out.get_device() == at
+        if ok:
+            Hq, q_at, out_at = q_shape[1], q.data_ptr(), q_out.data_ptr()
+    if ok and (cos is not None or sin is not None):
+        ok = cos is not None and sin is not None
+        if ok:
+            table = cos.dtype
+            ok = table in _CODES and sin.dtype is table and cos.shape == sin.shape == (shape[0], shape[2]) and cos.is_contiguous() and sin.is_contiguous() and \
+                cos.get_device() == at and sin.get_device() == at
+            table, c_at, s_at = _CODES.get(table), cos.data_ptr(), sin.data_ptr()
+    if not ok:
+        raise ValueError("paged_append: q [N, Hq, D] or None, k and v [N, Hkv, D] of one 16-bit type with contiguous rows, cos and sin dense [N, D] in fp32 or that "
+                         "type or both None, k_pages and v_pages alike [pages, Hkv, page_size, D], slots dense int64 [N], q_out dense like q, all on one "
+                         "device; got " + _seen(q=q, k=k, v=v, cos=cos, sin=sin, k_pages=k_pages, v_pages=v_pages, slots=slots, q_out=q_out))
+    if shape[0]:
+        native.on_stream(k.device, "paged_append", "b200_paged_append",
+                         _pack_append(q_at, k.data_ptr(), v.data_ptr(), c_at, s_at, out_at, k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(),
+                                      shape[0], pages[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ps[0], ps[1], ps[2],
+                                      Hq, shape[1], shape[2], pages[2], table, _CODES[dt]))
     return q_out
 
 
@@ -110,33 +84,31 @@ def paged_attention(q, k_pages, v_pages, q_start, kv_len, page_table, max_q, sca
     ``q_start[b + 1]``, at most ``max_q`` of them; ``kv_len`` int32 ``[B]``: its keys, the new tokens' among them; ``page_table`` int32 ``[B, n]``: its pages.
     A token sees the keys up to its own, with ``window`` > 0 the last ``window`` of them.  ``scale``: 1 / sqrt(D) unless given.  Rows of ``out`` behind
     the last sequence are left as they were (as they come, where ``out`` is made here)."""
-    what = "paged_attention"
-    _heads(what, "q", q, q.dtype)
-    N, Hq, D = q.shape
-    _pages(what, k_pages, v_pages, q.dtype, D)
-    if q.dtype not in _CODES:
-        raise ValueError(f"{what}: {q.dtype} is not supported")
-    n_pages, Hkv, page, _ = k_pages.shape
-    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    _index(what, "kv_len", kv_len, torch.int32, B)
-    _index(what, "q_start", q_start, torch.int32, B + 1)
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"{what}: page_table must be int32 [{B}, pages] with contiguous rows, got {tuple(page_table.shape)} {page_table.dtype}")
-    if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
-        raise ValueError(f"{what}: page_table must be dense")
+    dt, at = q.dtype, q.get_device()
+    qs, ps, shape, pages, table = q.stride(), k_pages.stride(), q.shape, k_pages.shape, page_table.shape
+    ok = len(shape) == 3 and len(pages) == 4 and len(table) == 2 and dt in _CODES and qs[2] == 1
+    ok = ok and pages == v_pages.shape and ps == v_pages.stride() and k_pages.dtype is dt and v_pages.dtype is dt and ps[3] == 1 and \
+        pages[3] == shape[2] and k_pages.get_device() == at and v_pages.get_device() == at
+    ok = ok and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32 and page_table.dtype is torch.int32 and kv_len.shape == table[:1] and \
+        q_start.shape == (table[0] + 1,) and q_start.is_contiguous() and kv_len.is_contiguous() and page_table.is_contiguous() and \
+        q_start.get_device() == at and kv_len.get_device() == at and page_table.get_device() == at
+    if ok and out is not None:
+        ok = out.shape == shape and out.dtype is dt and out.is_contiguous() and out.get_device() == at
+    if not ok:
+        raise ValueError("paged_attention: q [N, Hq, D] with contiguous rows, k_pages and v_pages alike [pages, Hkv, page_size, D] of its 16-bit type, q_start [B + 1], "
+                         "kv_len [B] and page_table [B, n] dense int32, out dense like q, all on one device; got " +
+                         _seen(q=q, k_pages=k_pages, v_pages=v_pages, q_start=q_start, kv_len=kv_len, page_table=page_table, out=out))
+    N, Hq, D = shape
     if out is None:
-        out = torch.empty(N, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"{what}: out must be a contiguous {tuple(q.shape)} tensor of {q.dtype}")
-    _same(what, q.device, k_pages=k_pages, v_pages=v_pages, q_start=q_start, kv_len=kv_len, page_table=page_table, out=out)
-    if N == 0 or B == 0:
-        return out
-    # from the allocator on every call: a captured graph gets a workspace of its own, calls on other streams theirs
-    need = native.load().b200_attn_paged_workspace_bytes(max_q, Hq, Hkv, D)
-    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call(q.device, what, "b200_attn_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
-          page_table.data_ptr(), B, N, max_q, Hq, Hkv, D, n_pages, page, page_table.shape[1], _S2(q.stride(0), q.stride(1)), _S3(*k_pages.stride()[:3]),
-          window, D ** -0.5 if scale is None else scale, _CODES[q.dtype], space.data_ptr() if need else None, need)
+        out = q.new_empty(shape)
+    if N and table[0]:
+        # from the allocator on every call: a captured graph gets a workspace of its own, calls on other streams theirs
+        need = _workspace_bytes(max_q, Hq, pages[1], D, native.load())
+        space = q.new_empty((need + 1) // 2)
+        native.on_stream(q.device, "paged_attention", "b200_attn_paged",
+                         _pack_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
+                                         page_table.data_ptr(), space.data_ptr(), need, table[0], N, max_q, pages[0], table[1],
+                                         qs[0], qs[1], ps[0], ps[1], ps[2], window, Hq, pages[1], D, pages[2], _CODES[dt], D ** -0.5 if scale is None else scale))
     return out
 
 

@@ -19,33 +19,26 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
     ``uniform`` fp32 ``[rows]`` in [0, 1): the random numbers.  ``temperature`` (<= 0: the arg-max), ``top_p`` (>= 1: off), ``min_p`` (<= 0: off) fp32
     and ``top_k`` int32 (<= 0: off), each ``[rows]`` or None.  Filters apply in the order top-k, top-p (of what top-k leaves), min-p (relative to the
     likeliest token); the draw goes through what is kept in the order of the token ids.  Enqueued on the current stream of the logits' device."""
-    if logits.dim() != 2 or logits.dtype not in _CODES or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.shape[1] < 1:
-        raise ValueError(f"sample_rows: logits must be [rows, cols] of a float type with contiguous columns, got {tuple(logits.shape)} {logits.dtype} "
-                         f"strides {logits.stride()}")
-    rows, cols = logits.shape
-    given = {"uniform": (uniform, torch.float32), "temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32),
-             "top_p": (top_p, torch.float32), "min_p": (min_p, torch.float32)}
-    if uniform is None:
-        raise ValueError("sample_rows: uniform is needed")
-    for name, (t, dtype) in given.items():
-        if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous() or t.device != logits.device):
-            raise ValueError(f"sample_rows: {name} must be a contiguous {dtype} tensor of {rows} numbers on {logits.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    shape, at, step = logits.shape, logits.get_device(), logits.stride()
+    ok = len(shape) == 2 and logits.dtype in _CODES and shape[1] > 0 and (step[1] == 1 or shape[1] == 1)
+    one = shape[:1]
+    places = [0, 0, 0, 0, 0]
+    for i, (t, dtype) in enumerate(((uniform, torch.float32), (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))):
+        if t is not None:
+            ok = ok and t.dtype is dtype and t.shape == one and t.is_contiguous() and t.get_device() == at
+            places[i] = t.data_ptr()
+    if ok and out is not None:
+        ok = out.dtype is torch.int64 and out.shape == one and out.is_contiguous() and out.get_device() == at
+    if not ok or uniform is None:
+        raise ValueError("sample_rows: logits [rows, cols] of a float type with contiguous columns; uniform and, where given, temperature, top_p, min_p dense fp32 and "
+                         "top_k dense int32 [rows]; out dense int64 [rows]; all on one device; got " +
+                         ", ".join(f"{n} {tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}" for n, t in
+                                   (("logits", logits), ("uniform", uniform), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("out", out))))
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    elif out.dtype != torch.int64 or tuple(out.shape) != (rows,) or not out.is_contiguous() or out.device != logits.device:
-        raise ValueError(f"sample_rows: out must be a contiguous int64 tensor of {rows} on {logits.device}")
-    if rows == 0:
-        return out
-    p = lambda t: None if t is None else t.data_ptr()
-    args = (logits.data_ptr(), out.data_ptr(), rows, cols, logits.stride(0), p(temperature), p(top_k), p(top_p), p(min_p), p(uniform), _CODES[logits.dtype])
-    lib, dev = native.load(), logits.device
-    if dev.type != "cuda":
-        native.check(lib.b200_sample_rows(*args, 0), "sample_rows")
-    elif dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            native.check(lib.b200_sample_rows(*args, torch.cuda.current_stream(dev).cuda_stream), "sample_rows")
-    else:
-        native.check(lib.b200_sample_rows(*args, torch.cuda.current_stream(dev).cuda_stream), "sample_rows")
+        out = logits.new_empty(one, dtype=torch.int64)
+    if shape[0]:
+        native.on_stream(logits.device, "sample_rows", "b200_sample_rows", logits.data_ptr(), out.data_ptr(), shape[0], shape[1], step[0], places[1], places[2],
+                         places[3], places[4], places[0], _CODES[logits.dtype])
     return out
 
 

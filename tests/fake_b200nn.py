@@ -16,6 +16,8 @@ import math
 
 import torch
 
+from cuda_runtime import native
+
 _DT = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16, 3: torch.int32, 4: torch.int64, 5: torch.uint8}
 _MAX_IN = 4
 _OPS = ("RELU", "SILU", "NEG", "RSQRT", "COS", "SIN", "ADD", "MUL", "DIV", "SUB", "ADD_S", "MUL_S", "DIV_S", "POW_S", "SUB_S",
@@ -447,9 +449,12 @@ class FakeLibrary:
     def b200_attn_paged_workspace_bytes(self, max_q, Hq, Hkv, D):
         return 256
 
-    def b200_attn_paged(self, q, kp, vp, out, q_start, kv_len, table, B, N, max_q, Hq, Hkv, D, num_pages, page, table_stride, qs, ks, window, scale, dtype,
-                        ws, ws_bytes, stream):
+    def b200_attn_paged(self, args, stream):
         self.calls.append("attn_paged")
+        a = native.AttnPagedArgs.from_buffer_copy(args)
+        q, kp, vp, out, q_start, kv_len, table, B, N, Hq, Hkv, D = (a.q, a.k_pages, a.v_pages, a.out, a.q_start, a.kv_len, a.page_table, a.B, a.n_tokens, a.Hq,
+                                                                    a.Hkv, a.D)
+        num_pages, page, table_stride, qs, ks, window, scale, dtype = a.num_pages, a.page_size, a.table_stride, a.q_strides, a.kv_strides, a.window, a.scale, a.dtype
         dt = _DT[dtype]
         Q, O = _raw(q, dt, [N, Hq, D], [*qs, 1]), _raw(out, dt, [N, Hq, D], [Hq * D, D, 1])
         K, Vv = (_raw(p, dt, [num_pages, Hkv, page, D], [*ks, 1]) for p in (kp, vp))
@@ -467,8 +472,12 @@ class FakeLibrary:
                 O[s + i] = self._attn(Q[s + i].float()[None, :, None], k.transpose(0, 1)[None], v.transpose(0, 1)[None], None, scale, dt)[0, :, 0].to(dt)
         return 0
 
-    def b200_paged_append(self, q, k, v, cos_t, sin_t, q_out, kp, vp, slots, N, Hq, Hkv, D, num_pages, page, qs, ks, vs, ps, table_dtype, dtype, stream):
+    def b200_paged_append(self, args, stream):
         self.calls.append("paged_append")
+        a = native.PagedAppendArgs.from_buffer_copy(args)
+        q, k, v, cos_t, sin_t, q_out, kp, vp, slots, N, Hq, Hkv, D = (a.q, a.k, a.v, a.cos_t, a.sin_t, a.q_out, a.k_pages, a.v_pages, a.slots, a.n_tokens, a.Hq,
+                                                                      a.Hkv, a.D)
+        num_pages, page, qs, ks, vs, ps, table_dtype, dtype = a.num_pages, a.page_size, a.q_strides, a.k_strides, a.v_strides, a.kv_strides, a.table_dtype, a.dtype
         dt, half = _DT[dtype], D // 2
         table = [_raw(t, _DT[table_dtype], [N, 1, D], [D, D, 1]).float() for t in (cos_t, sin_t)] if _addr(cos_t) else None
 

@@ -54,7 +54,7 @@ def _small():
 
 
 @pytest.mark.parametrize("change", [
-    {"q": torch.zeros(3, 4, 64)}, {"q": torch.zeros(3, 4, 128, dtype=BF)}, {"q": torch.zeros(3, 64, 4, dtype=BF).transpose(1, 2)},
+    {"q": torch.zeros(3, 4, 64)}, {"q": torch.zeros(3, 256, dtype=BF)}, {"k_pages": torch.zeros(8, 16, 64, dtype=BF)}, {"kv_len": torch.zeros((), dtype=torch.int32)}, {"q": torch.zeros(3, 4, 128, dtype=BF)}, {"q": torch.zeros(3, 64, 4, dtype=BF).transpose(1, 2)},
     {"v_pages": torch.zeros(4, 2, 32, 64, dtype=BF)}, {"q_start": torch.tensor([0, 3])}, {"q_start": torch.tensor([0, 1, 3], dtype=torch.int32)},
     {"kv_len": torch.tensor([3])}, {"page_table": torch.zeros(2, 2, dtype=torch.int32)}, {"page_table": torch.zeros(1, 2)},
     {"out": torch.zeros(3, 4, 64)}, {"out": torch.zeros(2, 4, 64, dtype=BF)}])
@@ -95,30 +95,44 @@ def test_sampling_refuses_on_the_host(fake_native, change):
 
 def _attn_args(**change):
     """Arguments of b200_attn_paged with made-up addresses: a call that must be refused before anything is launched."""
-    a = dict(q=4096, kp=4096, vp=4096, out=4096, q_start=4096, kv_len=4096, table=4096, B=1, N=3, max_q=3, Hq=4, Hkv=2, D=64, num_pages=4, page=16,
-             table_stride=2, qs=(C.c_int64 * 2)(256, 64), ks=(C.c_int64 * 3)(2048, 1024, 64), window=0, scale=0.125, dtype=2, ws=4096, ws_bytes=1 << 30, stream=0)
+    from cuda_runtime import native
+
+    a = dict(q=4096, k_pages=4096, v_pages=4096, out=4096, q_start=4096, kv_len=4096, page_table=4096, workspace=4096, workspace_bytes=1 << 30, B=1, n_tokens=3,
+             max_q=3, num_pages=4, table_stride=2, q_strides=(256, 64), kv_strides=(2048, 1024, 64), window=0, Hq=4, Hkv=2, D=64, page_size=16, dtype=2, scale=0.125)
     assert set(change) <= set(a)
-    a.update(change)
-    return list(a.values())
+    return C.byref(native.AttnPagedArgs(**{**a, **change}))
 
 
 @pytest.mark.parametrize("change,code", [
-    ({"q": 0}, -1), ({"table": 0}, -1), ({"D": 96}, -1), ({"Hq": 5}, -1), ({"Hq": 512, "Hkv": 2}, -1), ({"page": 24}, -1), ({"page": 0}, -1), ({"window": -1}, -1),
-    ({"B": -1}, -1), ({"table_stride": 0}, -1), ({"q": 4098}, -2), ({"out": 4104}, -2), ({"qs": (C.c_int64 * 2)(256, 60)}, -2),
-    ({"ks": (C.c_int64 * 3)(2048, 1024, -64)}, -2), ({"dtype": 0}, -4), ({"table_stride": 1 << 28}, -5)])
+    ({"q": 0}, -1), ({"page_table": 0}, -1), ({"D": 96}, -1), ({"Hq": 5}, -1), ({"Hq": 512, "Hkv": 2}, -1), ({"page_size": 24}, -1), ({"page_size": 0}, -1),
+    ({"window": -1}, -1), ({"B": -1}, -1), ({"table_stride": 0}, -1), ({"workspace": 0}, -1), ({"workspace_bytes": 100}, -1), ({"q": 4098}, -2), ({"out": 4104}, -2),
+    ({"workspace": 4104}, -2), ({"q_strides": (256, 60)}, -2), ({"q_strides": (256, 0)}, -2), ({"kv_strides": (2048, 1024, -64)}, -2),
+    ({"kv_strides": (0, 1024, 64)}, -2), ({"dtype": 0}, -4), ({"table_stride": 1 << 28}, -5), ({"B": 4097}, -5)])
 def test_library_refuses_attention_calls(native_lib, change, code):
-    assert native_lib.b200_attn_paged(*_attn_args(**change)) == code
+    assert native_lib.b200_attn_paged(_attn_args(**change), 0) == code
     assert native_lib.b200_last_error()
 
 
-@pytest.mark.parametrize("change,code", [({"k": 0}, -1), ({"q_out": 0}, -1), ({"cos": 0}, -1), ({"D": 24}, -1), ({"page": 0}, -1), ({"k": 4104}, -2),
-                                         ({"vs": (C.c_int64 * 2)(128, 4)}, -2), ({"table_dtype": 1}, -4), ({"dtype": 0}, -4)])
+def test_structures_and_their_packing_formats_agree():
+    import struct
+
+    from cuda_runtime import native
+
+    for cls, fmt in ((native.PagedAppendArgs, native.PAGED_APPEND_FORMAT), (native.AttnPagedArgs, native.ATTN_PAGED_FORMAT)):
+        flat = [(f, i) for f, t in cls._fields_ for i in range(t._length_ if hasattr(t, "_length_") else 1)]
+        made = cls.from_buffer_copy(struct.pack(fmt, *range(1, len(flat) + 1)))
+        got = [v for f, _ in cls._fields_ for v in (getattr(made, f) if hasattr(getattr(made, f), "__len__") else [getattr(made, f)])]
+        assert got == list(range(1, len(flat) + 1)) and struct.calcsize(fmt) == C.sizeof(cls)
+
+
+@pytest.mark.parametrize("change,code", [({"k": 0}, -1), ({"q_out": 0}, -1), ({"cos_t": 0}, -1), ({"D": 24}, -1), ({"page_size": 0}, -1), ({"k": 4104}, -2),
+                                         ({"v_strides": (128, 4)}, -2), ({"table_dtype": 1}, -4), ({"dtype": 0}, -4)])
 def test_library_refuses_append_calls(native_lib, change, code):
-    s2 = C.c_int64 * 2
-    a = dict(q=4096, k=4096, v=4096, cos=4096, sin=4096, q_out=4096, kp=4096, vp=4096, slots=4096, N=3, Hq=4, Hkv=2, D=64, num_pages=4, page=16, qs=s2(256, 64),
-             ks=s2(128, 64), vs=s2(128, 64), ps=(C.c_int64 * 3)(2048, 1024, 64), table_dtype=0, dtype=2, stream=0)
-    a.update(change)
-    assert native_lib.b200_paged_append(*a.values()) == code
+    from cuda_runtime import native
+
+    a = dict(q=4096, k=4096, v=4096, cos_t=4096, sin_t=4096, q_out=4096, k_pages=4096, v_pages=4096, slots=4096, n_tokens=3, num_pages=4, q_strides=(256, 64),
+             k_strides=(128, 64), v_strides=(128, 64), kv_strides=(2048, 1024, 64), Hq=4, Hkv=2, D=64, page_size=16, table_dtype=0, dtype=2)
+    assert native_lib.b200_paged_append(C.byref(native.PagedAppendArgs(**{**a, **change})), 0) == code
 
 
 @pytest.mark.parametrize("change,code", [({"logits": 0}, -1), ({"uniform": 0}, -1), ({"cols": 0}, -1), ({"cols": (1 << 22) + 1}, -5), ({"rows": 65536}, -5),
@@ -130,8 +144,8 @@ def test_library_refuses_sampling_calls(native_lib, change, code):
 
 
 def test_empty_calls_launch_nothing(native_lib):
-    for change in ({"B": 0}, {"N": 0}, {"max_q": 0}):
-        assert native_lib.b200_attn_paged(*_attn_args(**change)) == 0
+    for change in ({"B": 0}, {"n_tokens": 0}, {"max_q": 0}):
+        assert native_lib.b200_attn_paged(_attn_args(**change), 0) == 0
     assert native_lib.b200_sample_rows(4096, 4096, 0, 8, 8, None, None, None, None, 4096, 0, 0) == 0
 
 
@@ -529,6 +543,22 @@ def test_draw_of_equal_masked_and_odd_values(native_lib, cols):
     odd[14] = torch.finfo(F32).min
     for settings in ({}, {"top_k": k}, {"top_p": np.full(rows, 0.7)}, {"temperature": np.zeros(rows)}, {"min_p": np.full(rows, 0.3)}):
         check_draw(odd, u, **settings)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cols,rows", [(BF, 151936, 6), (F32, 151936, 70), (F32, 400001, 5), (HF, 700001, 3), (BF, 30011, 200)])
+def test_draw_from_more_than_a_list_holds(native_lib, dtype, cols, rows):
+    """Thousands of tokens kept, borders within thousands of equal logits, rows that do not fit into shared memory or start anywhere."""
+    x = logits_like(rows, cols, dtype, 3, spread=1.0)
+    r = np.random.default_rng(4)
+    u = r.random(rows)
+    for k in (2047, 2048, 2049, 5000, 20000):
+        check_draw(x, u, top_k=np.full(rows, k), temperature=np.full(rows, 2.0))
+    check_draw(x, u, temperature=np.full(rows, 3.0), top_p=r.uniform(0.5, 0.999, rows))
+    check_draw(x, u, temperature=np.full(rows, 3.0), top_p=r.uniform(0.5, 0.999, rows), top_k=r.integers(1, 30000, rows), min_p=np.full(rows, 1e-4))
+    coarse = (x.float() / 4).round().to(dtype)      # a handful of different values
+    check_draw(coarse, u, top_k=r.integers(1, cols, rows))
+    check_draw(coarse, u, top_k=r.integers(1, cols, rows), temperature=np.full(rows, 2.0), top_p=r.uniform(0.5, 0.999, rows))
 
 
 @pytest.mark.gpu
