@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   if (threadIdx.x == 0) { tc5::prefetch_tensormap(&map_k); tc5::prefetch_tensormap(&map_v); }
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
-  int64_t* const pre = reinterpret_cast<int64_t*>(smem);   // (nothing has been copied into the rings yet)
-  int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, pre, s_total);
+  const PagedWork work = paged_work(smem);   // (nothing has been copied into the rings yet)
+  int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);
   const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > FEW_MIN_SHARE ? even : FEW_MIN_SHARE;
   int64_t u0 = cta * share;
   const int64_t u1 = u0 + share < total ? u0 + share : total;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   while (u0 < u1) {
     if (warp == 0) {
       int count;
-      const int64_t next = paged_pieces<FEW_KEYS, FEW_OV>(p, tpt, pre, u0, u1, share, s_piece, count, head);
+      const int64_t next = paged_pieces<FEW_KEYS, FEW_OV>(p, tpt, work, u0, u1, share, s_piece, count, head);
       __syncwarp();
       if (lane == 0) {
         s_next = next;
@@ -319,25 +319,29 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
       __syncthreads();
       if (parked >= 0) copy();
     }
-    if (u0 < u1) total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, pre, s_total);   // (the rings lay over the running costs)
+    if (u0 < u1) total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);   // (the rings lay over the running costs)
   }
   if (threadIdx.x == 0) p.head[cta] = head;
 }
 
 // ===========================================================================
-// Joins the pieces of items that several blocks had a part in, in the order of the blocks.  RB rows of an item at a time, a thread per four dims;
-// every block goes through the list of such items (at most one begins in each block of the kernel before).
+// Joins the pieces of items that several blocks had a part in, in the order of the blocks (their sums are the same whoever adds them up).  A thread
+// per four dims; 256 / (D / 4) rows of an item at a time, or one row with as many groups of pieces where there are many pieces: then a thread's
+// chain of loads is short (71 pieces: 17.2 us with one group).  Every block goes through the list of such items (at most one begins in each
+// block of the kernel before).
 // ===========================================================================
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int RB = 256 / (D / 4);
+  constexpr int LPR = D / 4, RB = 256 / LPR, BATCH = 6;
   __shared__ int s_upto[PAGED_CTAS + 1], s_sum[8];
+  __shared__ __align__(16) float s_acc[RB][D];
+  __shared__ float s_m[RB], s_l[RB];
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int4 h = make_int4(0, 0, 0, 0);
   if (threadIdx.x < PAGED_CTAS) h = __ldg(p.head + threadIdx.x);
-  const int mine = h.x > 0 ? (h.w + RB - 1) / RB : 0;   // tasks of this item
+  const int mine = h.x > BATCH ? h.w : h.x > 0 ? (h.w + RB - 1) / RB : 0;   // tasks of this item
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
   if (threadIdx.x < PAGED_CTAS) s_upto[threadIdx.x + 1] = upto;
   if (threadIdx.x == 0) s_upto[0] = 0;
   __syncthreads();
-  const int tasks = s_upto[PAGED_CTAS];
+  const int tasks = s_upto[PAGED_CTAS], g = threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
     int lo = 0, hi = PAGED_CTAS;   // the item: the last one whose tasks begin at or before this one
     while (hi - lo > 1) {
@@ -358,41 +362,62 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
       if (s_upto[mid] <= task) lo = mid; else hi = mid;
     }
     const int4 it = __ldg(p.head + lo);
-    const int r = (task - s_upto[lo]) * RB + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    if (r >= it.w) continue;
+    const bool many = it.x > BATCH;
+    const int r = many ? task - s_upto[lo] : (task - s_upto[lo]) * RB + g, step = many ? RB : 1;
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int BATCH = 8;
-    for (int i0 = 0; i0 < it.x; i0 += BATCH) {
-      float2 ml[BATCH];
-      float4 a[BATCH];
+    if (r < it.w)
+      for (int i0 = many ? g : 0; i0 < it.x; i0 += BATCH * step) {
+        float2 ml[BATCH];
+        float4 a[BATCH];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        ml[i] = make_float2(-INFINITY, 0.f);
-        a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i0 + i < it.x) {
-          const int64_t slot = paged_slot(lo + i0 + i, i0 + i == 0, ROWS) + r;
-          ml[i] = __ldg(p.ml + slot);
-          a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
+        for (int i = 0; i < BATCH; ++i) {
+          const int at = i0 + i * step;
+          ml[i] = make_float2(-INFINITY, 0.f);
+          a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at < it.x) {
+            const int64_t slot = paged_slot(lo + at, at == 0, ROWS) + r;
+            ml[i] = __ldg(p.ml + slot);
+            a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
+          }
         }
-      }
-      float top = m;
+        float top = m;
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float c = ex2_approx(m - ref);
-      l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
+        for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float c = ex2_approx(m - ref);
+        l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const float f = ex2_approx(ml[i].x - ref);
-        l += ml[i].y * f;
-        acc.x += a[i].x * f; acc.y += a[i].y * f; acc.z += a[i].z * f; acc.w += a[i].w * f;
+        for (int i = 0; i < BATCH; ++i) {
+          const float f = ex2_approx(ml[i].x - ref);
+          l += ml[i].y * f;
+          acc.x += a[i].x * f; acc.y += a[i].y * f; acc.z += a[i].z * f; acc.w += a[i].w * f;
+        }
+        m = top;
       }
-      m = top;
+    T* const o = static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D;
+    if (!many) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (r < it.w) *reinterpret_cast<uint2*>(o + d) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      continue;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    T* const o = static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D + d;
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<float4*>(&s_acc[g][d]) = acc;
+    if (d == 0) { s_m[g] = m; s_l[g] = l; }
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float top = -INFINITY, sum = 0.f, a = 0.f;
+#pragma unroll
+      for (int e = 0; e < RB; ++e) top = fmaxf(top, s_m[e]);
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int e = 0; e < RB; ++e) {
+        const float f = ex2_approx(s_m[e] - ref);
+        sum += s_l[e] * f;
+        a += s_acc[e][threadIdx.x] * f;
+      }
+      o[threadIdx.x] = from_f32<T>(sum > 0.f ? a / sum : 0.f);
+    }
+    __syncthreads();
   }
 }
 

@@ -64,21 +64,41 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   return v;
 }
 
-// pre[b] = cost of the sequences before b, b = 0..B (shared memory); returns pre[B].  All THREADS threads; ends with a barrier.
-template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const PagedParams& p, int tpt, int64_t* pre, int64_t* warp_total) {
+// What every block keeps of the sequences while it looks for its pieces (shared memory)
+struct PagedWork {
+  int64_t* pre;        // [B + 1]: cost of the sequences before b
+  int32_t *first, *n;  // [B]: first token, keys
+  int32_t* T;          // [B]: tokens
+};
+constexpr int paged_work_bytes = PAGED_MAX_SEQS * 20 + 8;
+__device__ __forceinline__ PagedWork paged_work(void* at) {
+  PagedWork w;
+  w.pre = static_cast<int64_t*>(at);
+  w.first = reinterpret_cast<int32_t*>(w.pre + PAGED_MAX_SEQS + 1);
+  w.n = w.first + PAGED_MAX_SEQS;
+  w.T = w.n + PAGED_MAX_SEQS;
+  return w;
+}
+
+// Fills `w`; returns pre[B].  All THREADS threads; ends with a barrier.
+template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const PagedParams& p, int tpt, const PagedWork& w, int64_t* warp_total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = static_cast<int>(p.B);
   const int chunk = (B + THREADS - 1) / THREADS;
   int64_t run = 0;
   for (int c = 0; c < chunk; ++c) {
     const int b = threadIdx.x * chunk + c;
     PagedSeq s = {0, 0, 0};
-    if (b < B) s = paged_seq(p, b);
+    if (b < B) {
+      s = paged_seq(p, b);
+      w.first[b] = static_cast<int>(s.first);
+      w.n[b] = static_cast<int>(s.n);
+      w.T[b] = s.T;
+    }
     const int tiles = (s.T + tpt - 1) / tpt;
     int64_t cost = 0;
-    if (tiles <= 2)
-      for (int i = 0; i < tiles; ++i) cost += paged_tile<KT>(p, s.T, s.n, i, tpt).cnt + OV;
+    if (tiles == 1) cost = paged_tile<KT>(p, s.T, s.n, 0, tpt).cnt + OV;
     // a prompt's many tiles: the whole warp adds them up
-    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 2); many; many &= many - 1) {
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > 1); many; many &= many - 1) {
       const int src = __ffs(many) - 1, T = __shfl_sync(0xffffffffu, s.T, src), nt = (T + tpt - 1) / tpt;
       const int64_t n = __shfl_sync(0xffffffffu, s.n, src);
       int64_t sum = 0;
@@ -87,7 +107,7 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
       if (lane == src) cost = sum;
     }
     run += cost * p.Hkv;
-    if (b < B) pre[b + 1] = run;
+    if (b < B) w.pre[b + 1] = run;
   }
   int64_t upto = run;
 #pragma unroll
@@ -98,15 +118,16 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
   if (lane == 31) warp_total[warp] = upto;
   __syncthreads();
   int64_t before = upto - run, total = 0;
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warp_total[w];
-    total += warp_total[w];
+#pragma unroll
+  for (int v = 0; v < THREADS / 32; ++v) {
+    if (v < warp) before += warp_total[v];
+    total += warp_total[v];
   }
   for (int c = 0; c < chunk; ++c) {
     const int b = threadIdx.x * chunk + c;
-    if (b < B) pre[b + 1] += before;
+    if (b < B) w.pre[b + 1] += before;
   }
-  if (threadIdx.x == 0) pre[0] = 0;
+  if (threadIdx.x == 0) w.pre[0] = 0;
   __syncthreads();
   return total;
 }
@@ -114,26 +135,31 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
 // The pieces of items in the costs [u0, u1), at most PAGED_MAX_PIECES; returns where to go on (u1: that was all).  One whole warp.
 // head is written where an item begins in this block and does not end in it: how many blocks have pieces of it, and whose rows they are.
 template <int KT, int OV>
-__device__ int64_t paged_pieces(const PagedParams& p, int tpt, const int64_t* pre, int64_t u0, int64_t u1, int64_t share, PagedPiece* list, int& count, int4& head) {
+__device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& w, int64_t u0, int64_t u1, int64_t share, PagedPiece* list, int& count, int4& head) {
   const int lane = threadIdx.x & 31, B = static_cast<int>(p.B);
   count = 0;
   int lo = 0, hi = B;   // the last sequence that begins at or before u0 (and so is not empty)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= u0) lo = mid; else hi = mid;
+    if (w.pre[mid] <= u0) lo = mid; else hi = mid;
   }
-  for (int b = lo; b < B && pre[b] < u1; ++b) {
-    if (pre[b + 1] <= u0 || pre[b + 1] == pre[b]) continue;
-    const PagedSeq s = paged_seq(p, b);
-    const int tiles = (s.T + tpt - 1) / tpt;
-    const int64_t per_head = (pre[b + 1] - pre[b]) / p.Hkv;
-    const int64_t skip = u0 > pre[b] ? (u0 - pre[b]) / per_head : 0;
-    int64_t base = pre[b] + skip * per_head;
-    const int64_t items = static_cast<int64_t>(p.Hkv) * tiles;
-    for (int64_t e0 = skip * tiles; e0 < items && base < u1; e0 += 32) {
-      const int64_t e = e0 + lane;
+  for (int b = lo; b < B && w.pre[b] < u1; ++b) {
+    const int64_t begin = w.pre[b], all = w.pre[b + 1] - begin;
+    if (begin + all <= u0 || all == 0) continue;
+    const int T = w.T[b], first = w.first[b], tiles = (T + tpt - 1) / tpt;
+    const int64_t n = w.n[b];
+    int skip = 0;   // heads ahead of u0
+    int64_t base = begin;
+    if (u0 > begin && p.Hkv > 1) {
+      const int64_t per_head = all / p.Hkv;
+      skip = static_cast<int>((u0 - begin) / per_head);
+      base += skip * per_head;
+    }
+    const int items = p.Hkv * tiles;
+    for (int e0 = skip * tiles; e0 < items && base < u1; e0 += 32) {
+      const int e = e0 + lane, h = e / tiles;
       PagedTile t = {0, 0, 0, 0, 0};
-      if (e < items) t = paged_tile<KT>(p, s.T, s.n, static_cast<int>(e % tiles), tpt);
+      if (e < items) t = paged_tile<KT>(p, T, n, e - h * tiles, tpt);
       const int64_t cost = e < items ? t.cnt + OV : 0;
       int64_t upto = cost;
 #pragma unroll
@@ -141,15 +167,15 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const int64_t* pr
         const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const int64_t start = base + upto - cost + OV, end = base + upto, a = max(u0, start), z = min(u1, end);
+      const int64_t start = base + upto - cost + OV, end = base + upto, a = u0 > start ? u0 : start, z = u1 < end ? u1 : end;
       const unsigned mine = __ballot_sync(0xffffffffu, e < items && a < z);
       const int at = count + __popc(mine & ((1u << lane) - 1u));
       const bool taken = ((mine >> lane) & 1u) && at < PAGED_MAX_PIECES;
       if (taken) {
         PagedPiece f;
         f.b = b;
-        f.hk = static_cast<int>(e / tiles);
-        f.token = static_cast<int>(s.first) + t.t0;
+        f.hk = h;
+        f.token = first + t.t0;
         f.rows = (t.t1 - t.t0) * p.G;
         f.p0 = static_cast<int>(t.p0);
         f.j0 = t.j0 + static_cast<int>(a - start);
@@ -161,9 +187,9 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const int64_t* pr
       const unsigned opens = __ballot_sync(0xffffffffu, taken && a == start && z < end);
       if (opens) {
         const int src = __ffs(opens) - 1;
-        head.x = __shfl_sync(0xffffffffu, static_cast<int>((end - 1) / share - start / share) + 1, src);
-        head.y = __shfl_sync(0xffffffffu, static_cast<int>(s.first) + t.t0, src);
-        head.z = __shfl_sync(0xffffffffu, static_cast<int>(e / tiles), src);
+        head.x = static_cast<int>((__shfl_sync(0xffffffffu, end, src) - 1) / share - __shfl_sync(0xffffffffu, start, src) / share) + 1;
+        head.y = __shfl_sync(0xffffffffu, first + t.t0, src);
+        head.z = __shfl_sync(0xffffffffu, h, src);
         head.w = __shfl_sync(0xffffffffu, (t.t1 - t.t0) * p.G, src);
       }
       count += __popc(mine);

@@ -12,7 +12,7 @@
 // has grown by more than RESCALE_STEP.  A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
 // next item's first tile are computed while the last one's rows are written.
 //
-// Warp roles: warps 0-3 and 4-7 the softmax groups, warp 8 MMA issuer and owner of the tensor memory, warp 9 TMA producer, a box per lane.  Every
+// Warp roles: warps 0-3 and 4-7 the softmax groups, warp 8 MMA issuer and owner of the tensor memory, warps 9 and 10 TMA producers (Q and K; V), a box per lane.  Every
 // barrier wait is bounded; on a time-out the block records a code, stops issuing, waits for its copies, frees its tensor memory and returns.
 #include "attn_paged.cuh"
 #include "gemm_tc5.cuh"
@@ -26,7 +26,7 @@ namespace {
 
 constexpr int BKV = 128;
 constexpr int PANEL = 128 * 128;               // [128 rows][128 bytes]: 64 columns of an operand tile
-constexpr int THREADS = 320;
+constexpr int THREADS = 352;
 constexpr int OV = 1;                          // what an item costs besides its tiles, in tiles
 constexpr int MIN_SHARE = 2;                   // tiles (and OVs) of a block at least
 constexpr float LOG2E_F = 1.4426950408889634f;
@@ -88,9 +88,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 8) { tc5::tmem_alloc(&tmem_holder, TMEM_COLS); tc5::tmem_relinquish(); }
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
-  int64_t* const pre = reinterpret_cast<int64_t*>(p_s);
+  const PagedWork work = paged_work(smem);   // (no tile has been copied yet)
   tc5::tc_fence_before();
-  int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, pre, s_total);
+  int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);
   tc5::tc_fence_after();
   const uint32_t tmem_base = tmem_holder;
   const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > MIN_SHARE ? even : MIN_SHARE;
@@ -102,71 +102,74 @@ __global__ void __launch_bounds__(THREADS, 1)
   while (u0 < u1) {
     if (warp == 0) {
       int count;
-      const int64_t next = paged_pieces<BKV, OV>(p, tpt, pre, u0, u1, share, s_piece, count, head);
+      const int64_t next = paged_pieces<BKV, OV>(p, tpt, work, u0, u1, share, s_piece, count, head);
       if (lane == 0) { s_next = next; s_count = count; }
     }
+    tc5::fence_proxy_async();   // the tiles are copied over what has been written here
     __syncthreads();
     const int F = s_count;
     u0 = s_next;
 
-    if (warp == 9) {   // ---- TMA producer: lane l brings rows [l * box, (l + 1) * box) of a tile ----
+    if (warp >= 9) {   // ---- TMA producers, of Q and K and of V: lane l brings rows [l * box, (l + 1) * box) of a tile ----
+      const bool is_k = warp == 9;
+      const CUtensorMap* const map = is_k ? &map_k : &map_v;
+      uint64_t *const full = is_k ? k_full : v_full, *const empty = is_k ? k_empty : v_empty;
+      uint8_t* const tiles = (is_k ? k_s : v_s) + lane * box * 128;
       bool ok = true;
       int q_at = fg, kv_at = n;   // copies issued
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        bool got = tc5::mbar_wait(bar, parity);
-        got = __all_sync(0xffffffffu, got) && !*reinterpret_cast<volatile int*>(&failed);
-        if (!got && lane == 0 && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, code); }
-        return __all_sync(0xffffffffu, got);
+        const bool got = __all_sync(0xffffffffu, tc5::mbar_wait(bar, parity));
+        const bool gone = *reinterpret_cast<volatile int*>(&failed) != 0;
+        if (!got && !gone && lane == 0) { failed = 1; atomicExch(&g_attn_paged_error, code); }
+        return __all_sync(0xffffffffu, got && !gone);
       };
-      int at = n;
-      for (int f = 0; f < F && ok; ++f) {
-        const PagedPiece c = s_piece[f];
+      // the lane's rows of a tile: page and first row, looked up a tile ahead (a page number is a round trip to L2)
+      struct Rows { int page, row; bool there; };
+      auto locate = [&](const PagedPiece& c, int k) {
         const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
         const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
-        const int32_t* const pages = p.table + c.b * p.table_stride;
-        for (int k = 0; k < c.cnt && ok; ++k, ++at) {
-          const int st = at & 1, key = (c.j0 + k) * BKV + lane * box;
-          const bool there = lane * box < BKV && key < hi && key + box > lo;
-          const unsigned present = __ballot_sync(0xffffffffu, there);
-          int page = 0, row = 0;
-          if (there) {
-            const int i = key / p.page_size;
-            row = key - i * p.page_size;
-            page = __ldg(pages + i);
-            if (page < 0 || page >= p.num_pages) page = static_cast<int>(p.num_pages);   // outside the tensor: zeros
-          }
-          const uint32_t bytes = static_cast<uint32_t>(__popc(present)) * box * 128 * NP, parity = ((at >> 1) & 1) ^ 1;
-          if (at >= 2 && !(ok = wait(&k_empty[st], parity, 50))) break;
-          if (k == 0) {
+        const int key = (c.j0 + k) * BKV + lane * box;
+        Rows a = {0, 0, lane * box < BKV && key < hi && key + box > lo};
+        if (a.there) {
+          const int i = key / p.page_size;
+          a.row = key - i * p.page_size;
+          a.page = __ldg(p.table + c.b * p.table_stride + i);
+        }
+        return a;
+      };
+      int at = n;
+      PagedPiece c = s_piece[0];
+      Rows next = locate(c, 0);
+      for (int f = 0; f < F && ok; ++f) {
+        const int cnt = c.cnt, hk = c.hk, token = c.token;
+        for (int k = 0; k < cnt && ok; ++k, ++at) {
+          const int st = at & 1;
+          const Rows a = next;
+          if (k + 1 < cnt) next = locate(c, k + 1);
+          else if (f + 1 < F) { c = s_piece[f + 1]; next = locate(c, 0); }
+          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, a.there))) * box * 128 * NP;
+          if (at >= 2 && !(ok = wait(&empty[st], ((at >> 1) & 1) ^ 1, is_k ? 50 : 52))) break;
+          if (is_k && k == 0) {
             if (fg + f >= 1 && !(ok = wait(&q_empty, (fg + f - 1) & 1, 51))) break;
             if (lane == 0) {
               tc5::mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.G) * tpt * 128 * NP);
-              for (int h = 0; h < NP; ++h) tc5::tma_load_4d(q_s + h * PANEL, &map_q, &q_full, 0, c.hk * p.G, c.token, h);
+              for (int h = 0; h < NP; ++h) tc5::tma_load_4d(q_s + h * PANEL, &map_q, &q_full, 0, hk * p.G, token, h);
             }
             ++q_at;
           }
-          if (lane == 0) tc5::mbar_arrive_expect_tx(&k_full[st], bytes);
+          if (lane == 0) tc5::mbar_arrive_expect_tx(&full[st], bytes);
           __syncwarp();
-          if (there)
-            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(k_s + st * TILE + h * PANEL + lane * box * 128, &map_k, &k_full[st], 0, row, h, c.hk, page);
-          if (at >= 2 && !(ok = wait(&v_empty[st], parity, 52))) {
-            tc5::mbar_wait(&k_full[st], (at >> 1) & 1, 1u << 16);   // the copies just issued
-            break;
+          if (a.there) {
+            const int page = a.page < 0 || a.page >= p.num_pages ? static_cast<int>(p.num_pages) : a.page;   // outside the tensor: zeros
+            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(tiles + st * TILE + h * PANEL, map, &full[st], 0, a.row, h, hk, page);
           }
-          if (lane == 0) tc5::mbar_arrive_expect_tx(&v_full[st], bytes);
-          __syncwarp();
-          if (there)
-            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(v_s + st * TILE + h * PANEL + lane * box * 128, &map_v, &v_full[st], 0, row, h, c.hk, page);
           kv_at = at + 1;
         }
       }
       // on a failure elsewhere the copies in flight must land before the block leaves
       if (*reinterpret_cast<volatile int*>(&failed)) {
-        if (q_at > 0) tc5::mbar_wait(&q_full, (q_at - 1) & 1, 1u << 16);
-        for (int i = kv_at > 2 ? kv_at - 2 : 0; i < kv_at; ++i) {
-          tc5::mbar_wait(&k_full[i & 1], (i >> 1) & 1, 1u << 16);
-          tc5::mbar_wait(&v_full[i & 1], (i >> 1) & 1, 1u << 16);
-        }
+        if (is_k && q_at > 0) tc5::mbar_wait(&q_full, (q_at - 1) & 1, 1u << 16);
+        for (int i = kv_at > 2 ? kv_at - 2 : 0; i < kv_at; ++i) tc5::mbar_wait(&full[i & 1], (i >> 1) & 1, 1u << 16);
       }
     } else if (warp == 8) {
       if (lane == 0) {   // ---- MMA issuer ----
@@ -346,37 +349,60 @@ __global__ void __launch_bounds__(THREADS, 1)
             w_0 *= inv;
             w_1 *= inv;
           }
-          const int64_t slot = paged_slot(cta, pc.flags & 1, PAGED_TC5_ROWS) + r;
-          float* const part = p.acc + slot * D + g * (D / 2);
-          T* const orow = static_cast<T*>(p.out) + ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
-          if (!whole && g == 0 && row_live) p.ml[slot] = make_float2(m_all, l_all);
-#pragma unroll 1
-          for (int q = 0; q < D / 2; q += 16) {
-            float t0[16], t1[16];
-            tc5::tmem_ld_32x16(t_lane + 256 + g * (D / 2) + q, t0);
-            tc5::tmem_ld_32x16(t_lane + 384 + g * (D / 2) + q, t1);
-            tc5::tmem_ld_wait();
-            float o[16];
+          const int64_t slot = paged_slot(cta, pc.flags & 1, PAGED_TC5_ROWS);
+          if (!whole && g == 0 && row_live) p.ml[slot + r] = make_float2(m_all, l_all);
+          // Through this warp's rows of the probability buffers (chunk c of row r at c ^ (r & 7)), so that rows leave in whole lines
+          uint8_t* const own = p_s + g * PANEL + 32 * quarter * 128;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = fmaf(t1[e], w_1, t0[e] * w_0);
-            if (row_live) {
-              if (whole) {
-                reinterpret_cast<uint4*>(orow + q)[0] = pack8<T>(*reinterpret_cast<float(*)[8]>(&o[0]));
-                reinterpret_cast<uint4*>(orow + q)[1] = pack8<T>(*reinterpret_cast<float(*)[8]>(&o[8]));
-              } else {
-                tc5::st_global_f8(part + q, o);
-                tc5::st_global_f8(part + q + 8, o + 8);
-              }
+          for (int q = 0; q < D / 2; q += 32) {
+            float t0[32], t1[32];
+            tc5::tmem_ld_32x32_async(t_lane + 256 + g * (D / 2) + q, t0);
+            tc5::tmem_ld_32x32_async(t_lane + 384 + g * (D / 2) + q, t1);
+            tc5::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) { t0[e] = fmaf(t1[e], w_1, t0[e] * w_0); t0[e + 1] = fmaf(t1[e + 1], w_1, t0[e + 1] * w_0); }
+            if (whole) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(own + lane * 128 + (((q / 8 + e) ^ (r & 7)) << 4)) = pack8<T>(*reinterpret_cast<float(*)[8]>(&t0[8 * e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(own + (q / 32) * 2 * PANEL + lane * 128 + ((e ^ (r & 7)) << 4)) = *reinterpret_cast<float4*>(&t0[4 * e]);
             }
           }
           tc5::tc_fence_before();
+          __syncwarp();
+          const int live = pc.rows - 32 * quarter < 32 ? pc.rows - 32 * quarter : 32;   // rows of this warp
+          if (whole) {
+            constexpr int CH = D / 16;   // 16-byte chunks of half a row
+            const int64_t to = ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
+#pragma unroll
+            for (int it = 0; it < CH; ++it) {
+              const int row = it * (32 / CH) + lane / CH, ch = lane % CH;
+              const int64_t dst = __shfl_sync(0xffffffffu, to, row);
+              if (row < live)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + dst + ch * 8) = *reinterpret_cast<const uint4*>(own + row * 128 + ((ch ^ (row & 7)) << 4));
+            }
+          } else {
+            constexpr int CH = D / 8;
+            float* const part = p.acc + (slot + 32 * quarter) * D + g * (D / 2);
+#pragma unroll
+            for (int it = 0; it < CH; ++it) {
+              const int row = it * (32 / CH) + lane / CH, ch = lane % CH;
+              if (row < live)
+                *reinterpret_cast<float4*>(part + static_cast<int64_t>(row) * D + ch * 4) =
+                    *reinterpret_cast<const float4*>(own + (ch / 8) * 2 * PANEL + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+            }
+          }
+          __syncwarp();
         }
       }
     }
     for (int f = 0; f < F; ++f) n += s_piece[f].cnt;
     fg += F;
     if (__syncthreads_or(*reinterpret_cast<volatile int*>(&failed))) break;   // (what the threads see may differ: they agree)
-    if (u0 < u1) total = paged_prefix<BKV, OV, THREADS>(p, tpt, pre, s_total);   // (the probabilities lay over the running costs)
+    if (u0 < u1) total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);   // (the tiles lay over it)
   }
   if (threadIdx.x == 0) p.head[cta] = head;
   tc5::tc_fence_before();
