@@ -11,10 +11,11 @@
 // rare token is wide).  Thresholds are found on the logits themselves, never on weights.
 //
 // A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once (a bulk copy per warp)
-// and then goes through several times: for the maximum; for counts or weights in 16 intervals of z, then in 16 parts of the interval in which the k-th token or
-// the top_p-th part of the sum lies, and so on (private counters per lane: no atomics) until few enough tokens are left to be
-// sorted; for the tokens to be sorted.  Mostly all that is kept is in that list, and its CTA finishes alone; where more is kept than a list
-// holds, the list gives the last token kept and the row is drawn from by sums over ranges.
+// and then goes through a few times: for the maximum; for the sum of the weights where it is needed (about 15 instructions a token: that, and not the memory, is
+// what most of the time goes into); for the tokens that are large enough to matter. How large that is the maxima of the threads' own
+// tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are sorted by one CTA, which mostly finds everything
+// that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or weights in 16 intervals of z, then in 16 parts
+// of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is drawn from by sums over ranges.
 #include "common.cuh"
 #include "tc5.cuh"
 
@@ -53,24 +54,29 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T, by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a table for
-// the first eight, a cubic for the rest (its next term is below 2^-38).  The difference and its product with log2(e) / T are carried as
-// pairs of fp32 numbers: a rounding of t = 30 alone would be 2^-20 of the weight.
-struct Weigher {
+// exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  The difference and its product with log2(e) / T are carried as pairs of fp32 numbers: a rounding
+// of t = 30 alone would be 2^-20 of the weight.  Below t = 16 by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a
+// table for the first eight, a cubic for the rest (its next term is below 2^-38).  From there on, where most tokens lie, a weight is below 2^24 units and
+// the fast exponential of the fraction (2^-22 of itself) is as good.
+template <typename T> struct Weigher {
   float m, c_hi, c_lo;
   const uint32_t* table;   // 2^31 2^-(i / 256)
-  __device__ __forceinline__ u64 operator()(float z) const {
-    if (z == m) return ONE;
-    const float dh = m - z, bv = m - dh, dl = (m - (dh + bv)) + (bv - z);
-    const float p = __fmul_rn(dh, c_hi);
-    if (!(p < 41.f)) return 0;   // (a NaN or an infinite difference as well)
-    const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, dl * c_hi);
+  __device__ __forceinline__ float rest(float z, float dh) const {   // (m - z) - dh
+    const float bv = m - dh;
+    return (m - (dh + bv)) + (bv - z);
+  }
+  // p = fp32((m - z) c_hi), dh = fp32(m - z); for p < 41
+  __device__ __forceinline__ uint32_t small(float z, float dh, float p) const {
+    float e = fmaf(dh, c_lo, fmaf(dh, c_hi, -p));
+    if constexpr (sizeof(T) == 4) e = fmaf(rest(z, dh), c_hi, e);   // (differences of 16-bit logits are whole but for those next to zero)
+    const float shifted = p + 12582912.f, frac = p - (shifted - 12582912.f);   // (to the nearest whole number)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-frac - e));
+    return __float2uint_rz(y * __uint_as_float((167u << 23) - (__float_as_uint(shifted) << 23)));   // 2^(40 - whole)
+  }
+  __device__ __forceinline__ u64 large(float z, float dh, float p) const {   // (ONE for z == m)
+    const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, rest(z, dh) * c_hi);
     const float ip = floorf(p);
-    if (p >= 16.f) {   // most tokens: below 2^24 units, where the fast exponential of the fraction (2^-22 of itself) is as good
-      float y;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((ip - p) - e));
-      return __float2uint_rz(y * __int_as_float((167 - static_cast<int>(ip)) << 23));   // 2^(40 - ip)
-    }
     int64_t t = (static_cast<int64_t>(ip) << 32) + static_cast<int64_t>(__float2uint_rz((p - ip) * 4294967296.f)) + static_cast<int64_t>(__float2int_rn(e * 4294967296.f));
     t = t < 0 ? 0 : t;
     const uint32_t f = static_cast<uint32_t>(t);
@@ -80,17 +86,47 @@ struct Weigher {
     const uint32_t w = tab - static_cast<uint32_t>((static_cast<u64>(tab) * __float2uint_rn(q * 4294967296.f) + 0x80000000ull) >> 32);
     return (static_cast<u64>(w) << 9) >> static_cast<int>(t >> 32);
   }
+  __device__ __forceinline__ float far(float z, float& dh) const {   // p; not below 41 for what weighs nothing and for NaN
+    dh = m - z;
+    return __fmul_rn(dh, c_hi);
+  }
+  __device__ __forceinline__ u64 at(float z, float dh, float p) const { return p >= 16.f ? small(z, dh, p) : large(z, dh, p); }
+  __device__ __forceinline__ u64 operator()(float z) const {
+    float dh;
+    const float p = far(z, dh);
+    return p < 41.f ? at(z, dh, p) : 0;
+  }
+  // sum over eight tokens, straight through for the many that are far from the maximum
+  __device__ __forceinline__ u64 sum(const float (&z)[8]) const {
+    float p[8], dh[8], nearest = 41.f;
+    uint32_t s = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      p[k] = fminf(far(z[k], dh[k]), 41.f);   // (41, as for NaN: half a unit, which is none)
+      nearest = fminf(nearest, p[k]);
+    }
+    if (nearest >= 16.f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += small(z[k], dh[k], p[k]);
+      return s;
+    }
+    u64 t = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += p[k] < 16.f ? large(z[k], dh[k], p[k]) : small(z[k], dh[k], p[k]);
+    return t;
+  }
 };
+constexpr float END = 41.f;
 
 struct Shared {
   uint32_t table[256];
   u64 part[SW];
   u64 told[2][MAX_CTAS];   // values of all CTAs of the row, two exchanges deep
   u64 bin_mass[SW][BINS], told_mass[2][MAX_CTAS][BINS];
-  uint32_t bin_count[SW][BINS], told_count[2][MAX_CTAS][BINS];
+  uint32_t bin_count[SW][32], told_count[2][MAX_CTAS][32];
   u64 cut_last;            // from the list: key << 32 | index of the last token kept
   int listed;
-  int pick[2];
+  int pick[2], verdict;
   __align__(8) uint64_t full[SW];
 };
 
@@ -100,7 +136,14 @@ template <typename T> struct Row {
   const T* copy;             // of this warp's range, or nullptr
   int begin, end, copied;    // columns begin .. copied - 1 are in the copy
   bool vec;
+  bool infinite = false;     // the maximum is +infinity: as if it were 0 and all else -infinity
   __device__ __forceinline__ void load(int c, float (&f)[8]) const {   // columns c .. c + 7; those past the end as NaN
+    fetch(c, f);
+    if (infinite)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = f[k] == INFINITY ? 0.f : -INFINITY;
+  }
+  __device__ __forceinline__ void fetch(int c, float (&f)[8]) const {
     if (c + 8 <= copied) {
       unpack(copy + (c - begin), f);
     } else if (vec && c + 8 <= end) {
@@ -116,6 +159,14 @@ template <typename T> struct Row {
     } else {
       const float4 a = *reinterpret_cast<const float4*>(at), b = *(reinterpret_cast<const float4*>(at) + 1);
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+  }
+  template <typename F> __device__ __forceinline__ void packs(F&& f) const {
+#pragma unroll 2
+    for (int c = begin + (threadIdx.x & 31) * 8; c < end; c += 256) {
+      float v[8];
+      load(c, v);
+      f(v, c);
     }
   }
   template <typename F> __device__ __forceinline__ void each(F&& f) const {
@@ -167,16 +218,38 @@ template <bool TOP> __device__ u64 row_reduce(u64 v, Shared& sh, int ctas, int& 
 
 // list[0 .. n) in descending order; n a power of two.  All threads; begins and ends with a barrier.
 __device__ void sort_list(u64* list, int n) {
+  __syncthreads();
+  if (n <= ST) {   // an element per thread: steps within a warp by shuffles
+    const int i = threadIdx.x;
+    u64 v = i < n ? list[i] : 0;
+    for (int size = 2; size <= n; size <<= 1)
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        u64 w;
+        if (step >= 32) {
+          __syncthreads();
+          if (i < n) list[i] = v;
+          __syncthreads();
+          w = i < n ? list[i ^ step] : 0;
+        } else {
+          w = __shfl_xor_sync(0xffffffffu, v, step);
+        }
+        const bool larger = ((i & step) == 0) == ((i & size) == 0);   // the larger of the two stays here
+        v = larger == (w > v) ? w : v;
+      }
+    __syncthreads();
+    if (i < n) list[i] = v;
+    __syncthreads();
+    return;
+  }
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
       for (int i = threadIdx.x; i < n / 2; i += ST) {
         const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
         const u64 a = list[lo], b = list[hi];
         if ((a < b) == ((lo & size) == 0)) { list[lo] = b; list[hi] = a; }
       }
+      __syncthreads();
     }
-  __syncthreads();
 }
 
 // sums[i] = val(0) + .. + val(i) for i < n <= CAP (four to a thread).  All threads; ends with a barrier.
@@ -251,24 +324,32 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer; the table is there
   if (row.copied > row.begin && !tc5::mbar_wait(&sh.full[warp], 0) && lane == 0) atomicExch(&g_sample_error, 70);
 
-  // ---- the maximum, and of equal ones the lowest index ----
-  u64 best = 0;
-  {
-    float top = -INFINITY;   // (a lane's columns come in rising order: of equal ones the first stays)
-    int at = -1;
-    row.each([&](float z, int c) {
-      if (z > top) { top = z; at = c; }
-    });
-    if (at >= 0) best = static_cast<u64>(key_of(top)) << 32 | static_cast<uint32_t>(~at);
-  }
-  best = row_reduce<true>(best, sh, ctas, turn);
-  if (!(T_ > 0.f) || best == 0) {   // greedy; a row without any weight gives its first token
-    if (rank == 0 && threadIdx.x == 0) p.out[r] = best == 0 ? 0 : static_cast<int>(~static_cast<uint32_t>(best));
+  // ---- the maximum ----
+  float top = -INFINITY;   // of this thread's tokens (NaN is none)
+  row.packs([&](const float (&z)[8], int) {
+    top = fmaxf(top, fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))));
+  });
+  const u64 best = row_reduce<true>(key_of(top), sh, ctas, turn);
+  float m = value_of(static_cast<uint32_t>(best));
+  if (!(T_ > 0.f) || m == -INFINITY) {   // greedy: the first of the largest; a row without any weight gives its first token
+    u64 at = 0;
+    if (m > -INFINITY) {
+      row.each([&](float z, int c) {
+        if (z == m && at == 0) at = static_cast<uint32_t>(~c);
+      });
+      at = row_reduce<true>(at, sh, ctas, turn);
+    }
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = m > -INFINITY ? static_cast<int>(~static_cast<uint32_t>(at)) : 0;
     return;
   }
-  const double c_ = 1.4426950408889634074 / static_cast<double>(T_);
-  Weigher weight;
-  weight.m = value_of(static_cast<uint32_t>(best >> 32));
+  if (m == INFINITY) {
+    row.infinite = true;
+    top = top == m ? 0.f : -INFINITY;
+    m = 0.f;
+  }
+  const double c_ = fmin(1.4426950408889634074 / static_cast<double>(T_), 3e38);
+  Weigher<T> weight;
+  weight.m = m;
   weight.c_hi = static_cast<float>(c_);
   weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
   weight.table = sh.table;
@@ -279,19 +360,18 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return t < total ? t : total - 1;
   };
 
-  // What is kept: keys above `cut`, and of those equal to it the indices up to `last`
+  // What is kept: logits above that of key `cut`, and of those equal to it the indices up to `last`
   uint32_t cut = 0;
   int last = p.cols;
   auto stays = [&](float z, int i) {
     const uint32_t key = key_of(z);
-    return i < row.end && (key > cut || (key == cut && i <= last));
+    return key > cut || (key == cut && i <= last);
   };
 
-  // The place of a logit in [0, 2^32) below the maximum, 2^32 where weights end; not below 2^32 for those that weigh nothing and for NaN.  It
-  // falls as logits rise (every step of its arithmetic does), equal places need not mean equal logits.
-  const float to_place = weight.c_hi * (4294967296.f / 41.f);
-  auto place = [&](float z) { return z == weight.m ? 0.f : (weight.m - z) * to_place; };
-  constexpr float END = 4294967040.f;
+  // The place of a logit below the maximum: p in units of 2^-17, 23 bits.  It falls as logits rise (every step of its arithmetic does), equal
+  // places need not mean equal logits.
+  constexpr int PLACE_BITS = 23;
+  auto place = [](float p_) { return __float_as_uint(fmaf(p_, 131072.f, 8388608.f)) & 0x7fffffu; };
 
   // Looks for the token that the filter ends with: the k-th (count), or the one at which the running sum reaches `limit`.  Result: 0 nothing is cut off,
   // 1 all that is kept is in the list of CTA 0, 2 (cut, last) are found, 3 they are to be found bit by bit.
@@ -302,9 +382,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     const uint32_t to_count = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(&sh.listed), 0) : tc5::smem_addr(&sh.listed);
     const uint32_t to_list = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(bins), 0) : tc5::smem_addr(bins);
     row.each([&](float z, int i) {
-      const float pl = place(z);
-      if (pl < END && i < row.end) {
-        const uint32_t X = __float2uint_rz(pl);
+      float dh;
+      const float p_ = weight.far(z, dh);
+      if (p_ < END) {
+        const uint32_t X = place(p_);
         if (X >= lo && X <= hi && stays(z, i)) {
           uint32_t at;
           asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(to_count) : "memory");
@@ -323,22 +404,23 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return n;
   };
   auto search = [&](const bool by_mass) -> int {
-    uint32_t prefix = 0, above = 0;
+    uint32_t first = 0, end = (1u << PLACE_BITS) - 1u, above = 0;   // places that are looked at, tokens before them
     u64 above_mass = 0;
     double limit = 0.;
 #pragma unroll 1
-    for (int shift = 28; ; shift -= 4) {
+    for (int shift = PLACE_BITS - 4; ; shift = shift >= 4 ? shift - 4 : 0) {
       u64* const own = bins + warp * BINS * 32 + lane;
 #pragma unroll
       for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
       row.each([&](float z, int i) {
-        const float pl = place(z);
-        if (pl < END && i < row.end) {
-          const uint32_t X = __float2uint_rz(pl);
-          if (shift == 28 || (X >> (shift + 4)) == prefix) {
+        float dh;
+        const float p_ = weight.far(z, dh);
+        if (p_ < END) {
+          const uint32_t X = place(p_);
+          if (X >= first && X <= end) {
             u64 add = 1ull << 52;   // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1)
-            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight(z) : 0;
-            own[((X >> shift) & 15u) * 32] += add;
+            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight.at(z, dh, p_) : 0;
+            own[((X - first) >> shift) * 32] += add;
           }
         }
       });
@@ -386,7 +468,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
         const u64 t = __shfl_up_sync(0xffffffffu, s, o);
         if ((lane & 15) >= o) { n += a; s += t; }
       }
-      if (shift == 28 && by_mass) {
+      if (shift == PLACE_BITS - 4 && by_mass) {
         whole = __shfl_sync(0xffffffffu, s, 15);
         limit = limit_of(whole);
       }
@@ -397,14 +479,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       const uint32_t here = __shfl_sync(0xffffffffu, count, b);
       above += __shfl_sync(0xffffffffu, n, b) - here;
       above_mass += __shfl_sync(0xffffffffu, s, b) - __shfl_sync(0xffffffffu, mass, b);
-      prefix = prefix << 4 | static_cast<uint32_t>(b);
-      const uint32_t first = prefix << shift, end = first + ((1u << shift) - 1u);
+      first += static_cast<uint32_t>(b) << shift;
+      end = first + ((1u << shift) - 1u);
       if (above + here <= CAP) { collect(0, end); return 1; }
       if (here <= CAP && (above > CAP - CAP / 8 || shift == 0)) {   // the last token kept is among these
         collect(first, end);
         if (rank == 0) {
           const int n_ = sorted();
-          u64* const sums = bins + CAP;
+          u64* const sums = bins + CAP;   // (over the running sums)
           int want;
           if (by_mass) {
             scan_list(sums, n_, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
@@ -442,7 +524,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     for (int bit = 1 << 21; bit > 0; bit >>= 1) {
       const int next = at | bit;
       u64 n = 0;
-      row.each([&](float z, int i) { n += (i < next && i < last + 1 && key_of(z) == cut && i < row.end) ? 1 : 0; });
+      row.each([&](float z, int i) { n += (i < next && i <= last && i < row.end && key_of(z) == cut) ? 1 : 0; });
       if (row_reduce<false>(n, sh, ctas, turn) < need) at = next;
     }
     return at;
@@ -463,7 +545,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     auto mass_from = [&](uint32_t from) {   // of what is kept so far, with keys of at least `from`
       u64 s = 0;
       row.each([&](float z, int i) {
-        if (stays(z, i) && key_of(z) >= from) s += weight(z);
+        if (i < row.end && stays(z, i) && key_of(z) >= from) s += weight(z);
       });
       return row_reduce<false>(s, sh, ctas, turn);
     };
@@ -477,24 +559,57 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     last = min(last, index_limit(static_cast<u64>(ceil((limit - static_cast<double>(above)) / static_cast<double>(weight(value_of(at)))))));
   };
 
+  // Places up to which at least `want` of the threads' largest tokens lie, hardly more (all places where there are not that many)
+  auto reach = [&](uint32_t want) -> uint32_t {
+    float dh;
+    const float p_ = weight.far(top, dh);
+    const uint32_t X = p_ < END ? place(p_) : 1u << PLACE_BITS;
+    uint32_t first = 0, above = 0;
+#pragma unroll 1
+    for (int shift = PLACE_BITS - 5; ; shift -= 5) {
+      const uint32_t b = X >= first ? (X - first) >> shift : 32u;   // 32 and more: elsewhere
+      uint32_t count = 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, b == e));
+        count = lane == e ? n : count;
+      }
+      sh.bin_count[warp][lane] = count;
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < 32 * ctas) {
+        const int to = threadIdx.x / 32;
+        uint32_t n = 0;
+#pragma unroll
+        for (int w = 0; w < SW; ++w) n += sh.bin_count[w][lane];
+        if (ctas == 1) sh.told_count[turn][0][lane] = n;
+        else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.told_count[turn][rank][lane]), to)), "r"(n) : "memory");
+      }
+      if (ctas == 1) __syncthreads(); else tc5::cluster_sync();
+      uint32_t n = 0;
+      for (int i = 0; i < ctas; ++i) n += sh.told_count[turn][i][lane];
+      turn ^= 1;
+      const uint32_t here = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += a;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, above + n >= want);
+      if (!hit) return (1u << PLACE_BITS) - 1u;
+      const int at = __ffs(hit) - 1;
+      const uint32_t upto = above + __shfl_sync(0xffffffffu, n, at), size = __shfl_sync(0xffffffffu, here, at);
+      first += static_cast<uint32_t>(at) << shift;
+      if (upto <= want + want / 4 + 16 || shift <= 3) return first + ((1u << shift) - 1u);
+      above = upto - size;
+    }
+  };
+
+  const int threads = ctas * ST;
   int found = 0;
   bool all_k = false;    // the list holds the k tokens themselves
-  if (restricted_by_k) {
-    found = search(false);
-    all_k = found == 1;
-    if (found == 3) top_k_by_bits();
-  }
-  if (tp < 1.f && found != 1) {
-    found = search(true);
-    if (found == 3) top_p_by_bits();
-  }
-
-  if (found == 1) {
-    // ---- everything that can be kept is in the list of CTA 0: cut it off there, and draw in the order of the indices ----
-    if (rank != 0) return;
-    const int n = sorted();
-    u64 *const sums = bins + CAP, *const order = bins + 2 * CAP;
-    scan_list(sums, n, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
+  u64 *const sums = bins + CAP, *const order = bins + 2 * CAP;
+  // CTA 0: cuts the sorted list (of n tokens, with the running sums of their weights) off behind the last token kept, and draws in the order of the indices
+  auto finish = [&](int n) {
     int kept = all_k && k < n ? k : n;
     const double limit = tp < 1.f ? limit_of(all_k ? sums[kept - 1] : whole) : 0.;
     if (threadIdx.x == 0) sh.pick[0] = sh.pick[1] = kept;
@@ -519,6 +634,61 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       if (bins[i] > target) { atomicMin(&sh.pick[1], i); break; }
     __syncthreads();
     if (threadIdx.x == 0) p.out[r] = static_cast<int>(~static_cast<uint32_t>(order[min(sh.pick[1], kept - 1)] >> 32));
+  };
+
+  // ---- the short way: the largest tokens, as many as k or as a nucleus mostly has ----
+  const bool few_k = restricted_by_k && 2 * k <= threads;
+  if (few_k || (tp < 1.f && !restricted_by_k)) {
+    if (!few_k) {
+      u64 s = 0;
+      row.packs([&](const float (&z)[8], int) { s += weight.sum(z); });
+      whole = row_reduce<false>(s, sh, ctas, turn);
+    }
+    const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 192u);
+    collect(0, upto);
+    if (rank == 0) {
+      const bool fits = sh.listed <= CAP;
+      bool all = fits && few_k;
+      int n = 0;
+      if (fits) {
+        n = sorted();
+        scan_list(sums, n, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
+        if (!few_k) all = upto == (1u << PLACE_BITS) - 1u || static_cast<double>(sums[n - 1]) >= limit_of(whole);
+      }
+      if (static_cast<int>(threadIdx.x) < ctas) {
+        const int v = all ? 1 : 0;
+        if (ctas == 1) sh.verdict = v;
+        else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.verdict), threadIdx.x)), "r"(v) : "memory");
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) sh.listed = 0;
+      if (all) {
+        if (ctas > 1) tc5::cluster_arrive();
+        all_k = few_k;
+        finish(n);
+        if (ctas > 1) tc5::cluster_wait();
+        return;
+      }
+    }
+    if (ctas > 1) tc5::cluster_sync(); else __syncthreads();
+    if (sh.verdict) return;
+  }
+
+  // ---- the long way ----
+  if (restricted_by_k) {
+    found = search(false);
+    all_k = found == 1;
+    if (found == 3) top_k_by_bits();
+  }
+  if (tp < 1.f && found != 1) {
+    found = search(true);
+    if (found == 3) top_p_by_bits();
+  }
+  if (found == 1) {
+    if (rank != 0) return;
+    const int n = sorted();
+    scan_list(sums, n, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
+    finish(n);
     return;
   }
 
@@ -529,7 +699,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return w >= least ? w : 0;
   };
   u64 mine = 0;
-  row.each([&](float z, int i) { mine += kept(z, i); });
+  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int) { mine += weight.sum(z); });
+  else row.each([&](float z, int i) { mine += kept(z, i); });
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
