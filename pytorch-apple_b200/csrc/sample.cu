@@ -17,6 +17,7 @@
 // that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or weights in 16 intervals of z, then in 16 parts
 // of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is drawn from by sums over ranges.
 #include "common.cuh"
+#include "mma.cuh"
 #include "tc5.cuh"
 
 namespace b200 {
@@ -24,6 +25,9 @@ namespace b200 {
 namespace {
 
 using u64 = unsigned long long;
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 constexpr int ST = 512, SW = ST / 32;        // threads and warps of a CTA
 constexpr int MAX_CTAS = 8;                  // of a row
 constexpr int64_t MAX_COLS = 1 << 22;        // sums of weights stay below 2^62
@@ -55,26 +59,30 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 
 // exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  The difference and its product with log2(e) / T are carried as pairs of fp32 numbers: a rounding
-// of t = 30 alone would be 2^-20 of the weight.  Below t = 16 by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a
-// table for the first eight, a cubic for the rest (its next term is below 2^-38).  From there on, where most tokens lie, a weight is below 2^24 units and
-// the fast exponential of the fraction (2^-22 of itself) is as good.
+// of t = 30 alone would be 2^-20 of the weight.  Below t = 17 by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a
+// table for the first eight, a cubic for the rest (its next term is below 2^-38).  From there on, where most tokens lie, a weight is below 2^23 units and
+// the fast exponential of t's distance from a whole number (2^-22 of itself) is as good; no conversions there, which share its unit.
 template <typename T> struct Weigher {
   float m, c_hi, c_lo;
+  float end, near;         // differences at which t is 41 (half a unit: no weight) and 17
   const uint32_t* table;   // 2^31 2^-(i / 256)
   __device__ __forceinline__ float rest(float z, float dh) const {   // (m - z) - dh
     const float bv = m - dh;
     return (m - (dh + bv)) + (bv - z);
   }
-  // p = fp32((m - z) c_hi), dh = fp32(m - z); for p < 41
-  __device__ __forceinline__ uint32_t small(float z, float dh, float p) const {
-    float e = fmaf(dh, c_lo, fmaf(dh, c_hi, -p));
-    if constexpr (sizeof(T) == 4) e = fmaf(rest(z, dh), c_hi, e);   // (differences of 16-bit logits are whole but for those next to zero)
-    const float shifted = p + 12582912.f, frac = p - (shifted - 12582912.f);   // (to the nearest whole number)
+  // m - z, not above `end`: for NaN as well
+  __device__ __forceinline__ float difference(float z) const { return fminf(m - z, end); }
+  // weight + 0x4b000000, for differences (of z, or `end`) of at least `near`
+  __device__ __forceinline__ uint32_t small(float z, float dh) const {
+    const float shifted = fmaf(dh, c_hi, 12582912.f);      // + 1.5 2^23: t to the nearest whole number
+    float x = fmaf(dh, c_lo, fmaf(dh, c_hi, -(shifted - 12582912.f)));
+    if constexpr (sizeof(T) == 4) x = dh < end ? fmaf(rest(z, dh), c_hi, x) : x;   // (differences of 16-bit logits are whole but for those next to zero)
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-frac - e));
-    return __float2uint_rz(y * __uint_as_float((167u << 23) - (__float_as_uint(shifted) << 23)));   // 2^(40 - whole)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-x));
+    return __float_as_uint(__fadd_rz(y * __uint_as_float((167u << 23) - (__float_as_uint(shifted) << 23)), 8388608.f));   // 2^(40 - whole), cut to a whole number
   }
-  __device__ __forceinline__ u64 large(float z, float dh, float p) const {   // (ONE for z == m)
+  __device__ __forceinline__ u64 large(float z) const {   // (ONE for z == m)
+    const float dh = m - z, p = __fmul_rn(dh, c_hi);
     const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, rest(z, dh) * c_hi);
     const float ip = floorf(p);
     int64_t t = (static_cast<int64_t>(ip) << 32) + static_cast<int64_t>(__float2uint_rz((p - ip) * 4294967296.f)) + static_cast<int64_t>(__float2int_rn(e * 4294967296.f));
@@ -86,37 +94,35 @@ template <typename T> struct Weigher {
     const uint32_t w = tab - static_cast<uint32_t>((static_cast<u64>(tab) * __float2uint_rn(q * 4294967296.f) + 0x80000000ull) >> 32);
     return (static_cast<u64>(w) << 9) >> static_cast<int>(t >> 32);
   }
-  __device__ __forceinline__ float far(float z, float& dh) const {   // p; not below 41 for what weighs nothing and for NaN
-    dh = m - z;
-    return __fmul_rn(dh, c_hi);
-  }
-  __device__ __forceinline__ u64 at(float z, float dh, float p) const { return p >= 16.f ? small(z, dh, p) : large(z, dh, p); }
   __device__ __forceinline__ u64 operator()(float z) const {
-    float dh;
-    const float p = far(z, dh);
-    return p < 41.f ? at(z, dh, p) : 0;
+    const float dh = difference(z);
+    return dh < near ? large(z) : small(z, dh) - 0x4b000000u;
   }
-  // sum over eight tokens, straight through for the many that are far from the maximum
-  __device__ __forceinline__ u64 sum(const float (&z)[8]) const {
-    float p[8], dh[8], nearest = 41.f;
-    uint32_t s = 0;
+  // Sum of the weights of those of eight tokens that keep(token, column) lets through: straight through for the ones that are far from the maximum
+  // (FAR; else they are left out), then the few near ones with at least `least` one by one (a warp goes round as often as its lane with most of them has some).
+  template <bool FAR, typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, u64 least, K&& keep) const {
+    uint32_t s = 0, close = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      p[k] = fminf(far(z[k], dh[k]), 41.f);   // (41, as for NaN: half a unit, which is none)
-      nearest = fminf(nearest, p[k]);
+      const float dh = difference(z[k]);
+      close |= (dh < near ? 1u : 0u) << k;
+      if (FAR) s += small(z[k], dh < near || !keep(z[k], c + k) ? end : dh);
     }
-    if (nearest >= 16.f) {
+    u64 t = FAR ? s - 8u * 0x4b000000u : 0u;
+    while (close) {
+      const int at = __ffs(close) - 1;
+      close &= close - 1;
+      float v = z[0];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += small(z[k], dh[k], p[k]);
-      return s;
+      for (int k = 1; k < 8; ++k) v = at == k ? z[k] : v;
+      if (keep(v, c + at)) {
+        const u64 w = large(v);
+        t += w >= least ? w : 0;
+      }
     }
-    u64 t = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += p[k] < 16.f ? large(z[k], dh[k], p[k]) : small(z[k], dh[k], p[k]);
     return t;
   }
 };
-constexpr float END = 41.f;
 
 struct Shared {
   uint32_t table[256];
@@ -129,6 +135,16 @@ struct Shared {
   int pick[2], verdict;
   __align__(8) uint64_t full[SW];
 };
+
+template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {   // of pairs of 16-bit numbers
+  if constexpr (sizeof(T) == 4) {
+    return a;
+  } else {
+    using P = typename Pair<T>::type;
+    const P r = __hmax2(reinterpret_cast<const P&>(a), reinterpret_cast<const P&>(b));
+    return reinterpret_cast<const uint32_t&>(r);
+  }
+}
 
 // A thread's share of the CTA's columns: warp w has a contiguous range, 256 columns at a time, eight per lane.
 template <typename T> struct Row {
@@ -152,6 +168,21 @@ template <typename T> struct Row {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = c + k < end ? to_f32<T>(x[c + k]) : __uint_as_float(0x7fffffffu);
     }
+  }
+  // the largest of columns c .. c + 7 (NaN is none)
+  __device__ __forceinline__ float top(int c) const {
+    if constexpr (sizeof(T) == 2) {
+      if (!infinite && (c + 8 <= copied || (vec && c + 8 <= end))) {
+        const uint4 w = *reinterpret_cast<const uint4*>(c + 8 <= copied ? copy + (c - begin) : x + c);
+        const uint32_t v = max2<T>(max2<T>(w.x, w.y), max2<T>(w.z, w.w));
+        float a, b;
+        unpack2<T>(v, a, b);
+        return fmaxf(a, b);
+      }
+    }
+    float z[8];
+    load(c, z);
+    return fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
   }
   static __device__ __forceinline__ void unpack(const T* at, float (&f)[8]) {
     if constexpr (sizeof(T) == 2) {
@@ -216,52 +247,69 @@ template <bool TOP> __device__ u64 row_reduce(u64 v, Shared& sh, int ctas, int& 
   return r;
 }
 
-// list[0 .. n) in descending order; n a power of two.  All threads; begins and ends with a barrier.
+// list[0 .. n) in descending order; n a power of two.  All threads; begins and ends with a barrier.  Element e of thread i is number i + ST e: steps
+// within a warp go by shuffles, those of ST and more within a thread.
+template <int E> __device__ __forceinline__ void sort_elements(u64* list, int n) {
+  const int i = threadIdx.x;
+  u64 v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = i + ST * e < n ? list[i + ST * e] : 0;
+#pragma unroll 1
+  for (int size = 2; size <= n; size <<= 1)
+#pragma unroll 1
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      if (E > 1 && step >= ST) {
+#pragma unroll
+        for (int h = 1; h < E; h <<= 1)
+          if (step == ST * h)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (!(e & h)) {
+                const bool falling = ((i + ST * e) & size) == 0;
+                const u64 a = v[e], b = v[e | h];
+                if ((a < b) == falling) { v[e] = b; v[e | h] = a; }
+              }
+        continue;
+      }
+      if (step >= 32) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (i + ST * e < n) list[i + ST * e] = v[e];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = i + ST * e;
+        const u64 w = step >= 32 ? (at < n ? list[at ^ step] : 0) : __shfl_xor_sync(0xffffffffu, v[e], step);
+        const bool larger = ((at & step) == 0) == ((at & size) == 0);   // the larger of the two stays here
+        v[e] = larger == (w > v[e]) ? w : v[e];
+      }
+    }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (i + ST * e < n) list[i + ST * e] = v[e];
+  __syncthreads();
+}
 __device__ void sort_list(u64* list, int n) {
   __syncthreads();
-  if (n <= ST) {   // an element per thread: steps within a warp by shuffles
-    const int i = threadIdx.x;
-    u64 v = i < n ? list[i] : 0;
-    for (int size = 2; size <= n; size <<= 1)
-      for (int step = size >> 1; step > 0; step >>= 1) {
-        u64 w;
-        if (step >= 32) {
-          __syncthreads();
-          if (i < n) list[i] = v;
-          __syncthreads();
-          w = i < n ? list[i ^ step] : 0;
-        } else {
-          w = __shfl_xor_sync(0xffffffffu, v, step);
-        }
-        const bool larger = ((i & step) == 0) == ((i & size) == 0);   // the larger of the two stays here
-        v = larger == (w > v) ? w : v;
-      }
-    __syncthreads();
-    if (i < n) list[i] = v;
-    __syncthreads();
-    return;
-  }
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      for (int i = threadIdx.x; i < n / 2; i += ST) {
-        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const u64 a = list[lo], b = list[hi];
-        if ((a < b) == ((lo & size) == 0)) { list[lo] = b; list[hi] = a; }
-      }
-      __syncthreads();
-    }
+  if (n <= ST) sort_elements<1>(list, n);
+  else if (n <= 2 * ST) sort_elements<2>(list, n);
+  else sort_elements<4>(list, n);
 }
+static_assert(CAP == 4 * ST, "sort_list");
 
-// sums[i] = val(0) + .. + val(i) for i < n <= CAP (four to a thread).  All threads; ends with a barrier.
+// sums[i] = val(0) + .. + val(i) for i < n <= CAP.  All threads; ends with a barrier.
 template <typename F> __device__ void scan_list(u64* sums, int n, Shared& sh, F&& val) {
-  constexpr int PER = CAP / ST;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 v[PER], run = 0;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int i = threadIdx.x * PER + e;
-    run += i < n ? val(i) : 0;
-    v[e] = run;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (n + ST - 1) / ST;
+  u64 run = 0;
+  for (int e = 0; e < per; ++e) {
+    const int i = threadIdx.x * per + e;
+    if (i < n) {
+      run += val(i);
+      sums[i] = run;
+    }
   }
   u64 upto = run;
 #pragma unroll
@@ -273,11 +321,11 @@ template <typename F> __device__ void scan_list(u64* sums, int n, Shared& sh, F&
   if (lane == 31) sh.part[warp] = upto;
   __syncthreads();
   u64 before = upto - run;
-  for (int w = 0; w < warp; ++w) before += sh.part[w];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int i = threadIdx.x * PER + e;
-    if (i < n) sums[i] = before + v[e];
+  for (int w = 0; w < SW; ++w) before += w < warp ? sh.part[w] : 0;
+  for (int e = 0; e < per; ++e) {
+    const int i = threadIdx.x * per + e;
+    if (i < n) sums[i] += before;
   }
   __syncthreads();
 }
@@ -326,9 +374,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
 
   // ---- the maximum ----
   float top = -INFINITY;   // of this thread's tokens (NaN is none)
-  row.packs([&](const float (&z)[8], int) {
-    top = fmaxf(top, fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))));
-  });
+#pragma unroll 4
+  for (int c = row.begin + lane * 8; c < row.end; c += 256) top = fmaxf(top, row.top(c));
   const u64 best = row_reduce<true>(key_of(top), sh, ctas, turn);
   float m = value_of(static_cast<uint32_t>(best));
   if (!(T_ > 0.f) || m == -INFINITY) {   // greedy: the first of the largest; a row without any weight gives its first token
@@ -347,11 +394,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     top = top == m ? 0.f : -INFINITY;
     m = 0.f;
   }
-  const double c_ = fmin(1.4426950408889634074 / static_cast<double>(T_), 3e38);
+  // (temperatures past 1e30 and below 5e-39 count as those: differences of logits are not told apart any more, or not there at all)
+  const double c_ = fmin(1.4426950408889634074 / fmin(static_cast<double>(T_), 1e30), 3e38);
   Weigher<T> weight;
   weight.m = m;
   weight.c_hi = static_cast<float>(c_);
   weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
+  weight.end = static_cast<float>(41. / c_);
+  weight.near = static_cast<float>(17. / c_);
   weight.table = sh.table;
   const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;
   auto target_of = [&](u64 total) -> u64 {
@@ -368,32 +418,60 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return key > cut || (key == cut && i <= last);
   };
 
-  // The place of a logit below the maximum: p in units of 2^-17, 23 bits.  It falls as logits rise (every step of its arithmetic does), equal
-  // places need not mean equal logits.
+  // The place of a logit below the maximum, from its difference: t in units of 2^-17, 23 bits.  It falls as logits rise (every step of its arithmetic
+  // does), equal places need not mean equal logits.  Those at `end` weigh nothing and count as not there.
   constexpr int PLACE_BITS = 23;
-  auto place = [](float p_) { return __float_as_uint(fmaf(p_, 131072.f, 8388608.f)) & 0x7fffffu; };
+  constexpr uint32_t LAST_PLACE = (1u << PLACE_BITS) - 1u;
+  auto place = [&](float dh) { return __float_as_uint(fmaf(__fmul_rn(dh, weight.c_hi), 131072.f, 8388608.f)) & LAST_PLACE; };
 
   // Looks for the token that the filter ends with: the k-th (count), or the one at which the running sum reaches `limit`.  Result: 0 nothing is cut off,
   // 1 all that is kept is in the list of CTA 0, 2 (cut, last) are found, 3 they are to be found bit by bit.
   u64 whole = 0;         // sum of what is kept before top-p
   auto limit_of = [&](u64 sum) { return fmax(static_cast<double>(tp) * static_cast<double>(sum), 0.5); };
   const bool restricted_by_k = k > 0 && k < p.cols;
-  auto collect = [&](uint32_t lo, uint32_t hi) {   // tokens with places in [lo, hi], to CTA 0
-    const uint32_t to_count = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(&sh.listed), 0) : tc5::smem_addr(&sh.listed);
-    const uint32_t to_list = ctas > 1 ? tc5::map_to_rank(tc5::smem_addr(bins), 0) : tc5::smem_addr(bins);
-    row.each([&](float z, int i) {
-      float dh;
-      const float p_ = weight.far(z, dh);
-      if (p_ < END) {
-        const uint32_t X = place(p_);
-        if (X >= lo && X <= hi && stays(z, i)) {
-          uint32_t at;
-          asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(to_count) : "memory");
-          if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to_list + at * 8), "l"(static_cast<u64>(key_of(z)) << 32 | static_cast<uint32_t>(~i)) : "memory");
+  auto collect = [&](uint32_t lo, uint32_t hi) {   // tokens with places in [lo, hi], to CTA 0: into a list of each CTA's own, then in one piece
+    // (a bound on the logits with some room: places are looked at only behind it)
+    const float bound = weight.m - fminf((static_cast<float>(hi) + 8.f) * (1.0001f / 131072.f) / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f;
+#pragma unroll 2
+    for (int c = row.begin + lane * 8; c < row.end; c += 256) {
+      if (row.top(c) >= bound) {
+        float z[8];
+        uint32_t some = 0;
+        row.load(c, z);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) some |= (z[k] >= bound ? 1u : 0u) << k;
+        while (some) {
+          const int k = __ffs(some) - 1;
+          some &= some - 1;
+          float v = z[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) v = k == e ? z[e] : v;
+          const float dh = weight.difference(v);
+          const uint32_t X = place(dh);
+          if (dh < weight.end && X <= hi && X >= lo && stays(v, c + k)) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < CAP) bins[at] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~(c + k));
+          }
         }
       }
-    });
-    if (ctas > 1) tc5::cluster_sync(); else __syncthreads();
+    }
+    if (ctas == 1) { __syncthreads(); return; }
+    // (CTA 0's counter has its own tokens by the time the others reserve their places behind them)
+    tc5::cluster_sync();
+    const int mine = sh.listed;
+    if (rank != 0) {
+      if (threadIdx.x == 0) {
+        uint32_t at;
+        asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(tc5::map_to_rank(tc5::smem_addr(&sh.listed), 0)), "r"(mine) : "memory");
+        sh.pick[0] = static_cast<int>(at);
+      }
+      __syncthreads();
+      const int at = sh.pick[0], n = min(min(mine, CAP), CAP - at);
+      const uint32_t to = tc5::map_to_rank(tc5::smem_addr(bins), 0);
+      for (int i = threadIdx.x; i < n; i += ST) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + (at + i) * 8), "l"(bins[i]) : "memory");
+      if (threadIdx.x == 0) sh.listed = 0;
+    }
+    tc5::cluster_sync();
   };
   auto sorted = [&]() {   // CTA 0: its list in order; the number of tokens
     const int n = min(sh.listed, CAP);
@@ -404,7 +482,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return n;
   };
   auto search = [&](const bool by_mass) -> int {
-    uint32_t first = 0, end = (1u << PLACE_BITS) - 1u, above = 0;   // places that are looked at, tokens before them
+    uint32_t first = 0, end = LAST_PLACE, above = 0;   // places that are looked at, tokens before them
     u64 above_mass = 0;
     double limit = 0.;
 #pragma unroll 1
@@ -413,13 +491,12 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
 #pragma unroll
       for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
       row.each([&](float z, int i) {
-        float dh;
-        const float p_ = weight.far(z, dh);
-        if (p_ < END) {
-          const uint32_t X = place(p_);
+        const float dh = weight.difference(z);
+        if (dh < weight.end) {
+          const uint32_t X = place(dh);
           if (X >= first && X <= end) {
             u64 add = 1ull << 52;   // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1)
-            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight.at(z, dh, p_) : 0;
+            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight(z) : 0;
             own[((X - first) >> shift) * 32] += add;
           }
         }
@@ -561,9 +638,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
 
   // Places up to which at least `want` of the threads' largest tokens lie, hardly more (all places where there are not that many)
   auto reach = [&](uint32_t want) -> uint32_t {
-    float dh;
-    const float p_ = weight.far(top, dh);
-    const uint32_t X = p_ < END ? place(p_) : 1u << PLACE_BITS;
+    const float dh = weight.difference(top);
+    const uint32_t X = dh < weight.end ? place(dh) : 1u << PLACE_BITS;
     uint32_t first = 0, above = 0;
 #pragma unroll 1
     for (int shift = PLACE_BITS - 5; ; shift -= 5) {
@@ -595,7 +671,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
         if (lane >= o) n += a;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, above + n >= want);
-      if (!hit) return (1u << PLACE_BITS) - 1u;
+      if (!hit) return LAST_PLACE;
       const int at = __ffs(hit) - 1;
       const uint32_t upto = above + __shfl_sync(0xffffffffu, n, at), size = __shfl_sync(0xffffffffu, here, at);
       first += static_cast<uint32_t>(at) << shift;
@@ -641,10 +717,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (few_k || (tp < 1.f && !restricted_by_k)) {
     if (!few_k) {
       u64 s = 0;
-      row.packs([&](const float (&z)[8], int) { s += weight.sum(z); });
+      row.packs([&](const float (&z)[8], int c) { s += weight.template sum<true>(z, c, 0, [](float, int) { return true; }); });
       whole = row_reduce<false>(s, sh, ctas, turn);
     }
-    const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 192u);
+    const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 96u);
     collect(0, upto);
     if (rank == 0) {
       const bool fits = sh.listed <= CAP;
@@ -653,7 +729,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       if (fits) {
         n = sorted();
         scan_list(sums, n, sh, [&](int i) { return weight(value_of(static_cast<uint32_t>(bins[i] >> 32))); });
-        if (!few_k) all = upto == (1u << PLACE_BITS) - 1u || static_cast<double>(sums[n - 1]) >= limit_of(whole);
+        if (!few_k) all = upto == LAST_PLACE || static_cast<double>(sums[n - 1]) >= limit_of(whole);
       }
       if (static_cast<int>(threadIdx.x) < ctas) {
         const int v = all ? 1 : 0;
@@ -699,8 +775,16 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return w >= least ? w : 0;
   };
   u64 mine = 0;
-  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int) { mine += weight.sum(z); });
-  else row.each([&](float z, int i) { mine += kept(z, i); });
+  if (cut == 0 && least == 0) {
+    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, 0, [](float, int) { return true; }); });
+  } else if (least == 0) {
+    const float at_cut = value_of(cut);
+    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, 0, [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); }); });
+  } else if (least > 1ull << 23) {
+    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<false>(z, c, least, stays); });
+  } else {
+    row.each([&](float z, int i) { mine += kept(z, i); });
+  }
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
@@ -710,40 +794,20 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (target < before || target >= before + sh.told[slot][rank]) return;   // another CTA's
   int w_ = 0;
   while (before + sh.part[w_] <= target) before += sh.part[w_++];
-  // all warps take equal parts of warp w_'s range, in whole steps of 256 columns
-  const int b_ = min(c1, c0 + w_ * span), e_ = min(c1, b_ + span), step = ((e_ - b_ + 255) / 256 + SW - 1) / SW * 256;
-  const int from = min(e_, b_ + warp * step), upto_ = min(e_, from + step);
+  // the range of warp w_, 256 columns of it to each warp at a time
   Row<T> part = row;
-  part.begin = b_;
-  part.end = e_;
-  part.copy = reinterpret_cast<const T*>(dsm + BIN_BYTES) + (b_ - c0);
-  part.copied = p.staged && row.vec ? b_ + static_cast<int>((static_cast<uint32_t>(e_ - b_) * sizeof(T) & ~15u) / sizeof(T)) : b_;
-  auto kept_at = [&](float z, int i) -> u64 {
-    const uint32_t key = key_of(z);
-    if (i >= upto_ || key < cut || (key == cut && i > last)) return 0;
-    const u64 w = weight(z);
-    return w >= least ? w : 0;
-  };
-  u64 sum = 0;
-  for (int c = from + lane * 8; c < upto_; c += 256) {
-    float v[8];
-    part.load(c, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += kept_at(v[e], c + e);
-  }
-  sum = warp_add(sum);
-  __syncthreads();   // (the ranges' sums have been read)
-  if (lane == 0) sh.part[warp] = sum;
-  __syncthreads();
-  for (int i = 0; i < warp; ++i) before += sh.part[i];
-  if (target < before || target >= before + sum) return;
-  for (int c = from + lane * 8; ; c += 256) {   // (the whole warp goes round together, and the target lies in its part)
+  part.begin = min(c1, c0 + w_ * span);
+  part.end = min(c1, part.begin + span);
+  part.copy = reinterpret_cast<const T*>(dsm + BIN_BYTES) + (part.begin - c0);
+  part.copied = p.staged && row.vec ? part.begin + static_cast<int>((static_cast<uint32_t>(part.end - part.begin) * sizeof(T) & ~15u) / sizeof(T)) : part.begin;
+  for (int b_ = part.begin; b_ < part.end; b_ += SW * 256) {
+    const int c = b_ + warp * 256 + lane * 8;
     float v[8];
     u64 w[8], s = 0;
-    if (c < upto_) part.load(c, v);
+    if (c < part.end) part.load(c, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = c < upto_ ? kept_at(v[e], c + e) : 0;
+      w[e] = c < part.end ? kept(v[e], c + e) : 0;
       s += w[e];
     }
     u64 upto = s;
@@ -752,17 +816,24 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += t;
     }
-    const unsigned passed = __ballot_sync(0xffffffffu, before + upto > target);
-    if (passed) {
-      if (lane == __ffs(passed) - 1) {
-        u64 run = before + upto - s;
-        int e = 0;
-        while (e < 7 && run + w[e] <= target) run += w[e++];
-        p.out[r] = c + e;
-      }
-      return;
+    __syncthreads();   // (what was in sh.part has been read)
+    if (lane == 31) sh.part[warp] = upto;
+    __syncthreads();
+    u64 mine_ = before;
+#pragma unroll
+    for (int i = 0; i < SW; ++i) {
+      const u64 t = sh.part[i];
+      mine_ += i < warp ? t : 0;
+      before += t;
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    const unsigned passed = __ballot_sync(0xffffffffu, mine_ + upto > target);
+    if (target >= mine_ && passed && lane == __ffs(passed) - 1) {
+      u64 run = mine_ + upto - s;
+      int e = 0;
+      while (e < 7 && run + w[e] <= target) run += w[e++];
+      p.out[r] = c + e;
+    }
+    if (target < before) return;
   }
 }
 
