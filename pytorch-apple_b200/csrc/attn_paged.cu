@@ -120,6 +120,21 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
     __syncthreads();   // (the running costs lie in the rings: everybody is through with them)
     for (int s = 0; s < STAGES; ++s) copy();
 
+    // Q^T fragments: row 8 j + g, dims 16 ks + 2 t, +1 and 16 ks + 2 t + 8, +9
+    uint32_t qf[KS][NT][2];
+    auto load_q = [&](const PagedPiece& c) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = 8 * j + g;
+        const T* qr = static_cast<const T*>(p.q) + (static_cast<int64_t>(c.token) + r / p.G) * p.qs[0] + (c.hk * p.G + r % p.G) * p.qs[1] + 2 * t;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qf[ks][j][0] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks) : 0u;
+          qf[ks][j][1] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8) : 0u;
+        }
+      }
+    };
+    load_q(s_piece[0]);
     int x = warp;   // this warp's next block
 #pragma unroll 1
     for (int f = 0; f < F; ++f) {
@@ -144,18 +159,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
             see_min = min(see_min, see[j][e]);
             from_max = max(from_max, from[j][e]);
           }
-        // Q^T fragments: row 8 j + g, dims 16 ks + 2 t, +1 and 16 ks + 2 t + 8, +9
-        uint32_t qf[KS][NT][2];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const int r = 8 * j + g;
-          const T* qr = static_cast<const T*>(p.q) + (static_cast<int64_t>(c.token) + r / p.G) * p.qs[0] + (c.hk * p.G + r % p.G) * p.qs[1] + 2 * t;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            qf[ks][j][0] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks) : 0u;
-            qf[ks][j][1] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8) : 0u;
-          }
-        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -261,6 +264,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
           if (x >= x_end) { parked = was; break; }
           copy();
         }
+        if (f + 1 < F) load_q(s_piece[f + 1]);   // (on its way while this piece's sums are added up)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -286,31 +290,40 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
             for (int e = 0; e < 2; ++e) { s_m[warp][8 * j + 2 * t + e] = m[j][e]; s_l[warp][8 * j + 2 * t + e] = l[j][e]; }
         }
       }
+      if (parked < 0 && f + 1 < F) load_q(s_piece[f + 1]);
       if (lane == 0) s_park[warp] = parked;
       __syncthreads();
-      // ---- the block's sums: a thread per dim, the rows dealt to FEW_WARPS * 32 / D of them ----
+      // ---- the block's sums: a thread per four dims of a row ----
       {
-        const int d = threadIdx.x % D;
+        constexpr int LPR = D / 4;
+        const int d = threadIdx.x % LPR * 4;
         const bool whole = c.flags == 3;
         const int64_t slot = paged_slot(cta, c.flags & 1, ROWS);
-        for (int r = threadIdx.x / D; r < c.rows; r += FEW_WARPS * 32 / D) {
-          float top = -INFINITY;
+        for (int r = threadIdx.x / LPR; r < c.rows; r += FEW_WARPS * 32 / LPR) {
+          float mw[FEW_WARPS], top = -INFINITY;
+          float4 a[FEW_WARPS];
 #pragma unroll
-          for (int w = 0; w < FEW_WARPS; ++w)
-            if (s_park[w] >= 0) top = fmaxf(top, s_m[w][r]);
+          for (int w = 0; w < FEW_WARPS; ++w) {
+            const int at = s_park[w];
+            mw[w] = at >= 0 ? s_m[w][r] : -INFINITY;
+            a[w] = at >= 0 ? *reinterpret_cast<const float4*>(smem + w * FEW_RING + at * BLOCK + (r * D + (d ^ (((r & 7) >> 1) << 3))) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            top = fmaxf(top, mw[w]);
+          }
           const float ref = top == -INFINITY ? 0.f : top;
-          float acc = 0.f, sum = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < FEW_WARPS; ++w)
-            if (s_park[w] >= 0) {
-              const float f_ = ex2_approx(s_m[w][r] - ref);
-              acc += reinterpret_cast<const float*>(smem + w * FEW_RING + s_park[w] * BLOCK)[r * D + (d ^ (((r & 7) >> 1) << 3))] * f_;
-              sum += s_l[w][r] * f_;
-            }
+          for (int w = 0; w < FEW_WARPS; ++w) {
+            const float f_ = ex2_approx(mw[w] - ref);
+            acc.x += a[w].x * f_; acc.y += a[w].y * f_; acc.z += a[w].z * f_; acc.w += a[w].w * f_;
+            sum += s_park[w] >= 0 ? s_l[w][r] * f_ : 0.f;
+          }
           if (whole) {   // (a row without keys gives zeros)
-            static_cast<T*>(p.out)[((static_cast<int64_t>(c.token) + r / p.G) * p.Hq + c.hk * p.G + r % p.G) * D + d] = from_f32<T>(sum > 0.f ? acc / sum : 0.f);
+            const float inv = sum > 0.f ? 1.f / sum : 0.f;
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + ((static_cast<int64_t>(c.token) + r / p.G) * p.Hq + c.hk * p.G + r % p.G) * D + d) =
+                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
           } else {
-            p.acc[(slot + r) * D + d] = acc;
+            *reinterpret_cast<float4*>(p.acc + (slot + r) * D + d) = acc;
             if (d == 0) p.ml[slot + r] = make_float2(top, sum);
           }
         }
@@ -325,80 +338,57 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 }
 
 // ===========================================================================
-// Joins the pieces of items that several blocks had a part in, in the order of the blocks (their sums are the same whoever adds them up).  A thread
-// per four dims; 256 / (D / 4) rows of an item at a time, or one row with as many groups of pieces where there are many pieces: then a thread's
-// chain of loads is short (71 pieces: 17.2 us with one group).  Every block goes through the list of such items (at most one begins in each
-// block of the kernel before).
+// Joins the pieces of the item that begins in block blockIdx.x of the kernel before and goes on in the next ones, in the order of the blocks (their
+// sums are the same whoever adds them up): rows blockIdx.y * RPB and up.  A thread per four dims; few pieces: a row to each 256 / (D / 4)th of the block,
+// many: the pieces of one row dealt to them, so that a thread's chain of loads stays short (71 pieces: 17.2 us with a thread per piece and dim).
 // ===========================================================================
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, int RPB>
 __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int LPR = D / 4, RB = 256 / LPR, BATCH = 6;
-  __shared__ int s_upto[PAGED_CTAS + 1], s_sum[8];
-  __shared__ __align__(16) float s_acc[RB][D];
-  __shared__ float s_m[RB], s_l[RB];
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = 4;
+  __shared__ __align__(16) float s_acc[GROUPS][D];
+  __shared__ float s_m[GROUPS], s_l[GROUPS];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int4 h = make_int4(0, 0, 0, 0);
-  if (threadIdx.x < PAGED_CTAS) h = __ldg(p.head + threadIdx.x);
-  const int mine = h.x > BATCH ? h.w : h.x > 0 ? (h.w + RB - 1) / RB : 0;   // tasks of this item
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) s_sum[warp] = upto;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) upto += s_sum[w];
-  if (threadIdx.x < PAGED_CTAS) s_upto[threadIdx.x + 1] = upto;
-  if (threadIdx.x == 0) s_upto[0] = 0;
-  __syncthreads();
-  const int tasks = s_upto[PAGED_CTAS], g = threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
-  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    int lo = 0, hi = PAGED_CTAS;   // the item: the last one whose tasks begin at or before this one
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_upto[mid] <= task) lo = mid; else hi = mid;
-    }
-    const int4 it = __ldg(p.head + lo);
-    const bool many = it.x > BATCH;
-    const int r = many ? task - s_upto[lo] : (task - s_upto[lo]) * RB + g, step = many ? RB : 1;
+  const int4 it = __ldg(p.head + blockIdx.x);
+  const int g = threadIdx.x / LPR, d = threadIdx.x % LPR * 4, r0 = blockIdx.y * RPB;
+  if (it.x == 0 || r0 >= it.w) return;
+  const bool many = RPB == 1 || it.x > 2 * BATCH;
+  const int step = many ? GROUPS : 1;
+  for (int r = many ? r0 : r0 + g; r < min(it.w, r0 + RPB); r += many ? 1 : GROUPS) {   // (uniform where the block meets)
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < it.w)
-      for (int i0 = many ? g : 0; i0 < it.x; i0 += BATCH * step) {
-        float2 ml[BATCH];
-        float4 a[BATCH];
+    for (int i0 = many ? g : 0; i0 < it.x; i0 += BATCH * step) {
+      float2 ml[BATCH];
+      float4 a[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int at = i0 + i * step;
-          ml[i] = make_float2(-INFINITY, 0.f);
-          a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (at < it.x) {
-            const int64_t slot = paged_slot(lo + at, at == 0, ROWS) + r;
-            ml[i] = __ldg(p.ml + slot);
-            a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
-          }
+      for (int i = 0; i < BATCH; ++i) {
+        const int at = i0 + i * step;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at < it.x) {
+          const int64_t slot = paged_slot(blockIdx.x + at, at == 0, ROWS) + r;
+          ml[i] = __ldg(p.ml + slot);
+          a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
         }
-        float top = m;
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float c = ex2_approx(m - ref);
-        l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const float f = ex2_approx(ml[i].x - ref);
-          l += ml[i].y * f;
-          acc.x += a[i].x * f; acc.y += a[i].y * f; acc.z += a[i].z * f; acc.w += a[i].w * f;
-        }
-        m = top;
       }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float c = ex2_approx(m - ref);
+      l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float f = ex2_approx(ml[i].x - ref);
+        l += ml[i].y * f;
+        acc.x += a[i].x * f; acc.y += a[i].y * f; acc.z += a[i].z * f; acc.w += a[i].w * f;
+      }
+      m = top;
+    }
     T* const o = static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D;
     if (!many) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (r < it.w) *reinterpret_cast<uint2*>(o + d) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(o + d) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
       continue;
     }
     *reinterpret_cast<float4*>(&s_acc[g][d]) = acc;
@@ -407,10 +397,10 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
     if (threadIdx.x < D) {
       float top = -INFINITY, sum = 0.f, a = 0.f;
 #pragma unroll
-      for (int e = 0; e < RB; ++e) top = fmaxf(top, s_m[e]);
+      for (int e = 0; e < GROUPS; ++e) top = fmaxf(top, s_m[e]);
       const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int e = 0; e < RB; ++e) {
+      for (int e = 0; e < GROUPS; ++e) {
         const float f = ex2_approx(s_m[e] - ref);
         sum += s_l[e] * f;
         a += s_acc[e][threadIdx.x] * f;
@@ -572,10 +562,10 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
     });
   } else {
     B200_DISPATCH_HALF(dtype, T, {
-      const auto merge = [&](auto kernel, int blocks) { launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p); };
-      if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8>, PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 8>, PAGED_CTAS); }
-      else if (rows == 16) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 16>, 2 * PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 16>, 2 * PAGED_CTAS); }
-      else { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 128>, 8 * PAGED_CTAS); else merge(attn_paged_merge_kernel<T, 64, 128>, 8 * PAGED_CTAS); }
+      const auto merge = [&](auto kernel, int groups) { launch_pdl(kernel, dim3(PAGED_CTAS, static_cast<unsigned>(groups)), dim3(256), 0, st, p); };
+      if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8, 1>, 8); else merge(attn_paged_merge_kernel<T, 64, 8, 1>, 8); }
+      else if (rows == 16) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 16, 1>, 16); else merge(attn_paged_merge_kernel<T, 64, 16, 1>, 16); }
+      else { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 128, 8>, 16); else merge(attn_paged_merge_kernel<T, 64, 128, 16>, 8); }
     });
   }
   B200_CHECK_LAUNCH("attn_paged");

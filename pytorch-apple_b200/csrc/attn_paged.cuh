@@ -151,13 +151,13 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
     int skip = 0;   // heads ahead of u0
     int64_t base = begin;
     if (u0 > begin && p.Hkv > 1) {
-      const int64_t per_head = all / p.Hkv;
-      skip = static_cast<int>((u0 - begin) / per_head);
+      const int64_t per_head = tiles == 1 ? paged_tile<KT>(p, T, n, 0, tpt).cnt + OV : all / p.Hkv, off = u0 - begin;
+      skip = p.Hkv <= 32 ? __popc(__ballot_sync(0xffffffffu, lane < p.Hkv && (lane + 1) * per_head <= off)) : static_cast<int>(off / per_head);
       base += skip * per_head;
     }
     const int items = p.Hkv * tiles;
     for (int e0 = skip * tiles; e0 < items && base < u1; e0 += 32) {
-      const int e = e0 + lane, h = e / tiles;
+      const int e = e0 + lane, h = tiles == 1 ? e : e / tiles;
       PagedTile t = {0, 0, 0, 0, 0};
       if (e < items) t = paged_tile<KT>(p, T, n, e - h * tiles, tpt);
       const int64_t cost = e < items ? t.cnt + OV : 0;
