@@ -1,4 +1,4 @@
-"""Ahead-of-time build of ``libb200nn.so`` (sm_100a only).
+"""Ahead-of-time build of ``libb200nn.so`` (sm_100a only) and of ``b200_torch_calls.so``, the module that calls it with torch tensors.
 
 ``python build_native.py`` or ``build()`` compiles every ``csrc/*.cu`` with nvcc and
 links one shared library next to the Python runtime package, where
@@ -19,6 +19,7 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 OBJ_DIR = CSRC / "build"
 LIB_PATH = ROOT / "cuda_runtime" / "libb200nn.so"
+CALLS_PATH = ROOT / "cuda_runtime" / "b200_torch_calls.so"
 INCLUDE = ROOT.parent / "include"
 
 NVCC_FLAGS = [
@@ -65,7 +66,30 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_torch_calls(force, verbose)
     return LIB_PATH
+
+
+def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
+    """``csrc/torch_calls.cpp`` against the headers of the torch that is installed."""
+    src = CSRC / "torch_calls.cpp"
+    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime > max(src.stat().st_mtime, (INCLUDE / "b200nn.h").stat().st_mtime):
+        return CALLS_PATH
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1]
+    includes = [base / "include", base / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], cuda / "include"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in includes), str(src), "-o", str(CALLS_PATH), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    return CALLS_PATH
 
 
 if __name__ == "__main__":

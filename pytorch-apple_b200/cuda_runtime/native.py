@@ -58,10 +58,6 @@ class AttnPagedArgs(C.Structure):
                [(n, C.c_int32) for n in ("Hq", "Hkv", "D", "page_size", "dtype")] + [("scale", C.c_float)]
 
 
-# the same structures for struct.Struct, whose packing costs a tenth of filling a ctypes.Structure
-PAGED_APPEND_FORMAT = "@9P11q6i"
-ATTN_PAGED_FORMAT = "@8P12q5if"
-
 _vp, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
 _TP = C.POINTER(Tensor)
 _I64P = C.POINTER(C.c_int64)
@@ -107,8 +103,8 @@ SIGNATURES = {
     "b200_attn_prefill_reads_tiles": (_i, [_vp, _i64, _i64, _i64, _i]),
     "b200_mask_tiles": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp]),
     "b200_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i64, _i, _I64P, _I64P, _I64P, _i64, _i64, _f, _i, _vp]),
-    "b200_paged_append": (_i, [_vp, _vp]),   # PagedAppendArgs (or its bytes), stream
-    "b200_attn_paged": (_i, [_vp, _vp]),     # AttnPagedArgs (or its bytes), stream
+    "b200_paged_append": (_i, [_vp, _vp]),   # PagedAppendArgs, stream
+    "b200_attn_paged": (_i, [_vp, _vp]),     # AttnPagedArgs, stream
     "b200_attn_paged_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
     "b200_sample_rows": (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
 }
@@ -162,17 +158,39 @@ def install_test_library(lib, device: str = "cpu") -> None:
     _test_override = None if lib is None else (lib, device)
 
 
-def on_stream(device, what: str, name: str, *args) -> None:
-    """Entry point ``name`` with ``args`` and the current stream of ``device`` (a ``torch.device``), with that device current."""
-    import torch
+_calls = None
+_entries: dict = {}   # name -> (library, address, what must stay alive for it)
 
-    fn = getattr(_lib or load(), name) if _test_override is None else getattr(_test_override[0], name)
-    if device.type != "cuda":
-        return check(fn(*args, 0), what)
-    if device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
-            return check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
-    return check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
+
+def torch_calls():
+    """The module ``b200_torch_calls`` (csrc/torch_calls.cpp): entry points called with torch tensors."""
+    global _calls
+    if _calls is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries first)
+
+        path = Path(__file__).resolve().parent / "b200_torch_calls.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} not found: build it with `python build_native.py`; there is no fallback path without it")
+        loader = importlib.machinery.ExtensionFileLoader("b200_torch_calls", str(path))
+        _calls = importlib.util.module_from_spec(importlib.util.spec_from_loader("b200_torch_calls", loader))
+        loader.exec_module(_calls)
+    return _calls
+
+
+def entry(name: str) -> int:
+    """Address of entry point ``name`` of the library (or of the test stand-in) for ``torch_calls``."""
+    lib = _test_override[0] if _test_override is not None else _lib or load()
+    got = _entries.get(name)
+    if got is None or got[0] is not lib:
+        fn = getattr(lib, name)
+        if not isinstance(lib, C.CDLL):
+            restype, argtypes = SIGNATURES[name]
+            fn = C.CFUNCTYPE(restype, *argtypes)(fn)
+        got = _entries[name] = (lib, C.cast(fn, C.c_void_p).value, fn)
+    return got[1]
 
 
 def check(rc: int, what: str = "") -> None:

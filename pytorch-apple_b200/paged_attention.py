@@ -12,8 +12,7 @@ Work is enqueued on the current stream of the tensors' device.
 
 from __future__ import annotations
 
-import functools
-import struct
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -21,19 +20,13 @@ import torch
 
 from cuda_runtime import native
 
-_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_pack_append, _pack_attention = struct.Struct(native.PAGED_APPEND_FORMAT).pack, struct.Struct(native.ATTN_PAGED_FORMAT).pack
 
-
-# The checks of the two calls run in a few microseconds as long as they pass; what is wrong is looked for when they fail.
-def _seen(**tensors) -> str:
-    return ", ".join(f"{n} {tuple(t.shape)} {str(t.dtype)[6:]} strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}"
-                     for n, t in tensors.items())
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(max_q: int, Hq: int, Hkv: int, D: int, _lib) -> int:
-    return _lib.b200_attn_paged_workspace_bytes(max_q, Hq, Hkv, D)
+def _failed(what: str, rc: int, needs: str, **tensors):
+    """The call was not made (rc 1: the tensors do not fit) or refused by the library."""
+    if rc != 1:
+        native.check(rc, what)
+    raise ValueError(f"{what}: {needs}; got " + ", ".join(
+        f"{n} {tuple(t.shape)} {str(t.dtype)[6:]} strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}" for n, t in tensors.items()))
 
 
 def paged_append(q, k, v, cos, sin, k_pages, v_pages, slots, q_out=None):
@@ -42,39 +35,12 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, slots, q_out=None):
     ``q`` ``[N, Hq, D]`` (or None), ``k``, ``v`` ``[N, Hkv, D]``: any strides over tokens and heads (columns of a merged projection); ``cos``, ``sin``
     ``[N, D]`` in fp32 or the activation type (both None: no rotation); ``k_pages``, ``v_pages`` ``[pages, Hkv, page_size, D]``; ``slots`` int64 ``[N]``
     (page * page_size + row, negative: written nowhere).  ``q_out`` may be a dense ``q`` itself."""
-    dt, at = k.dtype, k.get_device()
-    ks, vs, ps, shape, pages = k.stride(), v.stride(), k_pages.stride(), k.shape, k_pages.shape
-    ok = len(shape) == 3 and len(pages) == 4 and dt in _CODES and v.shape == shape and v.dtype is dt and ks[2] == 1 and vs[2] == 1 and v.get_device() == at
-    ok = ok and pages == v_pages.shape and ps == v_pages.stride() and k_pages.dtype is dt and v_pages.dtype is dt and ps[3] == 1 and \
-        pages[1] == shape[1] and pages[3] == shape[2] and k_pages.get_device() == at and v_pages.get_device() == at
-    ok = ok and slots.dtype is torch.int64 and slots.shape == shape[:1] and slots.is_contiguous() and slots.get_device() == at
-    qs, Hq, q_at, out_at, c_at, s_at, table = (0, 0, 0), 0, 0, 0, 0, 0, 0
-    if ok and q is not None:
-        q_shape, qs = q.shape, q.stride()
-        ok = len(q_shape) == 3 and q.dtype is dt and qs[2] == 1 and q_shape[0] == shape[0] and q_shape[2] == shape[2] and q.get_device() == at
-        if q_out is None:
-            q_out = k.new_empty(q_shape)
-        else:
-            ok = ok and q_out.shape == q_shape and q_out.dtype is dt and q_out.is_contiguous() and q_out.get_device() == at
-        if ok:
-            Hq, q_at, out_at = q_shape[1], q.data_ptr(), q_out.data_ptr()
-    if ok and (cos is not None or sin is not None):
-        ok = cos is not None and sin is not None
-        if ok:
-            table = cos.dtype
-            ok = table in _CODES and sin.dtype is table and cos.shape == sin.shape == (shape[0], shape[2]) and cos.is_contiguous() and sin.is_contiguous() and \
-                cos.get_device() == at and sin.get_device() == at
-            table, c_at, s_at = _CODES.get(table), cos.data_ptr(), sin.data_ptr()
-    if not ok:
-        raise ValueError("paged_append: q [N, Hq, D] or None, k and v [N, Hkv, D] of one 16-bit type with contiguous rows, cos and sin dense [N, D] in fp32 or that "
-                         "type or both None, k_pages and v_pages alike [pages, Hkv, page_size, D], slots dense int64 [N], q_out dense like q, all on one "
-                         "device; got " + _seen(q=q, k=k, v=v, cos=cos, sin=sin, k_pages=k_pages, v_pages=v_pages, slots=slots, q_out=q_out))
-    if shape[0]:
-        native.on_stream(k.device, "paged_append", "b200_paged_append",
-                         _pack_append(q_at, k.data_ptr(), v.data_ptr(), c_at, s_at, out_at, k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(),
-                                      shape[0], pages[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ps[0], ps[1], ps[2],
-                                      Hq, shape[1], shape[2], pages[2], table, _CODES[dt]))
-    return q_out
+    out = native.torch_calls().paged_append(native.entry("b200_paged_append"), q, k, v, cos, sin, k_pages, v_pages, slots, q_out)
+    if out.__class__ is int:
+        _failed("paged_append", out, "q [N, Hq, D] or None, k and v [N, Hkv, D] of one type with contiguous rows, cos and sin dense [N, D] in fp32 or that type "
+                "or both None, k_pages and v_pages alike [pages, Hkv, page_size, D], slots dense int64 [N], q_out dense like q, all on one device",
+                q=q, k=k, v=v, cos=cos, sin=sin, k_pages=k_pages, v_pages=v_pages, slots=slots, q_out=q_out)
+    return out
 
 
 def paged_attention(q, k_pages, v_pages, q_start, kv_len, page_table, max_q, scale=None, window=0, out=None):
@@ -84,32 +50,13 @@ def paged_attention(q, k_pages, v_pages, q_start, kv_len, page_table, max_q, sca
     ``q_start[b + 1]``, at most ``max_q`` of them; ``kv_len`` int32 ``[B]``: its keys, the new tokens' among them; ``page_table`` int32 ``[B, n]``: its pages.
     A token sees the keys up to its own, with ``window`` > 0 the last ``window`` of them.  ``scale``: 1 / sqrt(D) unless given.  Rows of ``out`` behind
     the last sequence are left as they were (as they come, where ``out`` is made here)."""
-    dt, at = q.dtype, q.get_device()
-    qs, ps, shape, pages, table = q.stride(), k_pages.stride(), q.shape, k_pages.shape, page_table.shape
-    ok = len(shape) == 3 and len(pages) == 4 and len(table) == 2 and dt in _CODES and qs[2] == 1
-    ok = ok and pages == v_pages.shape and ps == v_pages.stride() and k_pages.dtype is dt and v_pages.dtype is dt and ps[3] == 1 and \
-        pages[3] == shape[2] and k_pages.get_device() == at and v_pages.get_device() == at
-    ok = ok and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32 and page_table.dtype is torch.int32 and kv_len.shape == table[:1] and \
-        q_start.shape == (table[0] + 1,) and q_start.is_contiguous() and kv_len.is_contiguous() and page_table.is_contiguous() and \
-        q_start.get_device() == at and kv_len.get_device() == at and page_table.get_device() == at
-    if ok and out is not None:
-        ok = out.shape == shape and out.dtype is dt and out.is_contiguous() and out.get_device() == at
-    if not ok:
-        raise ValueError("paged_attention: q [N, Hq, D] with contiguous rows, k_pages and v_pages alike [pages, Hkv, page_size, D] of its 16-bit type, q_start [B + 1], "
-                         "kv_len [B] and page_table [B, n] dense int32, out dense like q, all on one device; got " +
-                         _seen(q=q, k_pages=k_pages, v_pages=v_pages, q_start=q_start, kv_len=kv_len, page_table=page_table, out=out))
-    N, Hq, D = shape
-    if out is None:
-        out = q.new_empty(shape)
-    if N and table[0]:
-        # from the allocator on every call: a captured graph gets a workspace of its own, calls on other streams theirs
-        need = _workspace_bytes(max_q, Hq, pages[1], D, native.load())
-        space = q.new_empty((need + 1) // 2)
-        native.on_stream(q.device, "paged_attention", "b200_attn_paged",
-                         _pack_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(),
-                                         page_table.data_ptr(), space.data_ptr(), need, table[0], N, max_q, pages[0], table[1],
-                                         qs[0], qs[1], ps[0], ps[1], ps[2], window, Hq, pages[1], D, pages[2], _CODES[dt], D ** -0.5 if scale is None else scale))
-    return out
+    got = native.torch_calls().paged_attention(native.entry("b200_attn_paged"), native.entry("b200_attn_paged_workspace_bytes"), q, k_pages, v_pages, q_start, kv_len,
+                                               page_table, max_q, math.nan if scale is None else scale, window, out)
+    if got.__class__ is int:
+        _failed("paged_attention", got, "q [N, Hq, D] with contiguous rows, k_pages and v_pages alike [pages, Hkv, page_size, D] of its type, q_start [B + 1], kv_len "
+                "[B] and page_table [B, n] dense int32, out dense like q, all on one device", q=q, k_pages=k_pages, v_pages=v_pages, q_start=q_start,
+                kv_len=kv_len, page_table=page_table, out=out)
+    return got
 
 
 @dataclass

@@ -10,36 +10,21 @@ import torch
 
 from cuda_runtime import native
 
-_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
 def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
     """One token id per row of ``logits`` ``[rows, cols]`` (fp32, fp16 or bf16, any row stride); int64 ``[rows]``.
 
     ``uniform`` fp32 ``[rows]`` in [0, 1): the random numbers.  ``temperature`` (<= 0: the arg-max), ``top_p`` (>= 1: off), ``min_p`` (<= 0: off) fp32
     and ``top_k`` int32 (<= 0: off), each ``[rows]`` or None.  Filters apply in the order top-k, top-p (of what top-k leaves), min-p (relative to the
     likeliest token); the draw goes through what is kept in the order of the token ids.  Enqueued on the current stream of the logits' device."""
-    shape, at, step = logits.shape, logits.get_device(), logits.stride()
-    ok = len(shape) == 2 and logits.dtype in _CODES and shape[1] > 0 and (step[1] == 1 or shape[1] == 1)
-    one = shape[:1]
-    places = [0, 0, 0, 0, 0]
-    for i, (t, dtype) in enumerate(((uniform, torch.float32), (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))):
-        if t is not None:
-            ok = ok and t.dtype is dtype and t.shape == one and t.is_contiguous() and t.get_device() == at
-            places[i] = t.data_ptr()
-    if ok and out is not None:
-        ok = out.dtype is torch.int64 and out.shape == one and out.is_contiguous() and out.get_device() == at
-    if not ok or uniform is None:
+    got = native.torch_calls().sample_rows(native.entry("b200_sample_rows"), logits, uniform, temperature, top_k, top_p, min_p, out)
+    if got.__class__ is int:
+        if got != 1:
+            native.check(got, "sample_rows")
         raise ValueError("sample_rows: logits [rows, cols] of a float type with contiguous columns; uniform and, where given, temperature, top_p, min_p dense fp32 and "
                          "top_k dense int32 [rows]; out dense int64 [rows]; all on one device; got " +
                          ", ".join(f"{n} {tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}" for n, t in
                                    (("logits", logits), ("uniform", uniform), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("out", out))))
-    if out is None:
-        out = logits.new_empty(one, dtype=torch.int64)
-    if shape[0]:
-        native.on_stream(logits.device, "sample_rows", "b200_sample_rows", logits.data_ptr(), out.data_ptr(), shape[0], shape[1], step[0], places[1], places[2],
-                         places[3], places[4], places[0], _CODES[logits.dtype])
-    return out
+    return got
 
 
 class Sampler:

@@ -451,7 +451,7 @@ class FakeLibrary:
 
     def b200_attn_paged(self, args, stream):
         self.calls.append("attn_paged")
-        a = native.AttnPagedArgs.from_buffer_copy(args)
+        a = native.AttnPagedArgs.from_address(_addr(args))
         q, kp, vp, out, q_start, kv_len, table, B, N, Hq, Hkv, D = (a.q, a.k_pages, a.v_pages, a.out, a.q_start, a.kv_len, a.page_table, a.B, a.n_tokens, a.Hq,
                                                                     a.Hkv, a.D)
         num_pages, page, table_stride, qs, ks, window, scale, dtype = a.num_pages, a.page_size, a.table_stride, a.q_strides, a.kv_strides, a.window, a.scale, a.dtype
@@ -474,7 +474,7 @@ class FakeLibrary:
 
     def b200_paged_append(self, args, stream):
         self.calls.append("paged_append")
-        a = native.PagedAppendArgs.from_buffer_copy(args)
+        a = native.PagedAppendArgs.from_address(_addr(args))
         q, k, v, cos_t, sin_t, q_out, kp, vp, slots, N, Hq, Hkv, D = (a.q, a.k, a.v, a.cos_t, a.sin_t, a.q_out, a.k_pages, a.v_pages, a.slots, a.n_tokens, a.Hq,
                                                                       a.Hkv, a.D)
         num_pages, page, qs, ks, vs, ps, table_dtype, dtype = a.num_pages, a.page_size, a.q_strides, a.k_strides, a.v_strides, a.kv_strides, a.table_dtype, a.dtype
