@@ -40,8 +40,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   __shared__ int s_first[PAGED_MAX_PIECES + 1];   // blocks ahead of each piece of the list
   __shared__ float s_m[FEW_WARPS][ROWS], s_l[FEW_WARPS][ROWS];
   __shared__ int s_park[FEW_WARPS];               // where a warp has parked its accumulators (ring stage, -1: it has none)
-  __shared__ int64_t s_next, s_total[FEW_WARPS];
-  __shared__ int s_count;
+  __shared__ int64_t s_total[FEW_WARPS];
+  __shared__ int s_count, s_more;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
   uint8_t* const ring = smem + warp * FEW_RING;
@@ -53,10 +53,15 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
   const PagedWork work = paged_work(smem);   // (nothing has been copied into the rings yet)
-  int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);
-  const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > FEW_MIN_SHARE ? even : FEW_MIN_SHARE;
-  int64_t u0 = cta * share;
-  const int64_t u1 = u0 + share < total ? u0 + share : total;
+  int64_t u0 = 0, u1 = 0, share = 1, ends = 0;
+  auto deal = [&]() {   // this block's range of costs (as far as it is known to this warp)
+    const int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);
+    const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS;
+    share = even > FEW_MIN_SHARE ? even : FEW_MIN_SHARE;
+    u1 = (cta + 1) * share < total ? (cta + 1) * share : total;
+  };
+  deal();
+  u0 = cta * share;
   int4 head = make_int4(0, 0, 0, 0);
   const float sl = p.scale * LOG2E;
   uint32_t phase = 0;   // parity of each stage's next completion
@@ -68,13 +73,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   const uint32_t ring_addr = smem_u32(ring);
   const uint32_t k_row = (8 * (mi & 1) + mr) * 128, v_row = (8 * (mi >> 1) + mr) * 128;
 
-  while (u0 < u1) {
+  while (true) {
     if (warp == 0) {
-      int count;
-      const int64_t next = paged_pieces<FEW_KEYS, FEW_OV>(p, tpt, work, u0, u1, share, s_piece, count, head);
+      int count = 0;
+      if (u0 < u1) u0 = paged_pieces<FEW_KEYS, FEW_OV>(p, tpt, work, u0, u1, s_piece, count, head, ends);
       __syncwarp();
       if (lane == 0) {
-        s_next = next;
+        s_more = u0 < u1;
         s_count = count;
         int run = 0;
         for (int f = 0; f < count; ++f) { s_first[f] = run; run += s_piece[f].cnt; }
@@ -82,8 +87,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
       }
     }
     __syncthreads();
-    const int F = s_count, X = s_first[F];
-    u0 = s_next;
+    const int F = s_count;
+    const bool more = s_more;
+    if (F == 0) break;   // (a range that no item begins or goes on in)
+    const int X = s_first[F];
 
     // Copies: block x of the list is warp x % 8's; its page and row are looked up 32 blocks ahead, one per lane
     int id_page = 0, id_row = 0, id_hk = 0, next_page = 0, next_row = 0, next_hk = 0;
@@ -332,9 +339,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
       __syncthreads();
       if (parked >= 0) copy();
     }
-    if (u0 < u1) total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);   // (the rings lay over the running costs)
+    if (!more) break;
+    deal();   // (the rings lay over the running costs)
   }
-  if (threadIdx.x == 0) p.head[cta] = head;
+  if (threadIdx.x == 0 && !p.whole) {
+    if (head.x) head.x = static_cast<int>((ends - 1) / share) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
+    p.head[cta] = head;
+  }
 }
 
 // ===========================================================================
@@ -543,6 +554,9 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
   p.ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + ml);
   p.acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + acc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Short tables: no cache is so long that a block of its own for each item would take longer than joining pieces does (4 us, and a launch
+  // on the host).  us, pieces -> whole: one sequence of 613 keys 10.7 -> 8.5, 19 with four tokens each and up to 1111 keys of 64 dims 15.5 -> 13.3.
+  p.whole = a.table_stride * a.page_size * D <= (rows == PAGED_TC5_ROWS ? 512 : 1024) * 128 ? 1 : 0;
   int rc = B200_ENOTSUP;
   if (tc5_enabled()) {
     if (rows == PAGED_TC5_ROWS) {
@@ -560,7 +574,7 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
       launch_pdl(D == 128 ? attn_paged_plain_kernel<T, 128> : attn_paged_plain_kernel<T, 64>, dim3(static_cast<unsigned>(ceil_div(a.n_tokens * Hq, 4))),
                  dim3(128), 0, st, p);
     });
-  } else {
+  } else if (!p.whole) {
     B200_DISPATCH_HALF(dtype, T, {
       const auto merge = [&](auto kernel, int groups) { launch_pdl(kernel, dim3(PAGED_CTAS, static_cast<unsigned>(groups)), dim3(256), 0, st, p); };
       if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8, 1>, 8); else merge(attn_paged_merge_kernel<T, 64, 8, 1>, 8); }

@@ -13,6 +13,7 @@ struct PagedParams {
   int Hq, Hkv, G, page_size;
   int64_t window;                  // keys a token sees back from its own (0: all)
   float scale;
+  int whole;                       // items are not cut: a block takes those that begin in its range
   // partial results (paged_workspace)
   int4* head;                      // [PAGED_CTAS]: {pieces, first token, KV head, rows} of the item that begins in a block and ends in a later one
   float2* ml;                      // [PAGED_CTAS][2][rows]: (maximum in the log2 domain, sum)
@@ -80,10 +81,12 @@ __device__ __forceinline__ PagedWork paged_work(void* at) {
   return w;
 }
 
-// Fills `w`; returns pre[B].  All THREADS threads; ends with a barrier.
+// Fills `w`; returns pre[B].  All THREADS threads (up to 32 sequences: the first warp alone, the others get no answer); ends with a barrier
+// (of the warp).
 template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const PagedParams& p, int tpt, const PagedWork& w, int64_t* warp_total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = static_cast<int>(p.B);
   const int chunk = (B + THREADS - 1) / THREADS;
+  if (B <= 32 && warp > 0) return 0;
   int64_t run = 0;
   for (int c = 0; c < chunk; ++c) {
     const int b = threadIdx.x * chunk + c;
@@ -115,6 +118,12 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
     const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += t;
   }
+  if (B <= 32) {
+    if (lane < B) w.pre[lane + 1] = upto;
+    if (lane == 0) w.pre[0] = 0;
+    __syncwarp();
+    return __shfl_sync(0xffffffffu, upto, 31);
+  }
   if (lane == 31) warp_total[warp] = upto;
   __syncthreads();
   int64_t before = upto - run, total = 0;
@@ -133,9 +142,9 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
 }
 
 // The pieces of items in the costs [u0, u1), at most PAGED_MAX_PIECES; returns where to go on (u1: that was all).  One whole warp.
-// head is written where an item begins in this block and does not end in it: how many blocks have pieces of it, and whose rows they are.
+// head is written where an item begins in this block and does not end in it: whose rows they are, and (ends) where it ends.
 template <int KT, int OV>
-__device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& w, int64_t u0, int64_t u1, int64_t share, PagedPiece* list, int& count, int4& head) {
+__device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& w, int64_t u0, int64_t u1, PagedPiece* list, int& count, int4& head, int64_t& ends) {
   const int lane = threadIdx.x & 31, B = static_cast<int>(p.B);
   count = 0;
   int lo = 0, hi = B;   // the last sequence that begins at or before u0 (and so is not empty)
@@ -167,7 +176,9 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
         const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const int64_t start = base + upto - cost + OV, end = base + upto, a = u0 > start ? u0 : start, z = u1 < end ? u1 : end;
+      const int64_t start = base + upto - cost + OV, end = base + upto;
+      const bool here = start >= u0 && start < u1;
+      const int64_t a = p.whole ? start : u0 > start ? u0 : start, z = p.whole ? (here ? end : start) : u1 < end ? u1 : end;
       const unsigned mine = __ballot_sync(0xffffffffu, e < items && a < z);
       const int at = count + __popc(mine & ((1u << lane) - 1u));
       const bool taken = ((mine >> lane) & 1u) && at < PAGED_MAX_PIECES;
@@ -187,7 +198,8 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
       const unsigned opens = __ballot_sync(0xffffffffu, taken && a == start && z < end);
       if (opens) {
         const int src = __ffs(opens) - 1;
-        head.x = static_cast<int>((__shfl_sync(0xffffffffu, end, src) - 1) / share - __shfl_sync(0xffffffffu, start, src) / share) + 1;
+        ends = __shfl_sync(0xffffffffu, end, src);
+        head.x = 1;
         head.y = __shfl_sync(0xffffffffu, first + t.t0, src);
         head.z = __shfl_sync(0xffffffffu, h, src);
         head.w = __shfl_sync(0xffffffffu, (t.t1 - t.t0) * p.G, src);
@@ -196,7 +208,7 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
       if (count > PAGED_MAX_PIECES) {   // go on behind the last one taken
         const unsigned last = __ballot_sync(0xffffffffu, taken && at == PAGED_MAX_PIECES - 1);
         count = PAGED_MAX_PIECES;
-        return last ? __shfl_sync(0xffffffffu, z, __ffs(last) - 1) : base;   // (none of this round was taken: they begin at base or later)
+        return last ? __shfl_sync(0xffffffffu, p.whole ? start + 1 : z, __ffs(last) - 1) : base;   // (none of this round was taken: they begin at base or later)
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
     }

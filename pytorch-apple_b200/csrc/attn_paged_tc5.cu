@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __shared__ __align__(8) uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   __shared__ uint32_t tmem_holder;
   __shared__ __align__(16) PagedPiece s_piece[PAGED_MAX_PIECES];
-  __shared__ int64_t s_next, s_total[THREADS / 32];
-  __shared__ int s_count, failed;
+  __shared__ int64_t s_total[THREADS / 32];
+  __shared__ int s_count, s_more, failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
   if (warp == 9 && lane == 0) {
@@ -89,26 +89,33 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
   const PagedWork work = paged_work(smem);   // (no tile has been copied yet)
-  tc5::tc_fence_before();
-  int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);
-  tc5::tc_fence_after();
-  const uint32_t tmem_base = tmem_holder;
-  const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS, share = even > MIN_SHARE ? even : MIN_SHARE;
-  int64_t u0 = cta * share;
-  const int64_t u1 = u0 + share < total ? u0 + share : total;
+  int64_t u0 = 0, u1 = 0, share = 1, ends = 0;
+  auto deal = [&]() {   // this block's range of costs (as far as it is known to this warp)
+    const int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);
+    const int64_t even = (total + PAGED_CTAS - 1) / PAGED_CTAS;
+    share = even > MIN_SHARE ? even : MIN_SHARE;
+    u1 = (cta + 1) * share < total ? (cta + 1) * share : total;
+  };
+  deal();
+  u0 = cta * share;
   int4 head = make_int4(0, 0, 0, 0);
+  uint32_t tmem_base = 0;
   int n = 0, fg = 0;   // tiles and pieces behind this block, the same in every role
 
-  while (u0 < u1) {
+  while (true) {
     if (warp == 0) {
-      int count;
-      const int64_t next = paged_pieces<BKV, OV>(p, tpt, work, u0, u1, share, s_piece, count, head);
-      if (lane == 0) { s_next = next; s_count = count; }
+      int count = 0;
+      if (u0 < u1) u0 = paged_pieces<BKV, OV>(p, tpt, work, u0, u1, s_piece, count, head, ends);
+      if (lane == 0) { s_more = u0 < u1; s_count = count; }
     }
     tc5::fence_proxy_async();   // the tiles are copied over what has been written here
+    tc5::tc_fence_before();
     __syncthreads();
+    tc5::tc_fence_after();
+    tmem_base = tmem_holder;
     const int F = s_count;
-    u0 = s_next;
+    const bool more = s_more;
+    if (F == 0) break;   // (a range that no item begins or goes on in)
 
     if (warp >= 9) {   // ---- TMA producers, of Q and K and of V: lane l brings rows [l * box, (l + 1) * box) of a tile ----
       const bool is_k = warp == 9;
@@ -402,9 +409,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int f = 0; f < F; ++f) n += s_piece[f].cnt;
     fg += F;
     if (__syncthreads_or(*reinterpret_cast<volatile int*>(&failed))) break;   // (what the threads see may differ: they agree)
-    if (u0 < u1) total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);   // (the tiles lay over it)
+    if (!more) break;
+    deal();   // (the tiles lay over it)
   }
-  if (threadIdx.x == 0) p.head[cta] = head;
+  if (threadIdx.x == 0 && !p.whole) {
+    if (head.x) head.x = static_cast<int>((ends - 1) / share) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
+    p.head[cta] = head;
+  }
   tc5::tc_fence_before();
   __syncthreads();
   if (warp == 8) { tc5::tc_fence_after(); tc5::tmem_dealloc(tmem_base, TMEM_COLS); }
