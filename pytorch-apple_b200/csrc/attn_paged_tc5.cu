@@ -7,9 +7,11 @@
 // What is attended follows from positions alone: a tile that reaches past a row's last key or ahead of its window is masked in
 // registers, rows of V that no row of the tile may see are cleared in shared memory (0 times what lies there need not be 0).
 //
-// Within a tile as in the attention over static prompts: two groups of four softmax warps share a tile, group g on its keys
-// 64 g .. 64 g + 63 with running maxima and an accumulator of its own, one thread per row; the stored maximum follows the true one when that
-// has grown by more than RESCALE_STEP.  A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
+// Two groups of four softmax warps share a tile, group g on its keys 64 g .. 64 g + 63 with running maxima and an accumulator of its
+// own, one thread per row; the stored maximum follows the true one when that has grown by more than RESCALE_STEP.  What an SM's shared memory
+// delivers is the bound (operands of both products, probabilities and the arriving tiles were 224 KB a tile, 0.91 us of the 1.57 it took), so the probabilities
+// stay in tensor memory: they replace the scores that they come from and are the A operand of the second product from there (160 KB a tile, and room for
+// a third stage of keys, whose copies were late with two). A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
 // next item's first tile are computed while the last one's rows are written.
 //
 // Warp roles: warps 0-3 and 4-7 the softmax groups, warp 8 MMA issuer and owner of the tensor memory, warps 9 and 10 TMA producers (Q and K; V), a box per lane.  Every
@@ -46,7 +48,10 @@ __device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc5::smem_addr(bar)) : "memory");
 }
 
-constexpr int smem_bytes(int D) { return (5 * (D / 64) + 4) * PANEL + 1024; }   // Q, K x 2, V x 2, P x 2 (two panels each), alignment
+constexpr int KST = 3;                         // stages of K (V: two)
+constexpr int OUT_BYTES = 2 * PANEL;           // where rows are turned round on their way out, 4 KB per softmax warp
+constexpr int smem_bytes(int D) { return (3 + KST) * (D / 64) * PANEL + OUT_BYTES + 1024; }   // Q, K, V, rows, alignment
+static_assert(smem_bytes(64) >= paged_work_bytes + 1024, "the sequences' costs lie over the tiles");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -57,10 +62,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* q_s = smem;
   uint8_t* k_s = smem + TILE;
-  uint8_t* v_s = smem + 3 * TILE;
-  uint8_t* p_s = smem + 5 * TILE;
-  // tile n of the block lives in stage / buffer n & 1
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint8_t* v_s = smem + (1 + KST) * TILE;
+  uint8_t* out_s = smem + (3 + KST) * TILE;
+  // tile n of the block: keys in stage n % KST, values in stage n & 1, scores and probabilities in buffer n & 1
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[KST], k_empty[KST], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   __shared__ uint32_t tmem_holder;
   __shared__ __align__(16) PagedPiece s_piece[PAGED_MAX_PIECES];
   __shared__ int64_t s_total[THREADS / 32];
@@ -71,9 +76,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     failed = 0;
     tc5::mbar_init(&q_full, 1);
     tc5::mbar_init(&q_empty, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < KST; ++s) {
       tc5::mbar_init(&k_full[s], 1);
       tc5::mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
       tc5::mbar_init(&v_full[s], 1);
       tc5::mbar_init(&v_empty[s], 1);
       tc5::mbar_init(&s_full[s], 1);
@@ -119,6 +126,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (warp >= 9) {   // ---- TMA producers, of Q and K and of V: lane l brings rows [l * box, (l + 1) * box) of a tile ----
       const bool is_k = warp == 9;
+      const int stages = is_k ? KST : 2;
       const CUtensorMap* const map = is_k ? &map_k : &map_v;
       uint64_t *const full = is_k ? k_full : v_full, *const empty = is_k ? k_empty : v_empty;
       uint8_t* const tiles = (is_k ? k_s : v_s) + lane * box * 128;
@@ -150,12 +158,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int f = 0; f < F && ok; ++f) {
         const int cnt = c.cnt, hk = c.hk, token = c.token;
         for (int k = 0; k < cnt && ok; ++k, ++at) {
-          const int st = at & 1;
+          const int turn = at / stages, st = at - turn * stages;
           const Rows a = next;
           if (k + 1 < cnt) next = locate(c, k + 1);
           else if (f + 1 < F) { c = s_piece[f + 1]; next = locate(c, 0); }
           const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, a.there))) * box * 128 * NP;
-          if (at >= 2 && !(ok = wait(&empty[st], ((at >> 1) & 1) ^ 1, is_k ? 50 : 52))) break;
+          if (turn > 0 && !(ok = wait(&empty[st], (turn & 1) ^ 1, is_k ? 50 : 52))) break;
           if (is_k && k == 0) {
             if (fg + f >= 1 && !(ok = wait(&q_empty, (fg + f - 1) & 1, 51))) break;
             if (lane == 0) {
@@ -176,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // on a failure elsewhere the copies in flight must land before the block leaves
       if (*reinterpret_cast<volatile int*>(&failed)) {
         if (is_k && q_at > 0) tc5::mbar_wait(&q_full, (q_at - 1) & 1, 1u << 16);
-        for (int i = kv_at > 2 ? kv_at - 2 : 0; i < kv_at; ++i) tc5::mbar_wait(&full[i & 1], (i >> 1) & 1, 1u << 16);
+        for (int i = kv_at > stages ? kv_at - stages : 0; i < kv_at; ++i) tc5::mbar_wait(&full[i % stages], (i / stages) & 1, 1u << 16);
       }
     } else if (warp == 8) {
       if (lane == 0) {   // ---- MMA issuer ----
@@ -187,15 +195,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         // scores run up to two tiles ahead of the products with V: (sf, sk) is the next tile whose scores are to be issued
         int sf = 0, sk = 0, sn = n;
         auto issue_s = [&](bool look) {   // look: the K tile has not been looked for by the softmax threads
-          const int st = sn & 1;
+          const int st = sn & 1, turn = sn / KST, ks = sn - turn * KST;
           if (sk == 0 && !tc5::mbar_wait(&q_full, (fg + sf) & 1)) return false;
-          if (look && !tc5::mbar_wait(&k_full[st], (sn >> 1) & 1)) return false;
+          if (look && !tc5::mbar_wait(&k_full[ks], turn & 1)) return false;
           tc5::tc_fence_after();
-          const uint32_t k_lo = tc5::desc_sw128_lo(tc5::smem_addr(k_s + st * TILE));
+          const uint32_t k_lo = tc5::desc_sw128_lo(tc5::smem_addr(k_s + ks * TILE));
 #pragma unroll
           for (int h = 0; h < NP; ++h) tc5::umma_f16_kblock(tmem_base + 128 * st, q_lo + h * (PANEL >> 4), k_lo + h * (PANEL >> 4), idesc_s, h > 0);
           tc5::umma_commit(&s_full[st]);
-          tc5::umma_commit(&k_empty[st]);
+          tc5::umma_commit(&k_empty[ks]);
           if (++sk == s_piece[sf].cnt) {
             tc5::umma_commit(&q_empty);
             ++sf;
@@ -210,18 +218,19 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int cnt = s_piece[f].cnt;
           for (int k = 0; k < cnt && ok; ++k, ++at) {
             const int st = at & 1;
-            const uint32_t v_addr = tc5::smem_addr(v_s + st * TILE), p_addr = tc5::smem_addr(p_s + st * 2 * PANEL);
+            const uint32_t v_addr = tc5::smem_addr(v_s + st * TILE);
             if (!(ok = tc5::mbar_wait(&p_ready[st], (at >> 1) & 1))) break;
             tc5::tc_fence_after();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {     // 16 keys per instruction = two 8-key groups of the V panels
-              const uint64_t da = tc5::umma_desc_sw128(p_addr + (e >> 2) * PANEL) + 2 * (e & 3);
               const uint64_t db = tc5::umma_desc_sw128_mn(v_addr + e * 2048, PANEL, 1024);
-              tc5::umma_f16(tmem_base + 256 + 128 * (e >> 2), da, db, idesc_o, k > 0 || (e & 3) != 0);
+              tc5::umma_f16_ta(tmem_base + 256 + 128 * (e >> 2), tmem_base + 128 * st + 64 * (e >> 2) + 8 * (e & 3), db, idesc_o, k > 0 || (e & 3) != 0);
             }
             tc5::umma_commit(&o_full[st]);
             tc5::umma_commit(&v_empty[st]);
-            if (sf < F) ok = issue_s(false);
+            // (The queries of the next item are on their way once the last scores of this one are done: as long as there are scores for the
+            // softmax threads, its first tile waits until after the next product.)
+            while (ok && sf < F && sn <= at + 2 && !(sk == 0 && sn == at + 2 && !tc5::mbar_try_wait(&q_full, (fg + sf) & 1))) ok = issue_s(false);
           }
         }
         if (!ok && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, 53); }
@@ -255,8 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int k = 0; k < pc.cnt && alive; ++k, ++at, --left) {
           const int st = at & 1, key0 = (pc.j0 + k) * BKV;
-          uint8_t* const p_own = p_s + st * 2 * PANEL + g * PANEL + r * 128;
-          // S of this tile: its barrier also says that every product issued before it, that of this buffer's last probabilities among them, is complete
+          const uint32_t t_s = t_lane + 128 * st + 64 * g;   // this thread's scores, and where its probabilities replace them
           if (!wait_all(&s_full[st], (at >> 1) & 1, 54)) { alive = false; break; }
           tc5::tc_fence_after();
           // A tile that all rows see all of: the probabilities follow the scores at once, relative to the maximum so far; where a row has outgrown it the
@@ -265,6 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (warp_live && k > 0 && c > 0.f && key0 + BKV <= pc.p0 + 1 && (p.window == 0 || key0 + p.window >= pc.p0 + tokens)) {
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             float sum[4] = {0.f, 0.f, 0.f, 0.f}, mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            uint32_t w[32];
             auto probabilities = [&](float (&u)[32], int q0) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
@@ -278,24 +287,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                   pr[e + 1] = ex2(d);
                   tc5::add2(sum[e & 2], sum[(e & 2) + 1], pr[e], pr[e + 1]);
                 }
-                *reinterpret_cast<uint4*>(p_own + (((q0 + q) ^ (r & 7)) << 4)) = pack8<T>(pr);
+                const uint4 v = pack8<T>(pr);
+                w[4 * (q0 + q)] = v.x; w[4 * (q0 + q) + 1] = v.y; w[4 * (q0 + q) + 2] = v.z; w[4 * (q0 + q) + 3] = v.w;
               }
             };
             float u0_[32], u1_[32];
-            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g, u0_);
+            tc5::tmem_ld_32x32_async(t_s, u0_);
             tc5::tmem_ld_wait();
-            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g + 32, u1_);
+            tc5::tmem_ld_32x32_async(t_s + 32, u1_);
             probabilities(u0_, 0);
             tc5::tmem_ld_wait();
             probabilities(u1_, 4);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
             done = !__any_sync(0xffffffffu, row_live && (top > m_run + RESCALE_STEP || (m_run == -INFINITY && top > m_run)));
-            if (done) l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (done) {
+              l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+              tc5::tmem_st_32x32_raw(t_s, w);
+            }
           }
           if (warp_live && !done) {
             float u[64];
-            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g, *reinterpret_cast<float(*)[32]>(&u[0]));
-            tc5::tmem_ld_32x32_async(t_lane + 128 * st + 64 * g + 32, *reinterpret_cast<float(*)[32]>(&u[32]));
+            tc5::tmem_ld_32x32_async(t_s, *reinterpret_cast<float(*)[32]>(&u[0]));
+            tc5::tmem_ld_32x32_async(t_s + 32, *reinterpret_cast<float(*)[32]>(&u[32]));
             tc5::tmem_ld_wait();
             float to_log2 = c;
             if (c <= 0.f) {   // (with the factor left for later the maximum would be the minimum, and 0 times a masked key's -infinity no number)
@@ -336,6 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             m_run = m_new;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t w[32];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               float pr[8];
@@ -347,9 +361,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 pr[e + 1] = ex2(d);
                 tc5::add2(sum[e & 2], sum[(e & 2) + 1], pr[e], pr[e + 1]);
               }
-              *reinterpret_cast<uint4*>(p_own + ((q ^ (r & 7)) << 4)) = pack8<T>(pr);
+              const uint4 v = pack8<T>(pr);
+              w[4 * q] = v.x; w[4 * q + 1] = v.y; w[4 * q + 2] = v.z; w[4 * q + 3] = v.w;
             }
             l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc5::tmem_st_32x32_raw(t_s, w);
           }
           if (key0 + BKV > hi || key0 < lo) {   // clear the rows of V that no row sees
             if (!wait_all(&v_full[st], (at >> 1) & 1, 56)) { alive = false; break; }
@@ -359,24 +375,25 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 4 * NP; ++e) reinterpret_cast<uint4*>(at_v)[e] = make_uint4(0, 0, 0, 0);
             }
+            tc5::fence_proxy_async();   // (the tensor core reads through the async proxy)
           }
-          tc5::fence_proxy_async();   // the probabilities are read by the tensor core (async proxy)
-          tc5::tc_fence_before();     // this thread's tcgen05.ld / st are complete before S and O are touched again
+          if (warp_live) tc5::tmem_st_wait();
+          tc5::tc_fence_before();     // this thread's tcgen05.ld / st are complete before its probabilities are read, S and O touched again
           // what the products of this tile and the scores of the one after next read has landed: looked for by one warp per group
           if (quarter == 0) {
-            if (g == 0 ? !wait_all(&v_full[st], (at >> 1) & 1, 57) : left > 2 && !wait_all(&k_full[st], ((at + 2) >> 1) & 1, 58)) { alive = false; break; }
+            if (g == 0 ? !wait_all(&v_full[st], (at >> 1) & 1, 57) : left > 2 && !wait_all(&k_full[(at + 2) % KST], ((at + 2) / KST) & 1, 58)) { alive = false; break; }
           }
           mbar_arrive1(&p_ready[st]);
         }
         // ---- the piece's rows: the half of the head dimension that this group writes, from both accumulators ----
         if (alive) alive = wait_all(&o_full[(at - 1) & 1], ((at - 1) >> 1) & 1, 59);
-        float* const ml = reinterpret_cast<float*>(p_s + g * PANEL);   // (the probabilities have been read)
+        float* const ml = reinterpret_cast<float*>(out_s + g * 1024);
         ml[r] = m_run;
         ml[128 + r] = l_run;
         tc5::tc_fence_before();
         asm volatile("bar.sync 1, 256;" ::: "memory");
         tc5::tc_fence_after();
-        const float *ml_0 = reinterpret_cast<const float*>(p_s) + r, *ml_1 = reinterpret_cast<const float*>(p_s + PANEL) + r;
+        const float *ml_0 = reinterpret_cast<const float*>(out_s) + r, *ml_1 = reinterpret_cast<const float*>(out_s + 1024) + r;
         const float m_0 = ml_0[0], m_1 = ml_1[0], l_0 = ml_0[128], l_1 = ml_1[128];
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (alive && warp_live) {
@@ -391,8 +408,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const int64_t slot = paged_slot(cta, pc.flags & 1, PAGED_TC5_ROWS);
           if (!whole && g == 0 && row_live) p.ml[slot + r] = make_float2(m_all, l_all);
-          // Through this warp's rows of the probability buffers (chunk c of row r at c ^ (r & 7)), so that rows leave in whole lines
-          uint8_t* const own = p_s + g * PANEL + 32 * quarter * 128;
+          // Through 4 KB of this warp's (chunk c of row r at c ^ (r & 7)), so that rows leave in whole lines: half a row of results at once, 32 of the
+          // fp32 sums at a time
+          uint8_t* const own = out_s + warp * 4096;
+          const int live = pc.rows - 32 * quarter < 32 ? pc.rows - 32 * quarter : 32;   // rows of this warp
+          const int64_t to = ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
+          float* const part = p.acc + (slot + 32 * quarter) * D + g * (D / 2);
 #pragma unroll
           for (int q = 0; q < D / 2; q += 32) {
             float t0[32], t1[32];
@@ -406,33 +427,29 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (int e = 0; e < 4; ++e)
                 *reinterpret_cast<uint4*>(own + lane * 128 + (((q / 8 + e) ^ (r & 7)) << 4)) = pack8<T>(*reinterpret_cast<float(*)[8]>(&t0[8 * e]));
             } else {
+              __syncwarp();   // (the 32 before have been read)
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(own + (q / 32) * 2 * PANEL + lane * 128 + ((e ^ (r & 7)) << 4)) = *reinterpret_cast<float4*>(&t0[4 * e]);
+                *reinterpret_cast<float4*>(own + lane * 128 + ((e ^ (r & 7)) << 4)) = *reinterpret_cast<float4*>(&t0[4 * e]);
+              __syncwarp();
+#pragma unroll
+              for (int it = 0; it < 8; ++it) {
+                const int row = it * 4 + lane / 8, ch = lane % 8;
+                if (row < live)
+                  *reinterpret_cast<float4*>(part + static_cast<int64_t>(row) * D + q + ch * 4) = *reinterpret_cast<const float4*>(own + row * 128 + ((ch ^ (row & 7)) << 4));
+              }
             }
           }
           tc5::tc_fence_before();
-          __syncwarp();
-          const int live = pc.rows - 32 * quarter < 32 ? pc.rows - 32 * quarter : 32;   // rows of this warp
           if (whole) {
             constexpr int CH = D / 16;   // 16-byte chunks of half a row
-            const int64_t to = ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
+            __syncwarp();
 #pragma unroll
             for (int it = 0; it < CH; ++it) {
               const int row = it * (32 / CH) + lane / CH, ch = lane % CH;
               const int64_t dst = __shfl_sync(0xffffffffu, to, row);
               if (row < live)
                 *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + dst + ch * 8) = *reinterpret_cast<const uint4*>(own + row * 128 + ((ch ^ (row & 7)) << 4));
-            }
-          } else {
-            constexpr int CH = D / 8;
-            float* const part = p.acc + (slot + 32 * quarter) * D + g * (D / 2);
-#pragma unroll
-            for (int it = 0; it < CH; ++it) {
-              const int row = it * (32 / CH) + lane / CH, ch = lane % CH;
-              if (row < live)
-                *reinterpret_cast<float4*>(part + static_cast<int64_t>(row) * D + ch * 4) =
-                    *reinterpret_cast<const float4*>(own + (ch / 8) * 2 * PANEL + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
             }
           }
           __syncwarp();
