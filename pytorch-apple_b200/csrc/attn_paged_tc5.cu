@@ -11,7 +11,7 @@
 // own, one thread per row; the stored maximum follows the true one when that has grown by more than RESCALE_STEP.  What an SM's shared memory
 // delivers is the bound (operands of both products, probabilities and the arriving tiles were 224 KB a tile, 0.91 us of the 1.57 it took), so the probabilities
 // stay in tensor memory: they replace the scores that they come from and are the A operand of the second product from there (160 KB a tile, and room for
-// a third stage of keys, whose copies were late with two). A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
+// a second stage of queries). A block walks through its pieces (attn_paged.cuh) without draining: the scores of the
 // next item's first tile are computed while the last one's rows are written.
 //
 // Warp roles: warps 0-3 and 4-7 the softmax groups, warp 8 MMA issuer and owner of the tensor memory, warps 9 and 10 TMA producers (Q and K; V), a box per lane.  Every
@@ -48,24 +48,26 @@ __device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc5::smem_addr(bar)) : "memory");
 }
 
-constexpr int KST = 3;                         // stages of K (V: two)
 constexpr int OUT_BYTES = 2 * PANEL;           // where rows are turned round on their way out, 4 KB per softmax warp
-constexpr int smem_bytes(int D) { return (3 + KST) * (D / 64) * PANEL + OUT_BYTES + 1024; }   // Q, K, V, rows, alignment
+constexpr int smem_bytes(int D) { return 6 * (D / 64) * PANEL + OUT_BYTES + 1024; }   // Q, K, V twice each, rows, alignment
 static_assert(smem_bytes(64) >= paged_work_bytes + 1024, "the sequences' costs lie over the tiles");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     attn_paged_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                          const __grid_constant__ PagedParams p, const int tpt, const int box) {
+                          const __grid_constant__ PagedParams p, const int tpt, const int log_box) {
+  const int box = 1 << log_box;                   // keys of a copy
   constexpr int NP = D / 64, TILE = NP * PANEL;   // panels and bytes of a K, V or Q tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* q_s = smem;
-  uint8_t* k_s = smem + TILE;
-  uint8_t* v_s = smem + (1 + KST) * TILE;
-  uint8_t* out_s = smem + (3 + KST) * TILE;
-  // tile n of the block: keys in stage n % KST, values in stage n & 1, scores and probabilities in buffer n & 1
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[KST], k_empty[KST], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint8_t* k_s = smem + 2 * TILE;
+  uint8_t* v_s = smem + 4 * TILE;
+  uint8_t* out_s = smem + 6 * TILE;
+  // tile n of the block lives in stages and buffers n & 1, the queries of piece f in stage f & 1.  A stage of K is free when the scores made from it
+  // are there, one of V when the product is: the producers wait for what the softmax threads wait for (the next phase of these barriers
+  // needs the copy that they are about to issue, so they cannot miss one).
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[2], v_full[2], s_full[2], p_ready[2], o_full[2];
   __shared__ uint32_t tmem_holder;
   __shared__ __align__(16) PagedPiece s_piece[PAGED_MAX_PIECES];
   __shared__ int64_t s_total[THREADS / 32];
@@ -74,15 +76,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
   if (warp == 9 && lane == 0) {
     failed = 0;
-    tc5::mbar_init(&q_full, 1);
-    tc5::mbar_init(&q_empty, 1);
-    for (int s = 0; s < KST; ++s) {
-      tc5::mbar_init(&k_full[s], 1);
-      tc5::mbar_init(&k_empty[s], 1);
-    }
     for (int s = 0; s < 2; ++s) {
+      tc5::mbar_init(&q_full[s], 1);
+      tc5::mbar_init(&q_empty[s], 1);
+      tc5::mbar_init(&k_full[s], 1);
       tc5::mbar_init(&v_full[s], 1);
-      tc5::mbar_init(&v_empty[s], 1);
       tc5::mbar_init(&s_full[s], 1);
       tc5::mbar_init(&p_ready[s], 256);
       tc5::mbar_init(&o_full[s], 1);
@@ -126,9 +124,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (warp >= 9) {   // ---- TMA producers, of Q and K and of V: lane l brings rows [l * box, (l + 1) * box) of a tile ----
       const bool is_k = warp == 9;
-      const int stages = is_k ? KST : 2;
       const CUtensorMap* const map = is_k ? &map_k : &map_v;
-      uint64_t *const full = is_k ? k_full : v_full, *const empty = is_k ? k_empty : v_empty;
+      uint64_t *const full = is_k ? k_full : v_full, *const empty = is_k ? s_full : o_full;
       uint8_t* const tiles = (is_k ? k_s : v_s) + lane * box * 128;
       bool ok = true;
       int q_at = fg, kv_at = n;   // copies issued
@@ -138,14 +135,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!got && !gone && lane == 0) { failed = 1; atomicExch(&g_attn_paged_error, code); }
         return __all_sync(0xffffffffu, got && !gone);
       };
-      // the lane's rows of a tile: page and first row, looked up a tile ahead (a page number is a round trip to L2)
-      struct Rows { int page, row; bool there; };
-      auto locate = [&](const PagedPiece& c, int k) {
+      // Boxes of the next 32 / per_tile tiles of a piece, one per lane: page and first row (a page number is a round trip to L2: looked up a batch ahead)
+      struct Rows { int page, row; };
+      const int log_boxes = 7 - log_box, batch = 32 >> log_boxes;   // boxes of a tile, tiles looked up at a time
+      auto locate = [&](const PagedPiece& c, int k0) {
         const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
         const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
-        const int key = (c.j0 + k) * BKV + lane * box;
-        Rows a = {0, 0, lane * box < BKV && key < hi && key + box > lo};
-        if (a.there) {
+        const int k = k0 + (lane >> log_boxes), key = (c.j0 + k) * BKV + (lane & ((1 << log_boxes) - 1)) * box;
+        Rows a = {0, -1};
+        if (k < c.cnt && key < hi && key + box > lo) {
           const int i = key / p.page_size;
           a.row = key - i * p.page_size;
           a.page = __ldg(p.table + c.b * p.table_stride + i);
@@ -154,58 +152,63 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       int at = n;
       PagedPiece c = s_piece[0];
-      Rows next = locate(c, 0);
+      Rows next = locate(c, 0), cur = next;
       for (int f = 0; f < F && ok; ++f) {
         const int cnt = c.cnt, hk = c.hk, token = c.token;
         for (int k = 0; k < cnt && ok; ++k, ++at) {
-          const int turn = at / stages, st = at - turn * stages;
-          const Rows a = next;
-          if (k + 1 < cnt) next = locate(c, k + 1);
-          else if (f + 1 < F) { c = s_piece[f + 1]; next = locate(c, 0); }
-          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, a.there))) * box * 128 * NP;
-          if (turn > 0 && !(ok = wait(&empty[st], (turn & 1) ^ 1, is_k ? 50 : 52))) break;
+          const int st = at & 1, in_batch = k & (batch - 1);
+          if (in_batch == 0) {
+            cur = next;
+            if (k + batch < cnt) next = locate(c, k + batch);
+            else if (f + 1 < F) { c = s_piece[f + 1]; next = locate(c, 0); }
+          }
+          const int src = (in_batch << log_boxes) + (lane & ((1 << log_boxes) - 1));
+          const int page_ = __shfl_sync(0xffffffffu, cur.page, src), row = __shfl_sync(0xffffffffu, cur.row, src);
+          const bool there = lane < (1 << log_boxes) && row >= 0;
+          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, there))) * box * 128 * NP;
           if (is_k && k == 0) {
-            if (fg + f >= 1 && !(ok = wait(&q_empty, (fg + f - 1) & 1, 51))) break;
+            const int qs = (fg + f) & 1, turn = (fg + f) >> 1;
+            if (turn > 0 && !(ok = wait(&q_empty[qs], (turn & 1) ^ 1, 51))) break;
             if (lane == 0) {
-              tc5::mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(p.G) * tpt * 128 * NP);
-              for (int h = 0; h < NP; ++h) tc5::tma_load_4d(q_s + h * PANEL, &map_q, &q_full, 0, hk * p.G, token, h);
+              tc5::mbar_arrive_expect_tx(&q_full[qs], static_cast<uint32_t>(p.G) * tpt * 128 * NP);
+              for (int h = 0; h < NP; ++h) tc5::tma_load_4d(q_s + qs * TILE + h * PANEL, &map_q, &q_full[qs], 0, hk * p.G, token, h);
             }
             ++q_at;
           }
+          if (at >= 2 && !(ok = wait(&empty[st], ((at >> 1) & 1) ^ 1, is_k ? 50 : 52))) break;
           if (lane == 0) tc5::mbar_arrive_expect_tx(&full[st], bytes);
           __syncwarp();
-          if (a.there) {
-            const int page = a.page < 0 || a.page >= p.num_pages ? static_cast<int>(p.num_pages) : a.page;   // outside the tensor: zeros
-            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(tiles + st * TILE + h * PANEL, map, &full[st], 0, a.row, h, hk, page);
+          if (there) {
+            const int page = page_ < 0 || page_ >= p.num_pages ? static_cast<int>(p.num_pages) : page_;   // outside the tensor: zeros
+            for (int h = 0; h < NP; ++h) tc5::tma_load_5d(tiles + st * TILE + h * PANEL, map, &full[st], 0, row, h, hk, page);
           }
           kv_at = at + 1;
         }
       }
       // on a failure elsewhere the copies in flight must land before the block leaves
       if (*reinterpret_cast<volatile int*>(&failed)) {
-        if (is_k && q_at > 0) tc5::mbar_wait(&q_full, (q_at - 1) & 1, 1u << 16);
-        for (int i = kv_at > stages ? kv_at - stages : 0; i < kv_at; ++i) tc5::mbar_wait(&full[i % stages], (i / stages) & 1, 1u << 16);
+        for (int i = q_at > 2 ? q_at - 2 : 0; is_k && i < q_at; ++i) tc5::mbar_wait(&q_full[i & 1], (i >> 1) & 1, 1u << 16);
+        for (int i = kv_at > 2 ? kv_at - 2 : 0; i < kv_at; ++i) tc5::mbar_wait(&full[i & 1], (i >> 1) & 1, 1u << 16);
       }
     } else if (warp == 8) {
       if (lane == 0) {   // ---- MMA issuer ----
         constexpr uint32_t idesc_s = tc5::umma_idesc(128, BKV, Fmt<T>::value);
         constexpr uint32_t idesc_o = tc5::umma_idesc(128, D, Fmt<T>::value) | (1u << 16);   // B operand MN-major
-        const uint32_t q_lo = tc5::desc_sw128_lo(tc5::smem_addr(q_s));
+        const uint32_t q_first = tc5::desc_sw128_lo(tc5::smem_addr(q_s));
         bool ok = true;
         // scores run up to two tiles ahead of the products with V: (sf, sk) is the next tile whose scores are to be issued
         int sf = 0, sk = 0, sn = n;
         auto issue_s = [&](bool look) {   // look: the K tile has not been looked for by the softmax threads
-          const int st = sn & 1, turn = sn / KST, ks = sn - turn * KST;
-          if (sk == 0 && !tc5::mbar_wait(&q_full, (fg + sf) & 1)) return false;
-          if (look && !tc5::mbar_wait(&k_full[ks], turn & 1)) return false;
+          const int st = sn & 1, qs = (fg + sf) & 1;
+          if (sk == 0 && !tc5::mbar_wait(&q_full[qs], ((fg + sf) >> 1) & 1)) return false;
+          if (look && !tc5::mbar_wait(&k_full[st], (sn >> 1) & 1)) return false;
           tc5::tc_fence_after();
-          const uint32_t k_lo = tc5::desc_sw128_lo(tc5::smem_addr(k_s + ks * TILE));
+          const uint32_t k_lo = tc5::desc_sw128_lo(tc5::smem_addr(k_s + st * TILE)), q_lo = q_first + qs * (TILE >> 4);
 #pragma unroll
           for (int h = 0; h < NP; ++h) tc5::umma_f16_kblock(tmem_base + 128 * st, q_lo + h * (PANEL >> 4), k_lo + h * (PANEL >> 4), idesc_s, h > 0);
           tc5::umma_commit(&s_full[st]);
-          tc5::umma_commit(&k_empty[ks]);
           if (++sk == s_piece[sf].cnt) {
-            tc5::umma_commit(&q_empty);
+            tc5::umma_commit(&q_empty[qs]);
             ++sf;
             sk = 0;
           }
@@ -227,10 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               tc5::umma_f16_ta(tmem_base + 256 + 128 * (e >> 2), tmem_base + 128 * st + 64 * (e >> 2) + 8 * (e & 3), db, idesc_o, k > 0 || (e & 3) != 0);
             }
             tc5::umma_commit(&o_full[st]);
-            tc5::umma_commit(&v_empty[st]);
-            // (The queries of the next item are on their way once the last scores of this one are done: as long as there are scores for the
-            // softmax threads, its first tile waits until after the next product.)
-            while (ok && sf < F && sn <= at + 2 && !(sk == 0 && sn == at + 2 && !tc5::mbar_try_wait(&q_full, (fg + sf) & 1))) ok = issue_s(false);
+            if (sf < F) ok = issue_s(false);
           }
         }
         if (!ok && !*reinterpret_cast<volatile int*>(&failed)) { failed = 1; atomicExch(&g_attn_paged_error, 53); }
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc5::tc_fence_before();     // this thread's tcgen05.ld / st are complete before its probabilities are read, S and O touched again
           // what the products of this tile and the scores of the one after next read has landed: looked for by one warp per group
           if (quarter == 0) {
-            if (g == 0 ? !wait_all(&v_full[st], (at >> 1) & 1, 57) : left > 2 && !wait_all(&k_full[(at + 2) % KST], ((at + 2) / KST) & 1, 58)) { alive = false; break; }
+            if (g == 0 ? !wait_all(&v_full[st], (at >> 1) & 1, 57) : left > 2 && !wait_all(&k_full[st], ((at + 2) >> 1) & 1, 58)) { alive = false; break; }
           }
           mbar_arrive1(&p_ready[st]);
         }
@@ -483,8 +483,8 @@ template <typename T, int D> int launch(const PagedParams& p, int dtype, cudaStr
     *configured = true;
   }
   const int tpt = 128 / p.G;
-  int box = 16;
-  while (box < 128 && p.page_size % (2 * box) == 0) box *= 2;
+  int log_box = 4;
+  while (log_box < 7 && p.page_size % (2 << log_box) == 0) ++log_box;
   CUtensorMap mq, mk, mv;
   auto bytes = [](int64_t elems) { return elems > 0 ? static_cast<uint64_t>(elems) * 2 : static_cast<uint64_t>(D) * 2; };   // (0: an axis of length one)
   {
@@ -496,10 +496,10 @@ template <typename T, int D> int launch(const PagedParams& p, int dtype, cudaStr
   for (int i = 0; i < 2; ++i) {
     const uint64_t dims[5] = {64, static_cast<uint64_t>(p.page_size), D / 64, static_cast<uint64_t>(p.Hkv), static_cast<uint64_t>(p.num_pages)};
     const uint64_t str[4] = {bytes(p.ks[2]), 128, bytes(p.ks[1]), bytes(p.ks[0])};
-    const uint32_t b[5] = {64, static_cast<uint32_t>(box), 1, 1, 1};
+    const uint32_t b[5] = {64, 1u << log_box, 1, 1, 1};
     if (!tma_encode_sw128(i ? &mv : &mk, dtype, 5, i ? p.v_pages : p.k_pages, dims, str, b)) return B200_ENOTSUP;
   }
-  return launch_pdl(attn_paged_tc5_kernel<T, D>, dim3(PAGED_CTAS), dim3(THREADS), smem_bytes(D), st, mq, mk, mv, p, tpt, box) == cudaSuccess ? B200_OK : B200_ELAUNCH;
+  return launch_pdl(attn_paged_tc5_kernel<T, D>, dim3(PAGED_CTAS), dim3(THREADS), smem_bytes(D), st, mq, mk, mv, p, tpt, log_box) == cudaSuccess ? B200_OK : B200_ELAUNCH;
 }
 
 }  // namespace
