@@ -433,7 +433,8 @@ int b200_attn_prefill_reads_tiles(const void* mask, int64_t S, int64_t mask_b, i
  *   q [n_tokens, Hq, D], k, v [n_tokens, Hkv, D]: views with element strides (token, head); Hq = 0: no queries;
  *   cos_t, sin_t [n_tokens, D] of the tokens' positions, in f32 or the activation type (table_dtype); both NULL: no rotation;
  *   q_out [n_tokens, Hq, D] dense (may be q itself where that is dense); slots[n] = page * page_size + row, a
- *   slot outside the pages writes nothing (padding; its query is rotated all the same).  Of equal slots any one may stay.
+ *   slot outside the pages writes nothing (padding; its query is rotated all the same).  Slots that are not negative are to
+ *   differ: a row that two tokens are written to ends up with parts of both.
  * y = x*cos + rotate_half(x)*sin in fp32, rounded once.  head_dim a multiple of 16. */
 typedef struct b200_paged_append_args {
   const void *q, *k, *v, *cos_t, *sin_t;
@@ -451,10 +452,13 @@ int b200_paged_append(const b200_paged_append_args* args, void* stream);
  *   page_table[b * table_stride + j / page_size].  Token i of T sees the keys up to its own position p = kv_len[b] - T + i, with
  *   window > 0 only the last `window` of them (p included).  A token without any key gives zeros.
  *   q: element strides (token, head); out [n_tokens, Hq, D]; rows behind the last sequence are left as they were.
- * head_dim 64 or 128, f16 / bf16, up to 128 query heads per KV head, page_size a multiple of 16.  Page ids outside the
- * cache read as zeros; table entries of pages without an attended key are not looked at, and what lies in pages behind
- * kv_len or ahead of the window does not matter, whatever it is.  Probabilities are rounded to the activation type for the second product.
- * workspace: 16-byte aligned, b200_attn_paged_workspace_bytes bytes of any content; calls that may overlap need one each. */
+ * head_dim 64 or 128, f16 / bf16, up to 128 query heads per KV head and 4096 sequences, page_size a multiple of 16.  Page
+ * ids outside the cache read as zeros; table entries of pages without an attended key are not looked at, and what lies in pages
+ * behind kv_len or ahead of the window does not matter, whatever it is (keys and values that some token of the chunk does see
+ * have to be finite: other tokens of its tile give them the weight zero).  Lengths and starts are cut to the table and to n_tokens.
+ * Probabilities are rounded to the activation type for the second product; sums and accumulators are fp32.
+ * workspace: 16-byte aligned, b200_attn_paged_workspace_bytes bytes of any content; calls that may overlap need one each.
+ * The result depends on the arguments alone (pieces are joined in a fixed order, no atomics). */
 typedef struct b200_attn_paged_args {
   const void *q, *k_pages, *v_pages;
   void* out;

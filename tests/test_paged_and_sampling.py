@@ -644,3 +644,24 @@ def test_serving_steps_of_two_layers(native_lib):
     for s in list(seqs):
         cache.close(s)
     assert cache.free_pages == 40
+
+
+@pytest.mark.gpu
+def test_attention_without_the_tensor_core_kernels(native_lib):
+    """B200NN_DISABLE_TC5=1 takes another kernel for every shape; the switch is read once, so in a process of its own."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    tests = Path(__file__).resolve().parent
+    code = ("import sys; sys.path[:0] = [r'%s', r'%s']\n"
+            "import test_paged_and_sampling as t\n"
+            "from paged_attention import paged_attention\n"
+            "for name in ('empty_and_short', 'decode_d64', 'decode_window', 'draft_4', 'chunk_window', 'chunk_odd'):\n"
+            "    case = t.CASES[name]\n"
+            "    a, start, table = t.build(**case)\n"
+            "    t.check_attention(paged_attention(**a, window=case.get('window', 0)), a, start, table, case['seqs'], case.get('window', 0))\n"
+            "print('done')\n") % (tests, tests.parent / "pytorch-apple_b200")
+    res = subprocess.run([sys.executable, "-c", code], env={**os.environ, "B200NN_DISABLE_TC5": "1"}, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "done" in res.stdout, res.stderr[-2000:]
