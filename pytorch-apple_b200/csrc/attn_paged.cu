@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 // ===========================================================================
 template <typename T, int D, int ROWS, int RPB>
 __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = 4;
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = RPB == 1 ? 10 : 4;   // pieces that a thread has on their way
   __shared__ __align__(16) float s_acc[GROUPS][D];
   __shared__ float s_m[GROUPS], s_l[GROUPS];
   pdl_trigger();
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
   const int4 it = __ldg(p.head + blockIdx.x);
   const int g = threadIdx.x / LPR, d = threadIdx.x % LPR * 4, r0 = blockIdx.y * RPB;
   if (it.x == 0 || r0 >= it.w) return;
-  const bool many = RPB == 1 || it.x > 2 * BATCH;
+  const bool many = RPB == 1 || it.x > 8;
   const int step = many ? GROUPS : 1;
   for (int r = many ? r0 : r0 + g; r < min(it.w, r0 + RPB); r += many ? 1 : GROUPS) {   // (uniform where the block meets)
     float m = -INFINITY, l = 0.f;

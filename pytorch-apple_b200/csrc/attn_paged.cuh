@@ -171,10 +171,14 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
       if (e < items) t = paged_tile<KT>(p, T, n, e - h * tiles, tpt);
       const int64_t cost = e < items ? t.cnt + OV : 0;
       int64_t upto = cost;
+      if (tiles == 1) {   // (all items of a decoding sequence cost the same)
+        upto = static_cast<int64_t>(min(lane + 1, items - e0)) * __shfl_sync(0xffffffffu, t.cnt + OV, 0);
+      } else {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
       }
       const int64_t start = base + upto - cost + OV, end = base + upto;
       const bool here = start >= u0 && start < u1;

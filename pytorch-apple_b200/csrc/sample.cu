@@ -5,13 +5,13 @@
 // first always), min-p what weighs at least min_p.  The token drawn is the first one, by index, at which the running sum of what is kept
 // passes u times the whole sum.
 //
-// Weights are whole numbers in units of 2^-40 (their sums over a row stay below 2^62), good to about 2^-31 of the largest: integer sums
-// do not depend on the order of the additions, so the same row gives the same token however it is dealt to blocks, and a sum over
-// 150 000 tokens is as exact as its terms (in fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a
-// rare token is wide).  Thresholds are found on the logits themselves, never on weights.
+// Weights are whole numbers in units of 2^-40 (their sums over a row stay below 2^62): integer sums do not depend on the order of the additions,
+// so the same row gives the same token however it is dealt to blocks, and a sum over 150 000 tokens is as exact as its terms (in
+// fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a rare token is wide).  Thresholds are found on the logits
+// themselves, never on weights.
 //
 // A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once (a bulk copy per warp)
-// and then goes through a few times: for the maximum; for the sum of the weights where it is needed (about 15 instructions a token: that, and not the memory, is
+// and then goes through a few times: for the maximum; for the sum of the weights where it is needed (about 20 instructions a token: that, and not the memory, is
 // what most of the time goes into); for the tokens that are large enough to matter. How large that is the maxima of the threads' own
 // tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are sorted by one CTA, which mostly finds everything
 // that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or weights in 16 intervals of z, then in 16 parts
@@ -58,74 +58,62 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  The difference and its product with log2(e) / T are carried as pairs of fp32 numbers: a rounding
-// of t = 30 alone would be 2^-20 of the weight.  Below t = 17 by the table method (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a
-// table for the first eight, a cubic for the rest (its next term is below 2^-38).  From there on, where most tokens lie, a weight is below 2^23 units and
-// the fast exponential of t's distance from a whole number (2^-22 of itself) is as good; no conversions there, which share its unit.
+// exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  log2(e) / T is carried as a pair of fp32 numbers, and the difference where it need not be whole:
+// a rounding of t = 30 alone would be 2^-20 of the weight.  The fast exponential of t's distance from the nearest whole number is good to 2^-22
+// of itself. Those errors are as good as independent, so the sum before the i-th of n like tokens is off by sqrt(i) 2^-22 weights, and u falls
+// between the sum and the true one somewhere in the row once in 2^22 / sqrt(n) draws (16000 rows of 150 000 tokens; a table method good to 2^-31 took
+// five times as long where many tokens matter).  No conversions: they share their unit with the exponential.
 template <typename T> struct Weigher {
   float m, c_hi, c_lo;
-  float end, near;         // differences at which t is 41 (half a unit: no weight) and 17
-  const uint32_t* table;   // 2^31 2^-(i / 256)
-  __device__ __forceinline__ float rest(float z, float dh) const {   // (m - z) - dh
-    const float bv = m - dh;
-    return (m - (dh + bv)) + (bv - z);
-  }
+  float end;               // difference at which t is 41 (half a unit: no weight)
   // m - z, not above `end`: for NaN as well
   __device__ __forceinline__ float difference(float z) const { return fminf(m - z, end); }
-  // weight + 0x4b000000, for differences (of z, or `end`) of at least `near`
-  __device__ __forceinline__ uint32_t small(float z, float dh) const {
+  // weight = (hi - 0x4b000000) 2^20 + lo - 0x4b000000, both whole numbers below 2^21, for a difference of z or `end`
+  __device__ __forceinline__ void parts(float z, float dh, uint32_t& hi, uint32_t& lo) const {
     const float shifted = fmaf(dh, c_hi, 12582912.f);      // + 1.5 2^23: t to the nearest whole number
     float x = fmaf(dh, c_lo, fmaf(dh, c_hi, -(shifted - 12582912.f)));
-    if constexpr (sizeof(T) == 4) x = dh < end ? fmaf(rest(z, dh), c_hi, x) : x;   // (differences of 16-bit logits are whole but for those next to zero)
+    if constexpr (sizeof(T) == 4) {   // (differences of 16-bit logits are whole but for those next to zero)
+      const float bv = m - dh;
+      x = dh < end ? fmaf((m - (dh + bv)) + (bv - z), c_hi, x) : x;
+    }
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-x));
-    return __float_as_uint(__fadd_rz(y * __uint_as_float((167u << 23) - (__float_as_uint(shifted) << 23)), 8388608.f));   // 2^(40 - whole), cut to a whole number
+    y *= __uint_as_float((147u << 23) - (__float_as_uint(shifted) << 23));   // 2^(20 - whole): the weight in units of 2^-20
+    const float h = __fadd_rz(y, 8388608.f);
+    hi = __float_as_uint(h);
+    lo = __float_as_uint(__fadd_rz((y - (h - 8388608.f)) * 1048576.f, 8388608.f));
   }
-  __device__ __forceinline__ u64 large(float z) const {   // (ONE for z == m)
-    const float dh = m - z, p = __fmul_rn(dh, c_hi);
-    const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, rest(z, dh) * c_hi);
-    const float ip = floorf(p);
-    int64_t t = (static_cast<int64_t>(ip) << 32) + static_cast<int64_t>(__float2uint_rz((p - ip) * 4294967296.f)) + static_cast<int64_t>(__float2int_rn(e * 4294967296.f));
-    t = t < 0 ? 0 : t;
-    const uint32_t f = static_cast<uint32_t>(t);
-    const float a = static_cast<float>(f & 0xffffffu) * (0.6931471805599453f / 4294967296.f);
-    const float q = a - a * a * (0.5f - a * (1.f / 6.f));   // 1 - 2^-r
-    const uint32_t tab = table[f >> 24];
-    const uint32_t w = tab - static_cast<uint32_t>((static_cast<u64>(tab) * __float2uint_rn(q * 4294967296.f) + 0x80000000ull) >> 32);
-    return (static_cast<u64>(w) << 9) >> static_cast<int>(t >> 32);
+  __device__ __forceinline__ u64 operator()(float z) const { return at(z, difference(z)); }
+  __device__ __forceinline__ u64 at(float z, float dh) const {
+    uint32_t hi, lo;
+    parts(z, dh, hi, lo);
+    return (static_cast<u64>(hi - 0x4b000000u) << 20) + (lo - 0x4b000000u);
   }
-  __device__ __forceinline__ u64 operator()(float z) const {
-    const float dh = difference(z);
-    return dh < near ? large(z) : small(z, dh) - 0x4b000000u;
-  }
-  // Sum of the weights of those of eight tokens that keep(token, column) lets through: straight through for the ones that are far from the maximum
-  // (FAR; else they are left out), then the few near ones with at least `least` one by one (a warp goes round as often as its lane with most of them has some).
-  template <bool FAR, typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, u64 least, K&& keep) const {
-    uint32_t s = 0, close = 0;
+  // (of those that weigh at least `least`: see sum)
+  template <typename K> __device__ __forceinline__ u64 sum_from(const float (&z)[8], int c, u64 least, K&& keep) const {
+    u64 t = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float dh = difference(z[k]);
-      close |= (dh < near ? 1u : 0u) << k;
-      if (FAR) s += small(z[k], dh < near || !keep(z[k], c + k) ? end : dh);
-    }
-    u64 t = FAR ? s - 8u * 0x4b000000u : 0u;
-    while (close) {
-      const int at = __ffs(close) - 1;
-      close &= close - 1;
-      float v = z[0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k) v = at == k ? z[k] : v;
-      if (keep(v, c + at)) {
-        const u64 w = large(v);
-        t += w >= least ? w : 0;
-      }
+      const u64 w = at(z[k], keep(z[k], c + k) ? difference(z[k]) : end);
+      t += w >= least ? w : 0;
     }
     return t;
+  }
+  // Sum of the weights of those of eight tokens that keep(token, column) lets through
+  template <typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, K&& keep) const {
+    uint32_t hi = 0, lo = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t h, l;
+      parts(z[k], keep(z[k], c + k) ? difference(z[k]) : end, h, l);
+      hi += h;
+      lo += l;
+    }
+    return (static_cast<u64>(hi - 8u * 0x4b000000u) << 20) + (lo - 8u * 0x4b000000u);
   }
 };
 
 struct Shared {
-  uint32_t table[256];
   u64 part[SW];
   u64 told[2][MAX_CTAS];   // values of all CTAs of the row, two exchanges deep
   u64 bin_mass[SW][BINS], told_mass[2][MAX_CTAS][BINS];
@@ -365,11 +353,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
                    ::"r"(tc5::smem_addr(row.copy)), "l"(x + row.begin), "r"(bytes), "r"(tc5::smem_addr(&sh.full[warp])) : "memory");
     }
   }
-  if (threadIdx.x < 256) sh.table[threadIdx.x] = static_cast<uint32_t>(exp2(-static_cast<double>(threadIdx.x) / 256.) * 2147483648. + 0.5);
   const float T_ = p.temperature ? __ldg(p.temperature + r) : 1.f, tp = p.top_p ? __ldg(p.top_p + r) : 1.f, mp = p.min_p ? __ldg(p.min_p + r) : 0.f;
   const int k = p.top_k ? __ldg(p.top_k + r) : 0;
   const float uniform = __ldg(p.uniform + r);
-  if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer; the table is there
+  if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer
   if (row.copied > row.begin && !tc5::mbar_wait(&sh.full[warp], 0) && lane == 0) atomicExch(&g_sample_error, 70);
 
   // ---- the maximum ----
@@ -401,8 +388,6 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   weight.c_hi = static_cast<float>(c_);
   weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
   weight.end = static_cast<float>(41. / c_);
-  weight.near = static_cast<float>(17. / c_);
-  weight.table = sh.table;
   const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;
   auto target_of = [&](u64 total) -> u64 {
     const double d = static_cast<double>(uniform) * static_cast<double>(total);
@@ -431,15 +416,16 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const bool restricted_by_k = k > 0 && k < p.cols;
   auto collect = [&](uint32_t lo, uint32_t hi) {   // tokens with places in [lo, hi], to CTA 0: into a list of each CTA's own, then in one piece
     // (a bound on the logits with some room: places are looked at only behind it)
+    const float above = lo == 0 ? INFINITY : weight.m - (static_cast<float>(lo) - 8.f) * (0.9999f / 131072.f) / weight.c_hi + fabsf(weight.m) * 5e-7f;
     const float bound = weight.m - fminf((static_cast<float>(hi) + 8.f) * (1.0001f / 131072.f) / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f;
 #pragma unroll 2
     for (int c = row.begin + lane * 8; c < row.end; c += 256) {
-      if (row.top(c) >= bound) {
+      if (lo > 0 || row.top(c) >= bound) {
         float z[8];
         uint32_t some = 0;
         row.load(c, z);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) some |= (z[k] >= bound ? 1u : 0u) << k;
+        for (int k = 0; k < 8; ++k) some |= (z[k] >= bound && z[k] <= above ? 1u : 0u) << k;
         while (some) {
           const int k = __ffs(some) - 1;
           some &= some - 1;
@@ -490,15 +476,17 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       u64* const own = bins + warp * BINS * 32 + lane;
 #pragma unroll
       for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
-      row.each([&](float z, int i) {
-        const float dh = weight.difference(z);
-        if (dh < weight.end) {
-          const uint32_t X = place(dh);
-          if (X >= first && X <= end) {
-            u64 add = 1ull << 52;   // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1)
-            if (by_mass) add = !restricted_by_k || stays(z, i) ? add + weight(z) : 0;
-            own[((X - first) >> shift) * 32] += add;
-          }
+      // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1: 12 bits count, 52 add up)
+      row.packs([&](const float (&z)[8], int c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float dh = weight.difference(z[e]);
+          const uint32_t X = place(dh) - first;
+          bool in = dh < weight.end && X <= end - first;
+          if (by_mass && restricted_by_k) in = in && stays(z[e], c + e);
+          u64 add = 1ull << 52;
+          if (by_mass) add += weight.at(z[e], dh);
+          if (in) own[(X >> shift) * 32] += add;
         }
       });
       __syncwarp();
@@ -713,11 +701,11 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   };
 
   // ---- the short way: the largest tokens, as many as k or as a nucleus mostly has ----
-  const bool few_k = restricted_by_k && 2 * k <= threads;
+  const bool few_k = restricted_by_k && 2 * k <= threads && k <= CAP / 2;
   if (few_k || (tp < 1.f && !restricted_by_k)) {
     if (!few_k) {
       u64 s = 0;
-      row.packs([&](const float (&z)[8], int c) { s += weight.template sum<true>(z, c, 0, [](float, int) { return true; }); });
+      row.packs([&](const float (&z)[8], int c) { s += weight.sum(z, c, [](float, int) { return true; }); });
       whole = row_reduce<false>(s, sh, ctas, turn);
     }
     const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 96u);
@@ -775,16 +763,12 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     return w >= least ? w : 0;
   };
   u64 mine = 0;
-  if (cut == 0 && least == 0) {
-    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, 0, [](float, int) { return true; }); });
-  } else if (least == 0) {
-    const float at_cut = value_of(cut);
-    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, 0, [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); }); });
-  } else if (least > 1ull << 23) {
-    row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<false>(z, c, least, stays); });
-  } else {
-    row.each([&](float z, int i) { mine += kept(z, i); });
-  }
+  const float at_cut = value_of(cut);
+  const auto all = [](float, int) { return true; };
+  const auto some = [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); };
+  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.sum(z, c, all); });
+  else if (cut == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.sum_from(z, c, least, all); });
+  else row.packs([&](const float (&z)[8], int c) { mine += weight.sum_from(z, c, least, some); });
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
