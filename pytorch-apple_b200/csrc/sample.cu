@@ -59,23 +59,28 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 
 // exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  log2(e) / T is carried as a pair of fp32 numbers, and the difference where it need not be whole:
-// a rounding of t = 30 alone would be 2^-20 of the weight.  The fast exponential of t's distance from the nearest whole number is good to 2^-22
-// of itself. Those errors are as good as independent, so the sum before the i-th of n like tokens is off by sqrt(i) 2^-22 weights, and u falls
-// between the sum and the true one somewhere in the row once in 2^22 / sqrt(n) draws (16000 rows of 150 000 tokens; a table method good to 2^-31 took
-// five times as long where many tokens matter).  No conversions: they share their unit with the exponential.
+// a rounding of t = 30 alone would be 2^-20 of the weight.  Two ways:
+// - the few tokens that the row's sum mostly consists of (t below 12, less at temperatures above 1, where the sum spreads over more) by the table method
+//   (P. T. P. Tang, 1989): t to 32 binary places, 2^-(i / 256) from a table for the first eight, a cubic for the rest (its next term is below 2^-38).  The
+//   sum at every later boundary moves with their errors, and most of 150 000 tokens are less than 2^-22 of it wide: with the other way for them too,
+//   one draw in a hundred from a row without filters would give a neighbour of the right token; so it is one in 30 000.
+// - all others by the fast exponential of t's distance from the nearest whole number, good to 2^-22 of itself: errors of many small weights, as good as
+//   independent.  Straight through and without conversions (they share their unit with the exponential).
 template <typename T> struct Weigher {
   float m, c_hi, c_lo;
-  float end;               // difference at which t is 41 (half a unit: no weight)
+  float end, near;         // differences at which t is 41 (half a unit: no weight), and below which the table is used
+  const uint32_t* table;   // 2^31 2^-(i / 256)
   // m - z, not above `end`: for NaN as well
   __device__ __forceinline__ float difference(float z) const { return fminf(m - z, end); }
+  __device__ __forceinline__ float rest(float z, float dh) const {   // (m - z) - dh
+    const float bv = m - dh;
+    return (m - (dh + bv)) + (bv - z);
+  }
   // weight = (hi - 0x4b000000) 2^20 + lo - 0x4b000000, both whole numbers below 2^21, for a difference of z or `end`
   __device__ __forceinline__ void parts(float z, float dh, uint32_t& hi, uint32_t& lo) const {
     const float shifted = fmaf(dh, c_hi, 12582912.f);      // + 1.5 2^23: t to the nearest whole number
     float x = fmaf(dh, c_lo, fmaf(dh, c_hi, -(shifted - 12582912.f)));
-    if constexpr (sizeof(T) == 4) {   // (differences of 16-bit logits are whole but for those next to zero)
-      const float bv = m - dh;
-      x = dh < end ? fmaf((m - (dh + bv)) + (bv - z), c_hi, x) : x;
-    }
+    if constexpr (sizeof(T) == 4) x = dh < end ? fmaf(rest(z, dh), c_hi, x) : x;   // (differences of 16-bit logits are whole but for those next to zero)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-x));
     y *= __uint_as_float((147u << 23) - (__float_as_uint(shifted) << 23));   // 2^(20 - whole): the weight in units of 2^-20
@@ -83,37 +88,70 @@ template <typename T> struct Weigher {
     hi = __float_as_uint(h);
     lo = __float_as_uint(__fadd_rz((y - (h - 8388608.f)) * 1048576.f, 8388608.f));
   }
-  __device__ __forceinline__ u64 operator()(float z) const { return at(z, difference(z)); }
-  __device__ __forceinline__ u64 at(float z, float dh) const {
+  __device__ __forceinline__ u64 other(float z, float dh) const {
     uint32_t hi, lo;
     parts(z, dh, hi, lo);
     return (static_cast<u64>(hi - 0x4b000000u) << 20) + (lo - 0x4b000000u);
   }
-  // (of those that weigh at least `least`: see sum)
-  template <typename K> __device__ __forceinline__ u64 sum_from(const float (&z)[8], int c, u64 least, K&& keep) const {
+  __device__ __forceinline__ u64 large(float z) const {   // (ONE for z == m)
+    const float dh = m - z, p = __fmul_rn(dh, c_hi);
+    const float e = fmaf(dh, c_hi, -p) + fmaf(dh, c_lo, rest(z, dh) * c_hi);
+    const float ip = floorf(p);
+    int64_t t = (static_cast<int64_t>(ip) << 32) + static_cast<int64_t>(__float2uint_rz((p - ip) * 4294967296.f)) + static_cast<int64_t>(__float2int_rn(e * 4294967296.f));
+    t = t < 0 ? 0 : t;
+    const uint32_t f = static_cast<uint32_t>(t);
+    const float a = static_cast<float>(f & 0xffffffu) * (0.6931471805599453f / 4294967296.f);
+    const float q = a - a * a * (0.5f - a * (1.f / 6.f));   // 1 - 2^-r
+    const uint32_t tab = table[f >> 24];
+    const uint32_t w = tab - static_cast<uint32_t>((static_cast<u64>(tab) * __float2uint_rn(q * 4294967296.f) + 0x80000000ull) >> 32);
+    return (static_cast<u64>(w) << 9) >> static_cast<int>(t >> 32);
+  }
+  __device__ __forceinline__ u64 operator()(float z) const {
+    const float dh = difference(z);
+    return dh < near ? large(z) : other(z, dh);
+  }
+  // f(token, its place among the eight) for those whose bit is set, a token of each lane at a time (a warp goes round as often as its lane with most of them has some)
+  template <typename F> static __device__ __forceinline__ void each_set(uint32_t set, const float (&z)[8], F&& f) {
+    while (set) {
+      const int at = __ffs(set) - 1;
+      set &= set - 1;
+      float v = z[0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) v = at == k ? z[k] : v;
+      f(v, at);
+    }
+  }
+  // Sum of the weights, of at least `least`, of those of eight tokens that keep(token, column) lets through (FROM: there is a least weight)
+  template <bool FROM, typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, u64 least, K&& keep) const {
+    uint32_t hi = 0, lo = 0, close = 0;
     u64 t = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const u64 w = at(z[k], keep(z[k], c + k) ? difference(z[k]) : end);
-      t += w >= least ? w : 0;
+      const float dh = difference(z[k]);
+      const bool kept = keep(z[k], c + k);
+      close |= (kept && dh < near ? 1u : 0u) << k;
+      const float d = kept && dh >= near ? dh : end;
+      if (FROM) {
+        const u64 w = other(z[k], d);
+        t += w >= least ? w : 0;
+      } else {
+        uint32_t h, l;
+        parts(z[k], d, h, l);
+        hi += h;
+        lo += l;
+      }
     }
+    if (!FROM) t = (static_cast<u64>(hi - 8u * 0x4b000000u) << 20) + (lo - 8u * 0x4b000000u);
+    each_set(close, z, [&](float v, int) {
+      const u64 w = large(v);
+      t += !FROM || w >= least ? w : 0;
+    });
     return t;
-  }
-  // Sum of the weights of those of eight tokens that keep(token, column) lets through
-  template <typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, K&& keep) const {
-    uint32_t hi = 0, lo = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t h, l;
-      parts(z[k], keep(z[k], c + k) ? difference(z[k]) : end, h, l);
-      hi += h;
-      lo += l;
-    }
-    return (static_cast<u64>(hi - 8u * 0x4b000000u) << 20) + (lo - 8u * 0x4b000000u);
   }
 };
 
 struct Shared {
+  uint32_t table[256];
   u64 part[SW];
   u64 told[2][MAX_CTAS];   // values of all CTAs of the row, two exchanges deep
   u64 bin_mass[SW][BINS], told_mass[2][MAX_CTAS][BINS];
@@ -353,10 +391,11 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
                    ::"r"(tc5::smem_addr(row.copy)), "l"(x + row.begin), "r"(bytes), "r"(tc5::smem_addr(&sh.full[warp])) : "memory");
     }
   }
+  if (threadIdx.x < 256) sh.table[threadIdx.x] = static_cast<uint32_t>(exp2(-static_cast<double>(threadIdx.x) / 256.) * 2147483648. + 0.5);
   const float T_ = p.temperature ? __ldg(p.temperature + r) : 1.f, tp = p.top_p ? __ldg(p.top_p + r) : 1.f, mp = p.min_p ? __ldg(p.min_p + r) : 0.f;
   const int k = p.top_k ? __ldg(p.top_k + r) : 0;
   const float uniform = __ldg(p.uniform + r);
-  if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer
+  if (ctas > 1) tc5::cluster_sync(); else __syncthreads();   // every CTA of the row runs before anyone writes into a peer; the table is there
   if (row.copied > row.begin && !tc5::mbar_wait(&sh.full[warp], 0) && lane == 0) atomicExch(&g_sample_error, 70);
 
   // ---- the maximum ----
@@ -388,6 +427,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   weight.c_hi = static_cast<float>(c_);
   weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
   weight.end = static_cast<float>(41. / c_);
+  weight.near = static_cast<float>(12. / c_) / fmaxf(T_, 1.f);
+  weight.table = sh.table;
   const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;
   auto target_of = [&](u64 total) -> u64 {
     const double d = static_cast<double>(uniform) * static_cast<double>(total);
@@ -426,19 +467,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
         row.load(c, z);
 #pragma unroll
         for (int k = 0; k < 8; ++k) some |= (z[k] >= bound && z[k] <= above ? 1u : 0u) << k;
-        while (some) {
-          const int k = __ffs(some) - 1;
-          some &= some - 1;
-          float v = z[0];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) v = k == e ? z[e] : v;
+        weight.each_set(some, z, [&](float v, int k) {
           const float dh = weight.difference(v);
           const uint32_t X = place(dh);
           if (dh < weight.end && X <= hi && X >= lo && stays(v, c + k)) {
             const int at = atomicAdd(&sh.listed, 1);
             if (at < CAP) bins[at] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~(c + k));
           }
-        }
+        });
       }
     }
     if (ctas == 1) { __syncthreads(); return; }
@@ -478,6 +514,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
       // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1: 12 bits count, 52 add up)
       row.packs([&](const float (&z)[8], int c) {
+        uint32_t close = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float dh = weight.difference(z[e]);
@@ -485,9 +522,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
           bool in = dh < weight.end && X <= end - first;
           if (by_mass && restricted_by_k) in = in && stays(z[e], c + e);
           u64 add = 1ull << 52;
-          if (by_mass) add += weight.at(z[e], dh);
+          if (by_mass) {
+            close |= (in && dh < weight.near ? 1u : 0u) << e;
+            in = in && dh >= weight.near;
+            add += weight.other(z[e], dh);
+          }
           if (in) own[(X >> shift) * 32] += add;
         }
+        weight.each_set(close, z, [&](float v, int) { own[((place(weight.difference(v)) - first) >> shift) * 32] += (1ull << 52) + weight.large(v); });
       });
       __syncwarp();
       {
@@ -705,7 +747,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (few_k || (tp < 1.f && !restricted_by_k)) {
     if (!few_k) {
       u64 s = 0;
-      row.packs([&](const float (&z)[8], int c) { s += weight.sum(z, c, [](float, int) { return true; }); });
+      row.packs([&](const float (&z)[8], int c) { s += weight.template sum<false>(z, c, 0, [](float, int) { return true; }); });
       whole = row_reduce<false>(s, sh, ctas, turn);
     }
     const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 96u);
@@ -766,9 +808,9 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const float at_cut = value_of(cut);
   const auto all = [](float, int) { return true; };
   const auto some = [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); };
-  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.sum(z, c, all); });
-  else if (cut == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.sum_from(z, c, least, all); });
-  else row.packs([&](const float (&z)[8], int c) { mine += weight.sum_from(z, c, least, some); });
+  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<false>(z, c, 0, all); });
+  else if (cut == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, least, all); });
+  else row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, least, some); });
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);

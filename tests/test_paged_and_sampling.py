@@ -465,9 +465,10 @@ def check_draw(x, u, **settings):
     assert got == want, [(r, a, b) for r, (a, b) in enumerate(zip(got, want)) if a != b][:5]
 
 
-# A token differs from the 64-bit one only where u falls between a boundary and where the weights' errors (2^-22 of each at most, as good as independent)
-# have moved it: for n like tokens boundary i by sqrt(i) 2^-22 weights, 2/3 sqrt(n) 2^-22 of a token's width on average, 6e-5 a row for 151936 of them;
-# a row dominated by few tokens moves by 2^-22 of them.  Over the rows below less than one in a hundred runs; the seeds are fixed.
+# A token differs from the 64-bit one only where u falls between a boundary and where the weights' errors have moved it.  Tokens with t < 12 (temperature 1) are off
+# by 2^-31 of the row's maximum, the others by 2^-22 of themselves, as good as independent: behind the first ones every boundary has moved by some 2^-31 of the sum,
+# 151936 of them make 7e-5 of the draws from a row without filters; for n like tokens boundary i moves by sqrt(i) 2^-22 weights, 6e-5 of the draws.  Rows cut to a
+# list have a few hundred boundaries, 1e-6.  All rows below together: less than one run in ten; the seeds are fixed.
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("cols", [1, 2, 7, 100, 1000, 4097, 33000, 151936])
