@@ -477,8 +477,8 @@ int64_t b200_attn_paged_workspace_bytes(int64_t max_q, int Hq, int Hkv, int D);
  * [0, 1); NULL: temperature 1, filter off.  With w = exp((x - max) / temperature), tokens ordered by x, of equal ones the lower
  * index first: top-k keeps the first k; top-p of those the ones before which less than top_p of their sum lies (always the
  * first); min-p those with w >= min(min_p, 1).  out[r] = the first index at which the sum of what is kept, taken in the
- * order of the indices, passes uniform[r] times the whole.  Weights are whole multiples of 2^-40 (what weighs less is never
- * drawn), so the result depends on the row and its numbers alone; NaN counts as -infinity, a row of nothing else gives 0.
+ * order of the indices, passes uniform[r] times the whole.  Weights are whole multiples of 2^-40 (what weighs less than
+ * half of that is never drawn), so the result depends on the row and its numbers alone.  A row of nothing but -infinity, or with a NaN in it, gives 0.
  * At most 4194304 columns and 65535 rows. */
 int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, int64_t cols, int64_t row_stride, const float* temperature,
                      const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int dtype, void* stream);

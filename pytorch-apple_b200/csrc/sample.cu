@@ -51,9 +51,9 @@ struct SampleParams {
 // code left by a bounded wait that ran out
 __device__ int g_sample_error = 0;
 
-// Keys order like the logits they come from: equal keys, equal values (-0 counts as 0); NaN comes last, like -infinity.
+// Keys order like the logits they come from: equal keys, equal values (-0 counts as 0); NaN comes first.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0;
+  if (x != x) return 0xffffffffu;
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -68,15 +68,15 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 //   independent.  Straight through and without conversions (they share their unit with the exponential).
 template <typename T> struct Weigher {
   float m, c_hi, c_lo;
-  float end, near;         // differences at which t is 41 (half a unit: no weight), and below which the table is used
+  float end, near;         // differences at which t is 43 (an eighth of a unit: no weight), and below which the table is used
   const uint32_t* table;   // 2^31 2^-(i / 256)
-  // m - z, not above `end`: for NaN as well
+  // m - z, not above `end`
   __device__ __forceinline__ float difference(float z) const { return fminf(m - z, end); }
   __device__ __forceinline__ float rest(float z, float dh) const {   // (m - z) - dh
     const float bv = m - dh;
     return (m - (dh + bv)) + (bv - z);
   }
-  // weight = (hi - 0x4b000000) 2^20 + lo - 0x4b000000, both whole numbers below 2^21, for a difference of z or `end`
+  // weight = (hi - 0x4b000000) 2^20 + lo - 0x4b000000, both whole numbers up to 2^21, for a difference of z or `end`
   __device__ __forceinline__ void parts(float z, float dh, uint32_t& hi, uint32_t& lo) const {
     const float shifted = fmaf(dh, c_hi, 12582912.f);      // + 1.5 2^23: t to the nearest whole number
     float x = fmaf(dh, c_lo, fmaf(dh, c_hi, -(shifted - 12582912.f)));
@@ -86,7 +86,7 @@ template <typename T> struct Weigher {
     y *= __uint_as_float((147u << 23) - (__float_as_uint(shifted) << 23));   // 2^(20 - whole): the weight in units of 2^-20
     const float h = __fadd_rz(y, 8388608.f);
     hi = __float_as_uint(h);
-    lo = __float_as_uint(__fadd_rz((y - (h - 8388608.f)) * 1048576.f, 8388608.f));
+    lo = __float_as_uint(fmaf(y - (h - 8388608.f), 1048576.f, 8388608.f));   // (rounded: cut off, 150 000 small weights would lose 2^-24 of the sum)
   }
   __device__ __forceinline__ u64 other(float z, float dh) const {
     uint32_t hi, lo;
@@ -162,12 +162,18 @@ struct Shared {
   __align__(8) uint64_t full[SW];
 };
 
+// NaN where one of the two is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {   // of pairs of 16-bit numbers
   if constexpr (sizeof(T) == 4) {
     return a;
   } else {
     using P = typename Pair<T>::type;
-    const P r = __hmax2(reinterpret_cast<const P&>(a), reinterpret_cast<const P&>(b));
+    const P r = __hmax2_nan(reinterpret_cast<const P&>(a), reinterpret_cast<const P&>(b));
     return reinterpret_cast<const uint32_t&>(r);
   }
 }
@@ -179,7 +185,7 @@ template <typename T> struct Row {
   int begin, end, copied;    // columns begin .. copied - 1 are in the copy
   bool vec;
   bool infinite = false;     // the maximum is +infinity: as if it were 0 and all else -infinity
-  __device__ __forceinline__ void load(int c, float (&f)[8]) const {   // columns c .. c + 7; those past the end as NaN
+  __device__ __forceinline__ void load(int c, float (&f)[8]) const {   // columns c .. c + 7; those past the end as -infinity
     fetch(c, f);
     if (infinite)
 #pragma unroll
@@ -192,10 +198,10 @@ template <typename T> struct Row {
       unpack(x + c, f);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = c + k < end ? to_f32<T>(x[c + k]) : __uint_as_float(0x7fffffffu);
+      for (int k = 0; k < 8; ++k) f[k] = c + k < end ? to_f32<T>(x[c + k]) : -INFINITY;
     }
   }
-  // the largest of columns c .. c + 7 (NaN is none)
+  // the largest of columns c .. c + 7 (NaN where there is one)
   __device__ __forceinline__ float top(int c) const {
     if constexpr (sizeof(T) == 2) {
       if (!infinite && (c + 8 <= copied || (vec && c + 8 <= end))) {
@@ -203,12 +209,12 @@ template <typename T> struct Row {
         const uint32_t v = max2<T>(max2<T>(w.x, w.y), max2<T>(w.z, w.w));
         float a, b;
         unpack2<T>(v, a, b);
-        return fmaxf(a, b);
+        return max_nan(a, b);
       }
     }
     float z[8];
     load(c, z);
-    return fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+    return max_nan(max_nan(max_nan(z[0], z[1]), max_nan(z[2], z[3])), max_nan(max_nan(z[4], z[5]), max_nan(z[6], z[7])));
   }
   static __device__ __forceinline__ void unpack(const T* at, float (&f)[8]) {
     if constexpr (sizeof(T) == 2) {
@@ -399,20 +405,21 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (row.copied > row.begin && !tc5::mbar_wait(&sh.full[warp], 0) && lane == 0) atomicExch(&g_sample_error, 70);
 
   // ---- the maximum ----
-  float top = -INFINITY;   // of this thread's tokens (NaN is none)
+  float top = -INFINITY;   // of this thread's tokens
 #pragma unroll 4
-  for (int c = row.begin + lane * 8; c < row.end; c += 256) top = fmaxf(top, row.top(c));
+  for (int c = row.begin + lane * 8; c < row.end; c += 256) top = max_nan(top, row.top(c));
   const u64 best = row_reduce<true>(key_of(top), sh, ctas, turn);
   float m = value_of(static_cast<uint32_t>(best));
-  if (!(T_ > 0.f) || m == -INFINITY) {   // greedy: the first of the largest; a row without any weight gives its first token
+  const bool none = !(m > -INFINITY);     // a row without any weight, or with a NaN: there is nothing to draw from
+  if (!(T_ > 0.f) || none) {              // greedy: the first of the largest
     u64 at = 0;
-    if (m > -INFINITY) {
+    if (!none) {
       row.each([&](float z, int c) {
         if (z == m && at == 0) at = static_cast<uint32_t>(~c);
       });
       at = row_reduce<true>(at, sh, ctas, turn);
     }
-    if (rank == 0 && threadIdx.x == 0) p.out[r] = m > -INFINITY ? static_cast<int>(~static_cast<uint32_t>(at)) : 0;
+    if (rank == 0 && threadIdx.x == 0) p.out[r] = none ? 0 : static_cast<int>(~static_cast<uint32_t>(at));
     return;
   }
   if (m == INFINITY) {
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   weight.m = m;
   weight.c_hi = static_cast<float>(c_);
   weight.c_lo = static_cast<float>(c_ - static_cast<double>(weight.c_hi));
-  weight.end = static_cast<float>(41. / c_);
+  weight.end = static_cast<float>(43. / c_);
   weight.near = static_cast<float>(12. / c_) / fmaxf(T_, 1.f);
   weight.table = sh.table;
   const u64 least = mp > 0.f ? static_cast<u64>(ceil(static_cast<double>(fminf(mp, 1.f)) * static_cast<double>(ONE))) : 0;

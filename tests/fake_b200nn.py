@@ -180,7 +180,7 @@ class FakeLibrary:
     def b200_sample_rows(self, logits, out, rows, cols, row_stride, temperature, top_k, top_p, min_p, uniform, dtype, stream):
         self.calls.append("sample_rows")
         X = _raw(logits, _DT[dtype], [rows, cols], [row_stride, 1]).double()
-        X = torch.where(X.isnan(), torch.full_like(X, -math.inf), X)
+        X = torch.where(X.isnan().any(1, keepdim=True), torch.full_like(X, -math.inf), X)
         row = lambda ptr, code, off: _flat(ptr, code, rows).double() if _addr(ptr) else torch.full([rows], off, dtype=torch.float64)
         T, K, P, MP, U = row(temperature, 0, 1.0), row(top_k, 3, 0.0), row(top_p, 0, 1.0), row(min_p, 0, 0.0), row(uniform, 0, 0.0)
         for r in range(rows):

@@ -44,9 +44,9 @@ def draw(x, u, temperature=None, top_k=None, top_p=None, min_p=None):
     """Token ids of rows x [rows, cols] (float64 numpy)."""
     tokens = []
     for r in range(len(x)):
-        z = np.where(np.isnan(x[r]), -np.inf, x[r])
+        z = x[r]
         T = 1.0 if temperature is None else float(temperature[r])
-        if z.max() == -np.inf:
+        if np.isnan(z).any() or z.max() == -np.inf:   # nothing to draw from
             tokens.append(0)
             continue
         if not T > 0:
@@ -65,7 +65,7 @@ def draw(x, u, temperature=None, top_k=None, top_p=None, min_p=None):
         if min_p is not None and min_p[r] > 0:
             keep = w >= min(float(min_p[r]), 1.0)
             rank, w = rank[keep], w[keep]
-        w = np.where(w < 2.0 ** -40, 0.0, w)   # by definition nothing that weighs less is drawn (it matters where u is 0)
+        w = np.where(w < 2.0 ** -41, 0.0, w)   # by definition nothing that weighs less is drawn (it matters where u is 0)
         o = np.argsort(rank)
         rank, sums = rank[o], np.cumsum(w[o])
         tokens.append(int(rank[min(len(rank) - 1, np.searchsorted(sums, float(u[r]) * sums[-1], side="right"))]))

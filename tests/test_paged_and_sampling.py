@@ -529,7 +529,7 @@ def test_draw_of_equal_masked_and_odd_values(native_lib, cols):
     check_draw(masked, u, top_k=k)
     check_draw(masked, u, top_p=r.uniform(0.2, 0.9, rows))
     odd = few.clone()
-    odd[:, 1] = float("nan")
+    odd[3, 1] = odd[7, cols - 1] = float("nan")     # rows with a NaN have nothing to draw from
     odd[1::3, 2] = inf
     odd[1::3, 4] = inf
     odd[2::3, :] = -inf
