@@ -21,7 +21,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 // refilled afterwards; the others are on their way meanwhile) and the block adds them up.
 // ===========================================================================
 constexpr int FEW_WARPS = 8, FEW_KEYS = 16;
-constexpr int FEW_OV = 4;          // what an item costs besides its 16-key blocks, in blocks
+// What an item costs besides its 16-key blocks, in blocks (a round of the eight warps is eight).  us at 4 / 8 / 16 / 28: 64 ragged sequences 29.6 / 29.1 / 28.6 / 28.1,
+// 200 of 100 to 1500 keys 34.3 / 33.4 / 30.5 / 29.6, one of 2000 10.9 / 10.1 / 9.1 / 10.7, eight of 500 to 8000 12.5 / 11.6 / 10.3 / 11.5, eight of 4097 11.9 / 13.9 / 12.8 / 12.0.
+constexpr int FEW_OV = 16;
 constexpr int FEW_MIN_SHARE = 16;  // blocks (and OVs) of a CTA at least
 constexpr float FEW_STEP = 8.f;    // the stored maximum follows the true one when that has grown by more (log2)
 constexpr int FEW_RING = 24576;    // bytes of a warp's ring

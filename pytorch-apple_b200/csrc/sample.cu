@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       const int at = __ffs(hit) - 1;
       const uint32_t upto = above + __shfl_sync(0xffffffffu, n, at), size = __shfl_sync(0xffffffffu, here, at);
       first += static_cast<uint32_t>(at) << shift;
-      if (upto <= want + want / 4 + 16 || shift <= 3) return first + ((1u << shift) - 1u);
+      if (upto <= want + want / 16 + 24 || shift <= 3) return first + ((1u << shift) - 1u);
       above = upto - size;
     }
   };
