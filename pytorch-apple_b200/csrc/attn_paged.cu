@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
         sum += s_l[e] * f;
         a += s_acc[e][threadIdx.x] * f;
       }
-      o[threadIdx.x] = from_f32<T>(sum > 0.f ? a / sum : 0.f);
+      o[threadIdx.x] = from_f32<T>(sum == 0.f ? 0.f : a / sum);   // (a sum that is no number stays one that is none)
     }
     __syncthreads();
   }
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(128) attn_paged_plain_kernel(const __grid_cons
     m = mn;
   }
   T* out = static_cast<T*>(p.out) + (n * p.Hq + h) * D + lane * E;
-  for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l > 0.f ? o[e] / l : 0.f);
+  for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
 }
 
 template <typename T, int D, int NT> int launch_few(const PagedParams& p, int dtype, cudaStream_t st) {
@@ -551,7 +551,8 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
     B200_FAIL(B200_EINVAL, "b200_attn_paged: workspace of %lld bytes required (got %lld)", (long long)need, (long long)a.workspace_bytes);
   p.q = a.q; p.k_pages = a.k_pages; p.v_pages = a.v_pages; p.out = a.out; p.q_start = a.q_start; p.kv_len = a.kv_len; p.table = a.page_table;
   p.B = a.B; p.N = a.n_tokens; p.num_pages = a.num_pages; p.table_stride = a.table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.page_size = a.page_size;
-  p.window = a.window; p.scale = a.scale;
+  p.window = a.window < (1ll << 30) ? a.window : 0;   // (no sequence is that long)
+  p.scale = a.scale;
   p.head = static_cast<int4*>(a.workspace);
   p.ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + ml);
   p.acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + acc);

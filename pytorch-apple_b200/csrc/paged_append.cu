@@ -99,8 +99,9 @@ extern "C" int b200_paged_append(const b200_paged_append_args* a, void* stream) 
     p.xs[0][i] = a->Hq > 0 ? a->q_strides[i] : 0; p.xs[1][i] = a->k_strides[i]; p.xs[2][i] = a->v_strides[i];
     ok = ok && p.xs[0][i] % 8 == 0 && p.xs[1][i] % 8 == 0 && p.xs[2][i] % 8 == 0;
   }
-  for (int i = 0; i < 3; ++i) { p.ps[i] = a->kv_strides[i]; ok = ok && a->kv_strides[i] % 8 == 0; }
-  if (!ok) B200_FAIL(B200_EALIGN, "b200_paged_append: operands must be 16-byte aligned with strides multiple of 8");
+  const int64_t kv_len[3] = {a->num_pages, a->Hkv, a->page_size};
+  for (int i = 0; i < 3; ++i) { p.ps[i] = a->kv_strides[i]; ok = ok && a->kv_strides[i] % 8 == 0 && (a->kv_strides[i] > 0 || kv_len[i] <= 1); }
+  if (!ok) B200_FAIL(B200_EALIGN, "b200_paged_append: operands must be 16-byte aligned with strides multiple of 8, those of the pages positive");
   if (a->n_tokens == 0) return B200_OK;
   p.cos_t = a->cos_t; p.sin_t = a->sin_t; p.q_out = a->q_out; p.k_pages = a->k_pages; p.v_pages = a->v_pages; p.slots = a->slots;
   p.N = a->n_tokens; p.n_slots = a->num_pages * a->page_size; p.Hq = a->Hq; p.Hkv = a->Hkv; p.D = a->D; p.page_size = a->page_size;

@@ -1,8 +1,8 @@
 // The calls of paged_attention.py and sampling.py from torch tensors to the library, as a CPython module.
 //
 // Checking the tensors, making the output and the workspace and filling the argument structure costs 10 us in Python, more than most of these
-// kernels run; here it costs one.  Every function takes the address of the library's entry point first (so that the test-suite can
-// put a stand-in there) and returns the output tensor, 1 where the tensors do not fit together (the caller says what it has
+// kernels run; here it costs one.  Every function takes the address of the library's entry point first, or minus the address of a stand-in of the
+// test-suite, which works on host memory, and returns the output tensor, 1 where the tensors do not fit together (the caller says what it has
 // seen), or the library's negative code.  Work goes to the current stream of the tensors' device, with that device current.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -51,6 +51,12 @@ bool pages(const Tensor& k, const Tensor& v, const Tensor& with, int64_t dims) {
 Tensor made(const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false)); }
 void* stream_of(const Tensor& t) { return t.is_cuda() ? static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) : nullptr; }
 
+// The entry point that `a` stands for, as a function; nullptr: it does not take tensors on the device that `t` is on
+template <typename F> F* entry(PyObject* a, const Tensor& t) {
+  const int64_t at = PyLong_AsLongLong(a);
+  return t.is_cuda() == (at > 0) ? reinterpret_cast<F*>(at > 0 ? at : -at) : nullptr;
+}
+
 PyObject* one() { return PyLong_FromLong(1); }
 
 // address, q, k, v, cos, sin, k_pages, v_pages, slots, q_out
@@ -58,10 +64,10 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 10 || !is_optional(a[1]) || !is_tensor(a[2]) || !is_tensor(a[3]) || !is_optional(a[4]) || !is_optional(a[5]) || !is_tensor(a[6]) ||
       !is_tensor(a[7]) || !is_tensor(a[8]) || !is_optional(a[9])) return one();
-  auto call = reinterpret_cast<int (*)(const b200_paged_append_args*, void*)>(PyLong_AsVoidPtr(a[0]));
   const Tensor *q = tensor(a[1]), *cos = tensor(a[4]), *sin = tensor(a[5]), *given = tensor(a[9]);
   const Tensor &k = *tensor(a[2]), &v = *tensor(a[3]), &kp = *tensor(a[6]), &vp = *tensor(a[7]), &slots = *tensor(a[8]);
-  if (k.dim() != 3 || code(k.scalar_type()) < 0) return one();
+  auto* const call = entry<int(const b200_paged_append_args*, void*)>(a[0], k);
+  if (!call || k.dim() != 3 || code(k.scalar_type()) < 0) return one();
   const int64_t N = k.size(0), Hkv = k.size(1), D = k.size(2);
   if (!heads(k, k, N) || !heads(v, k, N) || v.sizes() != k.sizes() || !pages(kp, vp, k, D) || kp.size(1) != Hkv || !dense(slots, k, at::kLong, {N})) return one();
   if (q && (!heads(*q, k, N) || q->size(2) != D)) return one();
@@ -100,14 +106,14 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 12 || !is_tensor(a[2]) || !is_tensor(a[3]) || !is_tensor(a[4]) || !is_tensor(a[5]) || !is_tensor(a[6]) || !is_tensor(a[7]) || !is_optional(a[11]))
     return one();
-  auto call = reinterpret_cast<int (*)(const b200_attn_paged_args*, void*)>(PyLong_AsVoidPtr(a[0]));
-  auto size = reinterpret_cast<int64_t (*)(int64_t, int, int, int)>(PyLong_AsVoidPtr(a[1]));
   const Tensor &q = *tensor(a[2]), &kp = *tensor(a[3]), &vp = *tensor(a[4]), &start = *tensor(a[5]), &len = *tensor(a[6]), &table = *tensor(a[7]);
   const Tensor* given = tensor(a[11]);
   const int64_t max_q = PyLong_AsLongLong(a[8]), window = PyLong_AsLongLong(a[10]);
   const double scale = PyFloat_AsDouble(a[9]);
   if (PyErr_Occurred()) return nullptr;
-  if (q.dim() != 3 || code(q.scalar_type()) < 0 || table.dim() != 2) return one();
+  auto* const call = entry<int(const b200_attn_paged_args*, void*)>(a[0], q);
+  auto* const size = entry<int64_t(int64_t, int, int, int)>(a[1], q);
+  if (!call || !size || q.dim() != 3 || code(q.scalar_type()) < 0 || table.dim() != 2) return one();
   const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), B = table.size(0);
   if (!heads(q, q, N) || !pages(kp, vp, q, D) || !dense(start, q, at::kInt, {B + 1}) || !dense(len, q, at::kInt, {B}) ||
       !dense(table, q, at::kInt, table.sizes()) || (given && !dense(*given, q, q.scalar_type(), q.sizes()))) return one();
@@ -142,10 +148,9 @@ PyObject* sample_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 8 || !is_tensor(a[1]) || !is_tensor(a[2])) return one();
   for (int i = 3; i < 8; ++i)
     if (!is_optional(a[i])) return one();
-  auto call = reinterpret_cast<int (*)(const void*, int64_t*, int64_t, int64_t, int64_t, const float*, const int32_t*, const float*, const float*, const float*, int,
-                                       void*)>(PyLong_AsVoidPtr(a[0]));
   const Tensor& x = *tensor(a[1]);
-  if (x.dim() != 2 || code(x.scalar_type()) < 0 || x.size(1) < 1 || (x.size(1) > 1 && x.stride(1) != 1)) return one();
+  auto* const call = entry<int(const void*, int64_t*, int64_t, int64_t, int64_t, const float*, const int32_t*, const float*, const float*, const float*, int, void*)>(a[0], x);
+  if (!call || x.dim() != 2 || code(x.scalar_type()) < 0 || x.size(1) < 1 || (x.size(1) > 1 && x.stride(1) != 1)) return one();
   const int64_t rows = x.size(0);
   for (int i = 2; i < 8; ++i) {
     const at::ScalarType type = i == 4 ? at::kInt : i == 7 ? at::kLong : at::kFloat;

@@ -181,15 +181,17 @@ def torch_calls():
 
 
 def entry(name: str) -> int:
-    """Address of entry point ``name`` of the library (or of the test stand-in) for ``torch_calls``."""
+    """Entry point ``name`` for ``torch_calls``: its address in the library, which takes CUDA tensors, or minus that of the test stand-in's."""
     lib = _test_override[0] if _test_override is not None else _lib or load()
     got = _entries.get(name)
     if got is None or got[0] is not lib:
         fn = getattr(lib, name)
-        if not isinstance(lib, C.CDLL):
+        stand_in = not isinstance(lib, C.CDLL)
+        if stand_in:
             restype, argtypes = SIGNATURES[name]
             fn = C.CFUNCTYPE(restype, *argtypes)(fn)
-        got = _entries[name] = (lib, C.cast(fn, C.c_void_p).value, fn)
+        address = C.cast(fn, C.c_void_p).value
+        got = _entries[name] = (lib, -address if stand_in else address, fn)
     return got[1]
 
 

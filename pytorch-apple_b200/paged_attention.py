@@ -7,7 +7,7 @@ new tokens of each: decoding sequences, pieces of prompts and whole prompts in o
 
 ``paged_append`` and ``paged_attention`` are the library's calls on torch tensors (CUDA, or host
 memory under the test stand-in); ``PagedKVCache`` owns pages and makes the index tensors of a step.
-Work is enqueued on the current stream of the tensors' device.
+Work is enqueued on the current stream of the tensors' device.  For serving: no gradients are recorded.
 """
 
 from __future__ import annotations
@@ -38,7 +38,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, slots, q_out=None):
     out = native.torch_calls().paged_append(native.entry("b200_paged_append"), q, k, v, cos, sin, k_pages, v_pages, slots, q_out)
     if out.__class__ is int:
         _failed("paged_append", out, "q [N, Hq, D] or None, k and v [N, Hkv, D] of one type with contiguous rows, cos and sin dense [N, D] in fp32 or that type "
-                "or both None, k_pages and v_pages alike [pages, Hkv, page_size, D], slots dense int64 [N], q_out dense like q, all on one device",
+                "or both None, k_pages and v_pages alike [pages, Hkv, page_size, D], slots dense int64 [N], q_out dense like q, all on one CUDA device",
                 q=q, k=k, v=v, cos=cos, sin=sin, k_pages=k_pages, v_pages=v_pages, slots=slots, q_out=q_out)
     return out
 
@@ -54,7 +54,7 @@ def paged_attention(q, k_pages, v_pages, q_start, kv_len, page_table, max_q, sca
                                                page_table, max_q, math.nan if scale is None else scale, window, out)
     if got.__class__ is int:
         _failed("paged_attention", got, "q [N, Hq, D] with contiguous rows, k_pages and v_pages alike [pages, Hkv, page_size, D] of its type, q_start [B + 1], kv_len "
-                "[B] and page_table [B, n] dense int32, out dense like q, all on one device", q=q, k_pages=k_pages, v_pages=v_pages, q_start=q_start,
+                "[B] and page_table [B, n] dense int32, out dense like q, all on one CUDA device", q=q, k_pages=k_pages, v_pages=v_pages, q_start=q_start,
                 kv_len=kv_len, page_table=page_table, out=out)
     return got
 

@@ -10,6 +10,7 @@ import torch
 
 from cuda_runtime import native
 
+
 def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
     """One token id per row of ``logits`` ``[rows, cols]`` (fp32, fp16 or bf16, any row stride); int64 ``[rows]``.
 
@@ -21,28 +22,28 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
         if got != 1:
             native.check(got, "sample_rows")
         raise ValueError("sample_rows: logits [rows, cols] of a float type with contiguous columns; uniform and, where given, temperature, top_p, min_p dense fp32 and "
-                         "top_k dense int32 [rows]; out dense int64 [rows]; all on one device; got " +
+                         "top_k dense int32 [rows]; out dense int64 [rows]; all on one CUDA device; got " +
                          ", ".join(f"{n} {tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else f"{n} {t}" for n, t in
                                    (("logits", logits), ("uniform", uniform), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("out", out))))
     return got
 
 
 class Sampler:
-    """Settings of the draw, for all rows alike or one number per row, and the generator of its random numbers."""
+    """Settings of the draw, for all rows alike or one number per row (as they are when the sampler is made), and the generators of its
+    random numbers, one per device.  For calls that are captured into a graph take ``sample_rows`` and numbers of your own."""
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0):
-        self.settings = {"temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32), "top_p": (top_p, torch.float32),
-                         "min_p": (min_p, torch.float32)}
+        self.settings = {name: torch.as_tensor(value).detach().to("cpu", dtype, copy=True) for name, value, dtype in (
+            ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32))}
         self.seed = seed
-        self._generator = None
+        self._generators: dict[torch.device, torch.Generator] = {}
         self._on: dict[tuple, dict] = {}
 
     def _rows(self, rows: int, device) -> dict:
         key = (rows, device)
         if key not in self._on:
             made = {}
-            for name, (value, dtype) in self.settings.items():
-                t = torch.as_tensor(value, dtype=dtype)
+            for name, t in self.settings.items():
                 if t.dim() > 1 or (t.dim() == 1 and t.shape[0] != rows):
                     raise ValueError(f"Sampler: {name} must be one number or one for each of the {rows} rows, got shape {tuple(t.shape)}")
                 made[name] = t.expand(rows).contiguous().to(device)
@@ -51,7 +52,7 @@ class Sampler:
 
     def __call__(self, logits):
         """Token ids ``[rows]`` for logits ``[rows, cols]``."""
-        if self._generator is None or self._generator.device != logits.device:
-            self._generator = torch.Generator(device=logits.device).manual_seed(self.seed)
-        uniform = torch.rand(logits.shape[0], generator=self._generator, device=logits.device)
+        if logits.device not in self._generators:
+            self._generators[logits.device] = torch.Generator(device=logits.device).manual_seed(self.seed)
+        uniform = torch.rand(logits.shape[0], generator=self._generators[logits.device], device=logits.device)
         return sample_rows(logits, uniform, **self._rows(logits.shape[0], logits.device))

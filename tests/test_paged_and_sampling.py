@@ -138,6 +138,39 @@ def test_library_refuses_sampling_calls(native_lib, change, code):
     assert native_lib.b200_sample_rows(*a.values()) == code
 
 
+def test_library_refuses_to_append_to_expanded_pages(native_lib):
+    """Rows of all heads (or pages) in one place would be written at once."""
+    from cuda_runtime import native
+
+    a = dict(q=4096, k=4096, v=4096, cos_t=4096, sin_t=4096, q_out=4096, k_pages=4096, v_pages=4096, slots=4096, n_tokens=3, num_pages=4, q_strides=(256, 64),
+             k_strides=(128, 64), v_strides=(128, 64), Hq=4, Hkv=2, D=64, page_size=16, table_dtype=0, dtype=2)
+    for strides in ((0, 1024, 64), (2048, 0, 64), (2048, 1024, 0), (2048, 1024, -64)):
+        assert native_lib.b200_paged_append(C.byref(native.PagedAppendArgs(**a, kv_strides=strides)), 0) == -2
+
+
+def test_tensors_in_host_memory_do_not_reach_the_library(native_lib):
+    from paged_attention import paged_append, paged_attention
+    from sampling import sample_rows
+
+    kp = torch.zeros(4, 2, 16, 64, dtype=BF)
+    for call in (lambda: paged_attention(**_small()), lambda: sample_rows(torch.zeros(2, 8), torch.zeros(2)),
+                 lambda: paged_append(None, torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF), None, None, kp, kp.clone(), torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="CUDA device"):
+            call()
+
+
+def test_sampler_keeps_the_settings_it_was_made_with(fake_native):
+    from sampling import Sampler
+
+    temperature = torch.zeros(2)
+    logits = torch.randn(2, 50, generator=torch.Generator().manual_seed(1))
+    sampler, greedy = Sampler(temperature=temperature), logits.argmax(1)
+    temperature += 5.0
+    assert torch.equal(sampler(logits), greedy)
+    temperature += 5.0
+    assert torch.equal(sampler(logits), greedy)
+
+
 def test_empty_calls_launch_nothing(native_lib):
     for change in ({"B": 0}, {"n_tokens": 0}, {"max_q": 0}):
         assert native_lib.b200_attn_paged(_attn_args(**change), 0) == 0
@@ -309,6 +342,33 @@ def test_attention_reads_pages_that_are_not_there_as_zeros_and_cuts_lengths(nati
     a["q_start"][0] = -4
     paged_attention(**full | {"q_start": a["q_start"]}, out=out)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [[(1, 300), (3, 1)], [(40, 300), (60, 17)]])
+@pytest.mark.parametrize("window", [(1 << 30) - 1, 1 << 30, (1 << 63) - 1])
+def test_attention_windows_longer_than_any_sequence(native_lib, seqs, window):
+    """As if there were none, for tokens ahead of position 0 too."""
+    from paged_attention import paged_attention
+
+    a, start, table = build(seqs, seed=4)
+    check_attention(paged_attention(**a, window=window), a, start, table, seqs)
+    assert torch.equal(paged_attention(**a, window=window), paged_attention(**a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,keys,table_pages", [(1, 300, 20), (1, 20000, 1250), (40, 300, 20), (40, 9000, 600)])
+def test_attention_of_a_query_that_is_no_number_gives_none(native_lib, T, keys, table_pages):
+    """Whether or not its keys are shared out and joined again; its neighbours do not notice."""
+    from paged_attention import paged_attention
+
+    a, start, table = build([(T, keys)], seed=5, table_extra=table_pages - -(-keys // 16))
+    broken = a["q"].clone()
+    broken[T // 2, 3] = float("nan")
+    got = paged_attention(**{**a, "q": broken})
+    assert got[T // 2, 3].isnan().all()
+    got[T // 2, 3] = paged_attention(**a)[T // 2, 3]
+    check_attention(got, a, start, table, [(T, keys)])
 
 
 @pytest.mark.gpu
