@@ -16,6 +16,8 @@
 // tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are sorted by one CTA, which mostly finds everything
 // that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or weights in 16 intervals of z, then in 16 parts
 // of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is drawn from by sums over ranges.
+#include <type_traits>
+
 #include "common.cuh"
 #include "mma.cuh"
 #include "tc5.cuh"
@@ -58,6 +60,36 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// Two fp32 numbers in a pair of registers, and the instructions for both at once
+struct Two { u64 v; };
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float first(Two a) { return __uint_as_float(static_cast<uint32_t>(a.v)); }
+__device__ __forceinline__ float second(Two a) { return __uint_as_float(static_cast<uint32_t>(a.v >> 32)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2_down(Two a, Two b) {   // rounded towards zero
+  Two r;
+  asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // exp((z - m) / T) = 2^-t, t = (m - z) log2(e) / T.  log2(e) / T is carried as a pair of fp32 numbers, and the difference where it need not be whole:
 // a rounding of t = 30 alone would be 2^-20 of the weight.  Two ways:
 // - the few tokens that the row's sum mostly consists of (t below 12, less at temperatures above 1, where the sum spreads over more) by the table method
@@ -81,8 +113,7 @@ template <typename T> struct Weigher {
     const float shifted = fmaf(dh, c_hi, 12582912.f);      // + 1.5 2^23: t to the nearest whole number
     float x = fmaf(dh, c_lo, fmaf(dh, c_hi, -(shifted - 12582912.f)));
     if constexpr (sizeof(T) == 4) x = dh < end ? fmaf(rest(z, dh), c_hi, x) : x;   // (differences of 16-bit logits are whole but for those next to zero)
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(-x));
+    float y = exp2_fast(-x);
     y *= __uint_as_float((147u << 23) - (__float_as_uint(shifted) << 23));   // 2^(20 - whole): the weight in units of 2^-20
     const float h = __fadd_rz(y, 8388608.f);
     hi = __float_as_uint(h);
@@ -121,32 +152,61 @@ template <typename T> struct Weigher {
       f(v, at);
     }
   }
-  // Sum of the weights, of at least `least`, of those of eight tokens that keep(token, column) lets through (FROM: there is a least weight)
-  template <bool FROM, typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, u64 least, K&& keep) const {
-    uint32_t hi = 0, lo = 0, close = 0;
+  // Sum of the weights, of at least `least`, of those of eight tokens that keep(token, column) lets through
+  template <typename K> __device__ __forceinline__ u64 sum(const float (&z)[8], int c, u64 least, K&& keep) const {
+    uint32_t close = 0;
     u64 t = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float dh = difference(z[k]);
       const bool kept = keep(z[k], c + k);
       close |= (kept && dh < near ? 1u : 0u) << k;
-      const float d = kept && dh >= near ? dh : end;
-      if (FROM) {
-        const u64 w = other(z[k], d);
-        t += w >= least ? w : 0;
-      } else {
-        uint32_t h, l;
-        parts(z[k], d, h, l);
-        hi += h;
-        lo += l;
-      }
+      const u64 w = other(z[k], kept && dh >= near ? dh : end);
+      t += w >= least ? w : 0;
     }
-    if (!FROM) t = (static_cast<u64>(hi - 8u * 0x4b000000u) << 20) + (lo - 8u * 0x4b000000u);
     each_set(close, z, [&](float v, int) {
       const u64 w = large(v);
-      t += !FROM || w >= least ? w : 0;
+      t += w >= least ? w : 0;
     });
     return t;
+  }
+  // Running sum of a lane's weights: its two parts (with 0x4b000000 for every token so far: up to 1024 of them, below 2^31), and what near tokens weigh
+  // more than in the parts
+  struct Sum {
+    uint32_t hi = 0, lo = 0, tokens = 0;
+    u64 near = 0;
+    __device__ __forceinline__ u64 total() const { return (static_cast<u64>(hi - tokens * 0x4b000000u) << 20) + (lo - tokens * 0x4b000000u) + near; }
+  };
+  // Adds the weights of eight tokens, the largest of which is `top`: the other way for all of them, two at a time (as parts() to the bit), then the few near
+  // ones once more
+  __device__ __forceinline__ void add(Sum& sum, const float (&z)[8], float top) const {
+    const Two m2 = two(m, m), nch = two(-c_hi, -c_hi), ncl = two(-c_lo, -c_lo), minus = two(-1.f, -1.f), half = two(12582912.f, 12582912.f);
+    const Two unit = two(8388608.f, 8388608.f), low = two(1048576.f, 1048576.f);
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const Two z2 = two(z[k], z[k + 1]);
+      Two d = fma2(z2, minus, m2);
+      d = two(fminf(first(d), end), fminf(second(d), end));
+      const Two shifted = fma2(d, nch, half);              // t's nearest whole number, counted down
+      Two x = fma2(d, ncl, fma2(d, nch, fma2(shifted, minus, half)));   // - (t - the nearest whole number)
+      if constexpr (sizeof(T) == 4) {
+        const Two one = two(1.f, 1.f), bv = fma2(d, minus, m2), a = fma2(fma2(d, one, bv), minus, m2), b = fma2(z2, minus, bv);
+        const Two y = fma2(fma2(a, one, b), nch, x);
+        x = two(first(d) < end ? first(y) : first(x), second(d) < end ? second(y) : second(x));
+      }
+      Two y = two(exp2_fast(first(x)), exp2_fast(second(x)));
+      y = mul2(y, two(__uint_as_float((__float_as_uint(first(shifted)) << 23) + (147u << 23)), __uint_as_float((__float_as_uint(second(shifted)) << 23) + (147u << 23))));
+      const Two h = add2_down(y, unit), l = fma2(fma2(fma2(unit, minus, h), minus, y), low, unit);
+      sum.hi += __float_as_uint(first(h)) + __float_as_uint(second(h));
+      sum.lo += __float_as_uint(first(l)) + __float_as_uint(second(l));
+    }
+    sum.tokens += 8;
+    if (difference(top) < near) {
+      uint32_t close = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) close |= (difference(z[k]) < near ? 1u : 0u) << k;
+      each_set(close, z, [&](float v, int) { sum.near += large(v) - other(v, difference(v)); });
+    }
   }
 };
 
@@ -235,6 +295,60 @@ template <typename T> struct Row {
       float z[8];
       load(c, z);
       f(of(z), c);
+    }
+  }
+  // f(eight tokens, the largest of them, their first column) for all of the warp's columns
+  template <typename F> __device__ __forceinline__ void eights(F&& f) const {
+    const auto of = [](const float (&z)[8]) { return fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))); };
+    int c = begin + (threadIdx.x & 31) * 8;
+    if (!infinite && (copied > begin || vec)) {   // the next load is under way meanwhile
+      const T* const at = copied > begin ? copy - begin : x;
+      const int all = copied > begin ? copied : end;
+      using Raw = std::conditional_t<sizeof(T) == 2, uint4, float4>;
+      Raw w[8 * sizeof(T) / 16];
+      if (c + 8 <= all) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = *(reinterpret_cast<const Raw*>(at + c) + i);
+      }
+#pragma unroll 1
+      for (; c + 8 <= all; c += 256) {
+        float z[8], top;
+        if constexpr (sizeof(T) == 2) {
+          unpack8<T>(w[0], z);
+          float a, b;
+          unpack2<T>(max2<T>(max2<T>(w[0].x, w[0].y), max2<T>(w[0].z, w[0].w)), a, b);
+          top = fmaxf(a, b);
+        } else {
+          z[0] = w[0].x; z[1] = w[0].y; z[2] = w[0].z; z[3] = w[0].w; z[4] = w[1].x; z[5] = w[1].y; z[6] = w[1].z; z[7] = w[1].w;
+          top = of(z);
+        }
+        if (c + 256 + 8 <= all) {
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = *(reinterpret_cast<const Raw*>(at + c + 256) + i);
+        }
+        f(z, top, c);
+      }
+    }
+    for (; c < end; c += 256) {
+      float z[8];
+      load(c, z);
+      f(z, of(z), c);
+    }
+  }
+  // f(eight tokens, their first column) for those eights that have one of at least `floor`: first where there is any at all, 32 of a lane at a time, then
+  // those one after the other (a warp has few where few tokens matter, but hardly 256 columns without one: k = 400 in 64 rows 2 us instead of 7.5)
+  template <typename F> __device__ __forceinline__ void from(float floor, F&& f) const {
+#pragma unroll 1
+    for (int base = begin; base < end; base += 32 * 256) {
+      uint32_t some = 0;
+      tops(base, base + 32 * 256, [&](float z, int c) { some |= (z >= floor ? 1u : 0u) << ((c - base) >> 8); });
+      while (some) {
+        const int c = base + (__ffs(some) - 1) * 256 + (threadIdx.x & 31) * 8;
+        some &= some - 1;
+        float z[8];
+        load(c, z);
+        f(z, c);
+      }
     }
   }
   static __device__ __forceinline__ void unpack(const T* at, float (&f)[8]) {
@@ -497,33 +611,26 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   u64 whole = 0;         // sum of what is kept before top-p
   auto limit_of = [&](u64 sum) { return fmax(static_cast<double>(tp) * static_cast<double>(sum), 0.5); };
   const bool restricted_by_k = k > 0 && k < p.cols;
+  auto lowest = [&](uint32_t hi) {   // no token with a place up to `hi` is below this
+    return weight.m - fminf((static_cast<float>(hi) + 8.f) * (1.0001f / 131072.f) / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f;
+  };
   auto collect = [&](uint32_t lo, uint32_t hi) {   // tokens with places in [lo, hi], to CTA 0: into a list of each CTA's own, then in one piece
     // (a bound on the logits with some room: places are looked at only behind it)
     const float above = lo == 0 ? INFINITY : weight.m - (static_cast<float>(lo) - 8.f) * (0.9999f / 131072.f) / weight.c_hi + fabsf(weight.m) * 5e-7f;
-    const float bound = weight.m - fminf((static_cast<float>(hi) + 8.f) * (1.0001f / 131072.f) / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f;
-    // First where there is anything at all, 32 times eight tokens of a lane at a time, then those one after the other: a warp has few such, but hardly a
-    // 256 columns without one.  (k = 400: 2 us instead of 7.5.)
-    for (int base = row.begin; base < row.end; base += 32 * 256) {
-      uint32_t packs = 0;
-      row.tops(base, base + 32 * 256, [&](float z, int c) { packs |= (z >= bound ? 1u : 0u) << ((c - base) >> 8); });
-      while (packs) {
-        const int c = base + (__ffs(packs) - 1) * 256 + lane * 8;
-        packs &= packs - 1;
-        float z[8];
-        uint32_t some = 0;
-        row.load(c, z);
+    const float bound = lowest(hi);
+    row.from(bound, [&](const float (&z)[8], int c) {
+      uint32_t some = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) some |= (z[k] >= bound && z[k] <= above ? 1u : 0u) << k;
-        weight.each_set(some, z, [&](float v, int k) {
-          const float dh = weight.difference(v);
-          const uint32_t X = place(dh);
-          if (dh < weight.end && X <= hi && X >= lo && stays(v, c + k)) {
-            const int at = atomicAdd(&sh.listed, 1);
-            if (at < CAP) bins[at] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~(c + k));
-          }
-        });
-      }
-    }
+      for (int k = 0; k < 8; ++k) some |= (z[k] >= bound && z[k] <= above ? 1u : 0u) << k;
+      weight.each_set(some, z, [&](float v, int k) {
+        const float dh = weight.difference(v);
+        const uint32_t X = place(dh);
+        if (dh < weight.end && X <= hi && X >= lo && stays(v, c + k)) {
+          const int at = atomicAdd(&sh.listed, 1);
+          if (at < CAP) bins[at] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~(c + k));
+        }
+      });
+    });
     __syncthreads();
     if (ctas == 1) return;
     // Everybody learns how many the others have: a CTA's go behind those of the ones before it
@@ -553,7 +660,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     sort_list(bins, n);
     return n;
   };
-  auto search = [&](const bool by_mass) -> int {
+  auto search = [&](const bool by_mass) __attribute__((always_inline)) -> int {
     uint32_t first = 0, end = LAST_PLACE, above = 0;   // places that are looked at, tokens before them
     u64 above_mass = 0;
     double limit = 0.;
@@ -563,7 +670,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
 #pragma unroll
       for (int b = 0; b < BINS; ++b) own[b * 32] = 0;
       // (a lane has fewer than 2^12 columns of a row, each below 2^40 + 1: 12 bits count, 52 add up)
-      row.packs([&](const float (&z)[8], int c) {
+      const auto count_in = [&](const float (&z)[8], int c) {
         uint32_t close = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -580,7 +687,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
           if (in) own[(X >> shift) * 32] += add;
         }
         weight.each_set(close, z, [&](float v, int) { own[((place(weight.difference(v)) - first) >> shift) * 32] += (1ull << 52) + weight.large(v); });
-      });
+      };
+      if (end == LAST_PLACE) row.packs(count_in); else row.from(lowest(end), count_in);
       __syncwarp();
       {
         const int b = lane >> 1;
@@ -794,9 +902,9 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const bool few_k = restricted_by_k && 2 * k <= threads && k <= CAP / 2;
   if (few_k || (tp < 1.f && !restricted_by_k)) {
     if (!few_k) {
-      u64 s = 0;
-      row.packs([&](const float (&z)[8], int c) { s += weight.template sum<false>(z, c, 0, [](float, int) { return true; }); });
-      whole = row_reduce<false>(s, sh, ctas, turn);
+      typename Weigher<T>::Sum s;
+      row.eights([&](const float (&z)[8], float top_, int) { weight.add(s, z, top_); });
+      whole = row_reduce<false>(s.total(), sh, ctas, turn);
     }
     const uint32_t upto = reach(few_k ? static_cast<uint32_t>(k) : 96u);
     collect(0, upto);
@@ -851,9 +959,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const float at_cut = value_of(cut);
   const auto all = [](float, int) { return true; };
   const auto some = [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); };
-  if (cut == 0 && least == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<false>(z, c, 0, all); });
-  else if (cut == 0) row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, least, all); });
-  else row.packs([&](const float (&z)[8], int c) { mine += weight.template sum<true>(z, c, least, some); });
+  // (no token that weighs `least` is below this: the weight is at least half of it)
+  const float enough = least > 0 ? weight.m - fminf((41.01f - log2f(static_cast<float>(least))) * 1.0001f / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f : -INFINITY;
+  if (cut == 0 && least == 0) {
+    typename Weigher<T>::Sum s;
+    row.eights([&](const float (&z)[8], float top_, int) { weight.add(s, z, top_); });
+    mine = s.total();
+  } else if (cut == 0) row.from(enough, [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, all); });
+  else row.from(fmaxf(enough, at_cut), [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, some); });
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
