@@ -378,34 +378,26 @@ template <typename T> struct Row {
   }
 };
 
-__device__ __forceinline__ u64 warp_add(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ u64 warp_top(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+__device__ __forceinline__ u64 warp_add(u64 v) {   // (v below 2^62; in three parts the warp's own instruction does it)
+  const uint32_t a = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0x3ffffffu), b = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 26) & 0x3ffffffu);
+  return a + (static_cast<u64>(b) << 26) + (static_cast<u64>(__reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 52))) << 52);
 }
 
-// Sum or maximum over all threads of the row, known to all of them.  sh.told holds the CTAs' values afterwards, in slot `turn`.
+// Sum, or maximum (of 32 bits), over all threads of the row, known to all of them.  sh.told holds the CTAs' values afterwards, in slot `turn`.
 template <bool TOP> __device__ u64 row_reduce(u64 v, Shared& sh, int ctas, int& turn) {
-  v = TOP ? warp_top(v) : warp_add(v);
+  v = TOP ? __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v)) : warp_add(v);
   if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x < 32) {
     u64 s = threadIdx.x < SW ? sh.part[threadIdx.x] : 0;
-    s = TOP ? warp_top(s) : warp_add(s);
+    s = TOP ? __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(s)) : warp_add(s);
     if (ctas == 1) {
       if (threadIdx.x == 0) sh.told[turn][0] = s;
     } else if (static_cast<int>(threadIdx.x) < ctas) {
       const uint32_t to = tc5::map_to_rank(tc5::smem_addr(&sh.told[turn][tc5::cluster_ctarank()]), threadIdx.x);
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(s) : "memory");
     }
+    __syncwarp();
   }
   if (ctas == 1) __syncthreads(); else tc5::cluster_sync();
   u64 r = 0;
@@ -961,12 +953,19 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const auto some = [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); };
   // (no token that weighs `least` is below this: the weight is at least half of it)
   const float enough = least > 0 ? weight.m - fminf((41.01f - log2f(static_cast<float>(least))) * 1.0001f / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f : -INFINITY;
-  if (cut == 0 && least == 0) {
+  const bool everything = cut == 0 && least == 0;
+  if (everything) {
     typename Weigher<T>::Sum s;
     row.eights([&](const float (&z)[8], float top_, int) { weight.add(s, z, top_); });
     mine = s.total();
   } else if (cut == 0) row.from(enough, [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, all); });
   else row.from(fmaxf(enough, at_cut), [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, some); });
+  const auto sum_of = [&](const float (&z)[8], int c) -> u64 {
+    if (!everything) return weight.sum(z, c, least, stays);
+    typename Weigher<T>::Sum s;
+    weight.add(s, z, fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))));
+    return s.total();
+  };
   mine = warp_add(mine);
   const int slot = turn;
   const u64 total = row_reduce<false>(lane == 0 ? mine : 0, sh, ctas, turn);
@@ -985,12 +984,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   for (int b_ = part.begin; b_ < part.end; b_ += SW * 256) {
     const int c = b_ + warp * 256 + lane * 8;
     float v[8];
-    u64 w[8], s = 0;
-    if (c < part.end) part.load(c, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = c < part.end ? kept(v[e], c + e) : 0;
-      s += w[e];
+    u64 s = 0;
+    if (c < part.end) {
+      part.load(c, v);
+      s = sum_of(v, c);
     }
     u64 upto = s;
 #pragma unroll
@@ -1009,11 +1006,20 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       before += t;
     }
     const unsigned passed = __ballot_sync(0xffffffffu, mine_ + upto > target);
-    if (target >= mine_ && passed && lane == __ffs(passed) - 1) {
-      u64 run = mine_ + upto - s;
-      int e = 0;
-      while (e < 7 && run + w[e] <= target) run += w[e++];
-      p.out[r] = c + e;
+    if (target >= mine_ && passed) {   // one of the eight tokens of lane `src`: a lane for each of them
+      const int src = __ffs(passed) - 1, c_ = b_ + warp * 256 + src * 8;
+      part.load(c_, v);
+      float z = v[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) z = (lane & 7) == e ? v[e] : z;
+      u64 run = kept(z, c_ + (lane & 7));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, run, o);
+        if ((lane & 7) >= o) run += t;
+      }
+      const unsigned reached = __ballot_sync(0xffffffffu, __shfl_sync(0xffffffffu, mine_ + upto - s, src) + run > target) & 0x7fu;
+      if (lane == 0) p.out[r] = c_ + (reached ? __ffs(reached) - 1 : 7);
     }
     if (target < before) return;
   }
