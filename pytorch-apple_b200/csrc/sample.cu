@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   // Looks for the token that the filter ends with: the k-th (count), or the one at which the running sum reaches `limit`.  Result: 0 nothing is cut off,
   // 1 all that is kept is in the list of CTA 0, 2 (cut, last) are found, 3 they are to be found bit by bit.
   u64 whole = 0;         // sum of what is kept before top-p
+  bool few = false;      // the search knows that hardly an eighth of a warp's tokens can still matter: Row::from() instead of Row::eights()
   auto limit_of = [&](u64 sum) { return fmax(static_cast<double>(tp) * static_cast<double>(sum), 0.5); };
   const bool restricted_by_k = k > 0 && k < p.cols;
   auto lowest = [&](uint32_t hi) {   // no token with a place up to `hi` is below this
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     // (a bound on the logits with some room: places are looked at only behind it)
     const float above = lo == 0 ? INFINITY : weight.m - (static_cast<float>(lo) - 8.f) * (0.9999f / 131072.f) / weight.c_hi + fabsf(weight.m) * 5e-7f;
     const float bound = lowest(hi);
-    row.from(bound, [&](const float (&z)[8], int c) {
+    const auto take = [&](const float (&z)[8], int c) {
       uint32_t some = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) some |= (z[k] >= bound && z[k] <= above ? 1u : 0u) << k;
@@ -622,7 +623,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
           if (at < CAP) bins[at] = static_cast<u64>(key_of(v)) << 32 | static_cast<uint32_t>(~(c + k));
         }
       });
-    });
+    };
+    if (lo == 0 || few) row.from(bound, take); else row.eights([&](const float (&z)[8], float, int c) { take(z, c); });
     __syncthreads();
     if (ctas == 1) return;
     // Everybody learns how many the others have: a CTA's go behind those of the ones before it
@@ -676,11 +678,14 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
             in = in && dh >= weight.near;
             add += weight.other(z[e], dh);
           }
-          if (in) own[(X >> shift) * 32] += add;
+          own[in ? (X >> shift) * 32 : 0] += in ? add : 0;   // (without a branch)
         }
         weight.each_set(close, z, [&](float v, int) { own[((place(weight.difference(v)) - first) >> shift) * 32] += (1ull << 52) + weight.large(v); });
       };
-      if (end == LAST_PLACE) row.packs(count_in); else row.from(lowest(end), count_in);
+      const float floor = end == LAST_PLACE ? -INFINITY : lowest(end);
+      if (few) row.from(floor, count_in); else row.eights([&](const float (&z)[8], float top_, int c) {
+        if (top_ >= floor) count_in(z, c);
+      });
       __syncwarp();
       {
         const int b = lane >> 1;
@@ -738,6 +743,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       above_mass += __shfl_sync(0xffffffffu, s, b) - __shfl_sync(0xffffffffu, mass, b);
       first += static_cast<uint32_t>(b) << shift;
       end = first + ((1u << shift) - 1u);
+      few = (above + here) * 32 < static_cast<uint32_t>(p.cols);
       if (above + here <= CAP) { collect(0, end); return 1; }
       if (here <= CAP && (above > CAP - CAP / 8 || shift == 0)) {   // the last token kept is among these
         collect(first, end);
@@ -951,19 +957,28 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   const float at_cut = value_of(cut);
   const auto all = [](float, int) { return true; };
   const auto some = [&](float v, int i) { return v > at_cut || (v == at_cut && i <= last); };
+  const auto add = [&](typename Weigher<T>::Sum& s, const float (&z)[8], float top_, int c) {
+    if (cut == 0) {
+      weight.add(s, z, top_);
+    } else if (top_ >= at_cut) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = some(z[e], c + e) ? z[e] : -INFINITY;
+      weight.add(s, v, top_);
+    }
+  };
   // (no token that weighs `least` is below this: the weight is at least half of it)
   const float enough = least > 0 ? weight.m - fminf((41.01f - log2f(static_cast<float>(least))) * 1.0001f / weight.c_hi, weight.end) - fabsf(weight.m) * 5e-7f : -INFINITY;
-  const bool everything = cut == 0 && least == 0;
-  if (everything) {
+  if (least == 0 && !(few && cut != 0)) {
     typename Weigher<T>::Sum s;
-    row.eights([&](const float (&z)[8], float top_, int) { weight.add(s, z, top_); });
+    row.eights([&](const float (&z)[8], float top_, int c) { add(s, z, top_, c); });
     mine = s.total();
   } else if (cut == 0) row.from(enough, [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, all); });
   else row.from(fmaxf(enough, at_cut), [&](const float (&z)[8], int c) { mine += weight.sum(z, c, least, some); });
   const auto sum_of = [&](const float (&z)[8], int c) -> u64 {
-    if (!everything) return weight.sum(z, c, least, stays);
+    if (least != 0) return weight.sum(z, c, least, stays);
     typename Weigher<T>::Sum s;
-    weight.add(s, z, fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))));
+    add(s, z, fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))), c);
     return s.total();
   };
   mine = warp_add(mine);
