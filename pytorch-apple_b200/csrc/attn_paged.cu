@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   __shared__ int s_first[PAGED_MAX_PIECES + 1];   // blocks ahead of each piece of the list
   __shared__ float s_m[FEW_WARPS][ROWS], s_l[FEW_WARPS][ROWS];
   __shared__ int s_park[FEW_WARPS];               // where a warp has parked its accumulators (ring stage, -1: it has none)
-  __shared__ int64_t s_total[FEW_WARPS];
+  __shared__ int64_t s_total[FEW_WARPS], s_small[(32 * 20 + 8) / 8];
   __shared__ int s_count, s_more;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
   if (threadIdx.x == 0) { tc5::prefetch_tensormap(&map_k); tc5::prefetch_tensormap(&map_v); }
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
-  const PagedWork work = paged_work(smem);   // (nothing has been copied into the rings yet)
+  const bool small = p.B <= 32;   // the first warp's own matter (paged_prefix), in a place of its own; others lie over the rings, which are still empty
+  const PagedWork work = small ? paged_work(s_small, 32) : paged_work(smem, PAGED_MAX_SEQS);
   int64_t u0 = 0, u1 = 0, share = 1, ends = 0;
   auto deal = [&]() {   // this block's range of costs (as far as it is known to this warp)
     const int64_t total = paged_prefix<FEW_KEYS, FEW_OV, FEW_WARPS * 32>(p, tpt, work, s_total);
@@ -101,10 +102,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
       if (x < X) {
         int f = 0;
         while (x >= s_first[f + 1]) ++f;
-        const int key = (s_piece[f].j0 + x - s_first[f]) * FEW_KEYS, i = key / p.page_size;
+        const int key = (s_piece[f].j0 + x - s_first[f]) * FEW_KEYS, i = paged_page(p, key);
         row = key - i * p.page_size;
         hk = s_piece[f].hk;
-        const int hi = s_piece[f].p0 + s_piece[f].rows / p.G;
+        const int hi = s_piece[f].p0 + s_piece[f].tokens;
         page = key < hi ? __ldg(p.table + s_piece[f].b * p.table_stride + i) : -1;   // (an item without keys has no page either)
         if (page < 0 || page >= p.num_pages) page = static_cast<int>(p.num_pages);   // outside the tensor: zeros
       }
@@ -125,21 +126,24 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
       st_copy = st_copy + 1 == STAGES ? 0 : st_copy + 1;
     };
     look(warp + FEW_WARPS * lane, id_page, id_row, id_hk);
-    tc5::fence_proxy_async();
-    __syncthreads();   // (the running costs lie in the rings: everybody is through with them)
+    if (!small) {
+      tc5::fence_proxy_async();
+      __syncthreads();   // (everybody is through with the running costs)
+    }
     for (int s = 0; s < STAGES; ++s) copy();
 
     // Q^T fragments: row 8 j + g, dims 16 ks + 2 t, +1 and 16 ks + 2 t + 8, +9
     uint32_t qf[KS][NT][2];
     auto load_q = [&](const PagedPiece& c) {
+      const int rows = c.tokens * p.G;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int r = 8 * j + g;
         const T* qr = static_cast<const T*>(p.q) + (static_cast<int64_t>(c.token) + r / p.G) * p.qs[0] + (c.hk * p.G + r % p.G) * p.qs[1] + 2 * t;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          qf[ks][j][0] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks) : 0u;
-          qf[ks][j][1] = r < c.rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8) : 0u;
+          qf[ks][j][0] = r < rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks) : 0u;
+          qf[ks][j][1] = r < rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8) : 0u;
         }
       }
     };
@@ -148,7 +152,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 #pragma unroll 1
     for (int f = 0; f < F; ++f) {
       const PagedPiece c = s_piece[f];
-      const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
+      const int rows = c.tokens * p.G, hi = c.p0 + c.tokens;   // keys from here on nobody sees
       const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
       const int x_end = s_first[f + 1], key_base = (c.j0 - s_first[f]) * FEW_KEYS;
       float m[NT][2], l[NT][2], o[KS][NT][4];
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = 8 * j + 2 * t + e;
-            see[j][e] = r < c.rows ? c.p0 + r / p.G + 1 : hi;
+            see[j][e] = r < rows ? c.p0 + r / p.G + 1 : hi;
             from[j][e] = p.window > 0 && see[j][e] - p.window > 0 ? static_cast<int>(see[j][e] - p.window) : 0;
             see_min = min(see_min, see[j][e]);
             from_max = max(from_max, from[j][e]);
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
         const int d = threadIdx.x % LPR * 4;
         const bool whole = c.flags == 3;
         const int64_t slot = paged_slot(cta, c.flags & 1, ROWS);
-        for (int r = threadIdx.x / LPR; r < c.rows; r += FEW_WARPS * 32 / LPR) {
+        for (int r = threadIdx.x / LPR; r < rows; r += FEW_WARPS * 32 / LPR) {
           float mw[FEW_WARPS], top = -INFINITY;
           float4 a[FEW_WARPS];
 #pragma unroll
@@ -345,7 +349,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
     deal();   // (the rings lay over the running costs)
   }
   if (threadIdx.x == 0 && !p.whole) {
-    if (head.x) head.x = static_cast<int>((ends - 1) / share) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
+    if (head.x) head.x = static_cast<int>(paged_divide(ends - 1, share)) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
     p.head[cta] = head;
   }
 }
@@ -551,6 +555,7 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
     B200_FAIL(B200_EINVAL, "b200_attn_paged: workspace of %lld bytes required (got %lld)", (long long)need, (long long)a.workspace_bytes);
   p.q = a.q; p.k_pages = a.k_pages; p.v_pages = a.v_pages; p.out = a.out; p.q_start = a.q_start; p.kv_len = a.kv_len; p.table = a.page_table;
   p.B = a.B; p.N = a.n_tokens; p.num_pages = a.num_pages; p.table_stride = a.table_stride; p.Hq = Hq; p.Hkv = Hkv; p.G = G; p.page_size = a.page_size;
+  p.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz(a.page_size) : -1;
   p.window = a.window < (1ll << 30) ? a.window : 0;   // (no sequence is that long)
   p.scale = a.scale;
   p.head = static_cast<int4*>(a.workspace);

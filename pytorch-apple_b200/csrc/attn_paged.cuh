@@ -10,7 +10,7 @@ struct PagedParams {
   const int32_t *q_start, *kv_len, *table;
   int64_t B, N, num_pages, table_stride;
   int64_t qs[2], ks[3];            // element strides: q over (token, head), pages over (page, head, row)
-  int Hq, Hkv, G, page_size;
+  int Hq, Hkv, G, page_size, page_shift;   // page_shift: log2 of the page size, negative where that is no power of two
   int64_t window;                  // keys a token sees back from its own (0: all)
   float scale;
   int whole;                       // items are not cut: a block takes those that begin in its range
@@ -43,9 +43,16 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int64_t b) {
 // result.  Lengths are read on the device (a captured call follows them), every block works the cuts out for itself, and sequences
 // of any lengths load all blocks alike.
 struct PagedPiece {
-  int32_t b, hk, token, rows;   // sequence, KV head, first token (index into q), rows = tokens * G
+  int32_t b, hk, token, tokens;   // sequence, KV head, first token (index into q) and how many
   int32_t p0, j0, cnt, flags;   // position of the first token, first key tile and number of them, 1: the item begins here, 2: it ends here
 };
+
+// (A block has these on its way to its first key, where a division by a number that only the caller knows is 0.05 to 0.2 us)
+__device__ __forceinline__ int paged_page(const PagedParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size; }
+__device__ __forceinline__ int paged_tiles(int T, int tpt) { return T <= tpt ? (T > 0 ? 1 : 0) : (T + tpt - 1) / tpt; }
+__device__ __forceinline__ int64_t paged_divide(int64_t a, int64_t b) {   // (neither is negative)
+  return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
 
 struct PagedTile { int t0, t1, j0, cnt; int64_t p0; };
 template <int KT> __device__ __forceinline__ PagedTile paged_tile(const PagedParams& p, int T, int64_t n, int i, int tpt) {
@@ -72,12 +79,12 @@ struct PagedWork {
   int32_t* T;          // [B]: tokens
 };
 constexpr int paged_work_bytes = PAGED_MAX_SEQS * 20 + 8;
-__device__ __forceinline__ PagedWork paged_work(void* at) {
+__device__ __forceinline__ PagedWork paged_work(void* at, int seqs) {   // 20 bytes per sequence and 8
   PagedWork w;
   w.pre = static_cast<int64_t*>(at);
-  w.first = reinterpret_cast<int32_t*>(w.pre + PAGED_MAX_SEQS + 1);
-  w.n = w.first + PAGED_MAX_SEQS;
-  w.T = w.n + PAGED_MAX_SEQS;
+  w.first = reinterpret_cast<int32_t*>(w.pre + seqs + 1);
+  w.n = w.first + seqs;
+  w.T = w.n + seqs;
   return w;
 }
 
@@ -97,7 +104,7 @@ template <int KT, int OV, int THREADS> __device__ int64_t paged_prefix(const Pag
       w.n[b] = static_cast<int>(s.n);
       w.T[b] = s.T;
     }
-    const int tiles = (s.T + tpt - 1) / tpt;
+    const int tiles = paged_tiles(s.T, tpt);
     int64_t cost = 0;
     if (tiles == 1) cost = paged_tile<KT>(p, s.T, s.n, 0, tpt).cnt + OV;
     // a prompt's many tiles: the whole warp adds them up
@@ -155,13 +162,13 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
   for (int b = lo; b < B && w.pre[b] < u1; ++b) {
     const int64_t begin = w.pre[b], all = w.pre[b + 1] - begin;
     if (begin + all <= u0 || all == 0) continue;
-    const int T = w.T[b], first = w.first[b], tiles = (T + tpt - 1) / tpt;
+    const int T = w.T[b], first = w.first[b], tiles = paged_tiles(T, tpt);
     const int64_t n = w.n[b];
     int skip = 0;   // heads ahead of u0
     int64_t base = begin;
     if (u0 > begin && p.Hkv > 1) {
-      const int64_t per_head = tiles == 1 ? paged_tile<KT>(p, T, n, 0, tpt).cnt + OV : all / p.Hkv, off = u0 - begin;
-      skip = p.Hkv <= 32 ? __popc(__ballot_sync(0xffffffffu, lane < p.Hkv && (lane + 1) * per_head <= off)) : static_cast<int>(off / per_head);
+      const int64_t per_head = tiles == 1 ? paged_tile<KT>(p, T, n, 0, tpt).cnt + OV : paged_divide(all, p.Hkv), off = u0 - begin;
+      skip = p.Hkv <= 32 ? __popc(__ballot_sync(0xffffffffu, lane < p.Hkv && (lane + 1) * per_head <= off)) : static_cast<int>(paged_divide(off, per_head));
       base += skip * per_head;
     }
     const int items = p.Hkv * tiles;
@@ -191,7 +198,7 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
         f.b = b;
         f.hk = h;
         f.token = first + t.t0;
-        f.rows = (t.t1 - t.t0) * p.G;
+        f.tokens = t.t1 - t.t0;
         f.p0 = static_cast<int>(t.p0);
         f.j0 = t.j0 + static_cast<int>(a - start);
         f.cnt = static_cast<int>(z - a);

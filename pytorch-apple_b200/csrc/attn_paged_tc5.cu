@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 8) { tc5::tmem_alloc(&tmem_holder, TMEM_COLS); tc5::tmem_relinquish(); }
   pdl_trigger();
   pdl_wait();   // lengths, pages, queries and cache rows come from earlier kernels
-  const PagedWork work = paged_work(smem);   // (no tile has been copied yet)
+  const PagedWork work = paged_work(smem, PAGED_MAX_SEQS);   // (no tile has been copied yet)
   int64_t u0 = 0, u1 = 0, share = 1, ends = 0;
   auto deal = [&]() {   // this block's range of costs (as far as it is known to this warp)
     const int64_t total = paged_prefix<BKV, OV, THREADS>(p, tpt, work, s_total);
@@ -139,12 +139,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       struct Rows { int page, row; };
       const int log_boxes = 7 - log_box, batch = 32 >> log_boxes;   // boxes of a tile, tiles looked up at a time
       auto locate = [&](const PagedPiece& c, int k0) {
-        const int hi = c.p0 + c.rows / p.G;   // keys from here on nobody sees
+        const int hi = c.p0 + c.tokens;   // keys from here on nobody sees
         const int lo = p.window > 0 && c.p0 - p.window + 1 > 0 ? static_cast<int>(c.p0 - p.window + 1) : 0;
         const int k = k0 + (lane >> log_boxes), key = (c.j0 + k) * BKV + (lane & ((1 << log_boxes) - 1)) * box;
         Rows a = {0, -1};
         if (k < c.cnt && key < hi && key + box > lo) {
-          const int i = key / p.page_size;
+          const int i = paged_page(p, key);
           a.row = key - i * p.page_size;
           a.page = __ldg(p.table + c.b * p.table_stride + i);
         }
@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
       for (int f = 0; f < F; ++f) {   // (a thread that has given up still meets the others at the end of every piece)
         const PagedPiece pc = s_piece[f];
-        const int tokens = pc.rows / p.G;
-        const bool row_live = r < pc.rows, warp_live = 32 * quarter < pc.rows;
+        const int rows = pc.tokens * p.G;
+        const bool row_live = r < rows, warp_live = 32 * quarter < rows;
         const int see = row_live ? pc.p0 + r / p.G + 1 : 0;   // keys from here on this row does not see
         const int from = p.window > 0 && see - p.window > 0 ? static_cast<int>(see - p.window) : 0;   // nor those ahead of this one
-        const int hi = pc.p0 + tokens, lo = p.window > 0 && pc.p0 - p.window + 1 > 0 ? static_cast<int>(pc.p0 - p.window + 1) : 0;   // nor any row
+        const int hi = pc.p0 + pc.tokens, lo = p.window > 0 && pc.p0 - p.window + 1 > 0 ? static_cast<int>(pc.p0 - p.window + 1) : 0;   // nor any row
         float m_run = -INFINITY, l_run = 0.f;   // maximum that the row's sums are relative to, sum of the probabilities
 #pragma unroll 1
         for (int k = 0; k < pc.cnt && alive; ++k, ++at, --left) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // A tile that all rows see all of: the probabilities follow the scores at once, relative to the maximum so far; where a row has outgrown it the
           // tile is done again below (S is still there, and nobody has been told of the probabilities).
           bool done = false;
-          if (warp_live && k > 0 && c > 0.f && key0 + BKV <= pc.p0 + 1 && (p.window == 0 || key0 + p.window >= pc.p0 + tokens)) {
+          if (warp_live && k > 0 && c > 0.f && key0 + BKV <= pc.p0 + 1 && (p.window == 0 || key0 + p.window >= pc.p0 + pc.tokens)) {
             const float m_use = m_run == -INFINITY ? 0.f : m_run;
             float sum[4] = {0.f, 0.f, 0.f, 0.f}, mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             uint32_t w[32];
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // Through 4 KB of this warp's (chunk c of row r at c ^ (r & 7)), so that rows leave in whole lines: half a row of results at once, 32 of the
           // fp32 sums at a time
           uint8_t* const own = out_s + warp * 4096;
-          const int live = pc.rows - 32 * quarter < 32 ? pc.rows - 32 * quarter : 32;   // rows of this warp
+          const int live = rows - 32 * quarter < 32 ? rows - 32 * quarter : 32;   // rows of this warp
           const int64_t to = ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
           float* const part = p.acc + (slot + 32 * quarter) * D + g * (D / 2);
 #pragma unroll
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     deal();   // (the tiles lay over it)
   }
   if (threadIdx.x == 0 && !p.whole) {
-    if (head.x) head.x = static_cast<int>((ends - 1) / share) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
+    if (head.x) head.x = static_cast<int>(paged_divide(ends - 1, share)) - cta + 1;   // blocks with pieces of the item that begins here and ends in another
     p.head[cta] = head;
   }
   tc5::tc_fence_before();
