@@ -37,42 +37,52 @@ template <typename T>
 __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant__ AppendParams p) {
   const int hp = p.D >> 4, H = p.Hq + 2 * p.Hkv;   // pairs of packs per head
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  pdl_wait();
-  pdl_trigger();
-  const int64_t row = gid / hp;
-  const int pk = static_cast<int>(gid - row * hp);
-  const int64_t n = row / H;
+  int64_t n;
+  int h, pk;
+  if (gid >> 32 == 0) {   // (a division in 64 bits takes longer than all the rest of the arithmetic)
+    const uint32_t row = static_cast<uint32_t>(gid) / static_cast<uint32_t>(hp), token = row / static_cast<uint32_t>(H);
+    pk = static_cast<int>(static_cast<uint32_t>(gid) - row * hp);
+    h = static_cast<int>(row - token * H);
+    n = token;
+  } else {
+    const int64_t row = gid / hp;
+    pk = static_cast<int>(gid - row * hp);
+    n = row / H;
+    h = static_cast<int>(row - n * H);
+  }
   if (n >= p.N) return;
-  int h = static_cast<int>(row - n * H);
   const int which = h < p.Hq ? 0 : (h < p.Hq + p.Hkv ? 1 : 2);
   if (which == 1) h -= p.Hq;
   if (which == 2) h -= p.Hq + p.Hkv;
+  pdl_wait();
+  pdl_trigger();
+  // all that is read is on its way at once
+  const int64_t slot = which == 0 ? 0 : __ldg(p.slots + n);
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x[which]) + n * p.xs[which][0] + h * p.xs[which][1]);
+  uint4 lo = src[pk], hi = src[pk + hp];
+  if (which != 2 && p.cos_t) {
+    float a[8], b[8], c0[8], s0[8], c1[8], s1[8], o[8];
+    const int64_t t = n * p.D + pk * 8;
+    load_table(p.cos_t, t, p.table_dtype, c0);
+    load_table(p.sin_t, t, p.table_dtype, s0);
+    load_table(p.cos_t, t + (p.D >> 1), p.table_dtype, c1);
+    load_table(p.sin_t, t + (p.D >> 1), p.table_dtype, s1);
+    unpack8<T>(lo, a);
+    unpack8<T>(hi, b);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = a[k] * c0[k] - b[k] * s0[k];
+    lo = pack8<T>(o);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = b[k] * c1[k] + a[k] * s1[k];
+    hi = pack8<T>(o);
+  }
   T* dst;
   if (which == 0) {
     dst = static_cast<T*>(p.q_out) + (n * p.Hq + h) * p.D;
   } else {
-    const int64_t slot = __ldg(p.slots + n);
     if (slot < 0 || slot >= p.n_slots) return;   // a row of padding
-    const int64_t page = slot / p.page_size, r = slot - page * p.page_size;
-    dst = static_cast<T*>(which == 1 ? p.k_pages : p.v_pages) + page * p.ps[0] + h * p.ps[1] + r * p.ps[2];
-  }
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x[which]) + n * p.xs[which][0] + h * p.xs[which][1]);
-  uint4 lo = src[pk], hi = src[pk + hp];
-  if (which != 2 && p.cos_t) {
-    float a[8], b[8], c[8], s[8], o[8];
-    unpack8<T>(lo, a);
-    unpack8<T>(hi, b);
-    const int64_t t = n * p.D + pk * 8;
-    load_table(p.cos_t, t, p.table_dtype, c);
-    load_table(p.sin_t, t, p.table_dtype, s);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = a[k] * c[k] - b[k] * s[k];
-    lo = pack8<T>(o);
-    load_table(p.cos_t, t + (p.D >> 1), p.table_dtype, c);
-    load_table(p.sin_t, t + (p.D >> 1), p.table_dtype, s);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = b[k] * c[k] + a[k] * s[k];
-    hi = pack8<T>(o);
+    const int64_t page = p.n_slots >> 32 == 0 ? static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.page_size) : slot / p.page_size;
+    dst = static_cast<T*>(which == 1 ? p.k_pages : p.v_pages) + page * p.ps[0] + h * p.ps[1] + (slot - page * p.page_size) * p.ps[2];
   }
   reinterpret_cast<uint4*>(dst)[pk] = lo;
   reinterpret_cast<uint4*>(dst)[pk + hp] = hi;
