@@ -19,6 +19,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 // in shared memory, filled by TMA (one box of 16 rows of a page each for K and V, 128-byte swizzle), so that nothing in the loop
 // waits for another warp.  At the end of a piece each warp parks its accumulators in the ring stage that it has just read (which is
 // refilled afterwards; the others are on their way meanwhile) and the block adds them up.
+//
+// us: one sequence of 613 keys 8.4 (launch 2.3, lengths and pages 3, keys 2, sums 1), of 20001 keys 10.9; 64 of 512 to 4352 keys 28.5, of which 17 are the
+// keys at 6.5 TB/s, 4.3 what precedes the first copy and 4.5 the joining kernel.  A warp has 24 KB on its way, 196 KB per SM.
 // ===========================================================================
 constexpr int FEW_WARPS = 8, FEW_KEYS = 16;
 // What an item costs besides its 16-key blocks, in blocks (a round of the eight warps is eight).  us at 4 / 8 / 16 / 28: 64 ragged sequences 29.6 / 29.1 / 28.6 / 28.1,
@@ -356,43 +359,29 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 
 // ===========================================================================
 // Joins the pieces of the item that begins in block blockIdx.x of the kernel before and goes on in the next ones, in the order of the blocks (their
-// sums are the same whoever adds them up): rows blockIdx.y * RPB and up.  A thread per four dims; few pieces: a row to each 256 / (D / 4)th of the block,
-// many: the pieces of one row dealt to them, so that a thread's chain of loads stays short (71 pieces: 17.2 us with a thread per piece and dim).
+// sums are the same whoever adds them up).  Bound by latency: the wait for the kernel before, the item, then its pieces (3 to 5 us).
+//
+// Few rows: row blockIdx.y, a thread per four dims, the pieces dealt to the 256 / (D / 4)ths of the block, so that a thread's chain of loads stays short
+// (71 pieces: 17.2 us with a thread per piece and dim).
 // ===========================================================================
-template <typename T, int D, int ROWS, int RPB>
-__global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int LPR = D / 4, GROUPS = 256 / LPR, BATCH = RPB == 1 ? 10 : 4;   // pieces that a thread has on their way
-  __shared__ __align__(16) float s_acc[GROUPS][D];
-  __shared__ float s_m[GROUPS], s_l[GROUPS];
-  pdl_trigger();
-  pdl_wait();
-  const int4 it = __ldg(p.head + blockIdx.x);
-  const int g = threadIdx.x / LPR, d = threadIdx.x % LPR * 4, r0 = blockIdx.y * RPB;
-  if (it.x == 0 || r0 >= it.w) return;
-  const bool many = RPB == 1 || it.x > 8;
-  const int step = many ? GROUPS : 1;
-  for (int r = many ? r0 : r0 + g; r < min(it.w, r0 + RPB); r += many ? 1 : GROUPS) {   // (uniform where the block meets)
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = many ? g : 0; i0 < it.x; i0 += BATCH * step) {
+struct PagedSum {   // of a thread's four dims: relative to m
+  float m = -INFINITY, l = 0.f;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  // pieces first, first + step, .. of `pieces`, BATCH of them under way; read(piece, ml, acc) fetches one
+  template <int BATCH, typename F> __device__ __forceinline__ void add(int first, int step, int pieces, F&& read) {
+    for (int i0 = first; i0 < pieces; i0 += BATCH * step) {
       float2 ml[BATCH];
       float4 a[BATCH];
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
-        const int at = i0 + i * step;
         ml[i] = make_float2(-INFINITY, 0.f);
         a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < it.x) {
-          const int64_t slot = paged_slot(blockIdx.x + at, at == 0, ROWS) + r;
-          ml[i] = __ldg(p.ml + slot);
-          a[i] = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D + d));
-        }
+        if (i0 + i * step < pieces) read(i0 + i * step, ml[i], a[i]);
       }
       float top = m;
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float c = ex2_approx(m - ref);
+      const float ref = top == -INFINITY ? 0.f : top, c = ex2_approx(m - ref);
       l *= c; acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
@@ -402,30 +391,56 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_cons
       }
       m = top;
     }
-    T* const o = static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D;
-    if (!many) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      *reinterpret_cast<uint2*>(o + d) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-      continue;
-    }
-    *reinterpret_cast<float4*>(&s_acc[g][d]) = acc;
-    if (d == 0) { s_m[g] = m; s_l[g] = l; }
-    __syncthreads();
-    if (threadIdx.x < D) {
-      float top = -INFINITY, sum = 0.f, a = 0.f;
-#pragma unroll
-      for (int e = 0; e < GROUPS; ++e) top = fmaxf(top, s_m[e]);
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int e = 0; e < GROUPS; ++e) {
-        const float f = ex2_approx(s_m[e] - ref);
-        sum += s_l[e] * f;
-        a += s_acc[e][threadIdx.x] * f;
-      }
-      o[threadIdx.x] = from_f32<T>(sum == 0.f ? 0.f : a / sum);   // (a sum that is no number stays one that is none)
-    }
-    __syncthreads();
   }
+  template <typename T> __device__ __forceinline__ uint2 result() const {   // (no key: zeros; a sum that is no number stays none)
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    return make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  }
+};
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ float4 s_acc[GROUPS][LPR];
+  __shared__ float2 s_ml[GROUPS];
+  pdl_trigger();
+  pdl_wait();
+  const int4 it = __ldg(p.head + blockIdx.x);
+  const int g = threadIdx.x / LPR, c = threadIdx.x % LPR, r = blockIdx.y;
+  if (it.x == 0 || r >= it.w) return;
+  PagedSum sum;
+  sum.add<10>(g, GROUPS, it.x, [&](int piece, float2& ml, float4& a) {
+    const int64_t slot = paged_slot(blockIdx.x + piece, piece == 0, ROWS) + r;
+    ml = __ldg(p.ml + slot);
+    a = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D) + c);
+  });
+  s_acc[g][c] = sum.acc;
+  if (c == 0) s_ml[g] = make_float2(sum.m, sum.l);
+  __syncthreads();
+  if (threadIdx.x >= LPR) return;
+  PagedSum all;
+  all.add<GROUPS>(0, 1, GROUPS, [&](int e, float2& ml, float4& a) { ml = s_ml[e]; a = s_acc[e][c]; });
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D + c * 4) = all.result<T>();
+}
+
+// Tiles of 128 rows, whose sums lie as [D / 4][rows] of four each: 1024 / D rows from blockIdx.y * (1024 / D) on, a thread per row and four dims.  Many pieces too
+// (a few tokens over a very long history): eight threads to share them, with a barrier per eighth of the dims, took 46 against 34 us for 128 tokens over 20000
+// keys, 34 against 28 for 21 over 30000; eight pieces on their way instead of four 35 and 29.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_paged_merge_rows_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int LPR = D / 4, RPB = 256 / LPR, ROWS = PAGED_TC5_ROWS;
+  pdl_trigger();
+  pdl_wait();
+  const int4 it = __ldg(p.head + blockIdx.x);
+  const int r = blockIdx.y * RPB + threadIdx.x % RPB, c = threadIdx.x / RPB;
+  if (it.x == 0 || r >= it.w) return;
+  PagedSum sum;
+  sum.add<4>(0, 1, it.x, [&](int piece, float2& ml, float4& a) {
+    const int64_t slot = paged_slot(blockIdx.x + piece, piece == 0, ROWS);
+    ml = __ldg(p.ml + slot + r);
+    a = __ldg(reinterpret_cast<const float4*>(p.acc + slot * D) + c * ROWS + r);
+  });
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + ((static_cast<int64_t>(it.y) + r / p.G) * p.Hq + it.z * p.G + r % p.G) * D + c * 4) = sum.result<T>();
 }
 
 // ===========================================================================
@@ -585,9 +600,9 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
   } else if (!p.whole) {
     B200_DISPATCH_HALF(dtype, T, {
       const auto merge = [&](auto kernel, int groups) { launch_pdl(kernel, dim3(PAGED_CTAS, static_cast<unsigned>(groups)), dim3(256), 0, st, p); };
-      if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8, 1>, 8); else merge(attn_paged_merge_kernel<T, 64, 8, 1>, 8); }
-      else if (rows == 16) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 16, 1>, 16); else merge(attn_paged_merge_kernel<T, 64, 16, 1>, 16); }
-      else { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 128, 8>, 16); else merge(attn_paged_merge_kernel<T, 64, 128, 16>, 8); }
+      if (rows == 8) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 8>, 8); else merge(attn_paged_merge_kernel<T, 64, 8>, 8); }
+      else if (rows == 16) { if (D == 128) merge(attn_paged_merge_kernel<T, 128, 16>, 16); else merge(attn_paged_merge_kernel<T, 64, 16>, 16); }
+      else { if (D == 128) merge(attn_paged_merge_rows_kernel<T, 128>, 16); else merge(attn_paged_merge_rows_kernel<T, 64>, 8); }
     });
   }
   B200_CHECK_LAUNCH("attn_paged");

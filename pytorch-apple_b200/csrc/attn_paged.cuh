@@ -17,7 +17,7 @@ struct PagedParams {
   // partial results (paged_workspace)
   int4* head;                      // [PAGED_CTAS]: {pieces, first token, KV head, rows} of the item that begins in a block and ends in a later one
   float2* ml;                      // [PAGED_CTAS][2][rows]: (maximum in the log2 domain, sum)
-  float* acc;                      // [PAGED_CTAS][2][rows][D]
+  float* acc;                      // [PAGED_CTAS][2][rows][D], with tiles of 128 rows [PAGED_CTAS][2][D / 4][rows][4]
 };
 
 constexpr int PAGED_CTAS = 148;        // blocks that share the work (fixed, so that the workspace does not depend on the device)

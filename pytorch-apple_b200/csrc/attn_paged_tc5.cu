@@ -29,7 +29,9 @@ namespace {
 constexpr int BKV = 128;
 constexpr int PANEL = 128 * 128;               // [128 rows][128 bytes]: 64 columns of an operand tile
 constexpr int THREADS = 352;
-constexpr int OV = 2;                          // what an item costs besides its tiles, in tiles (1, 2, 3: 36.5, 34.8, 34.3 us for a chunk, 29.3, 27.3, 27.9 for a mixed step)
+// What an item costs besides its tiles, in tiles.  us at 2 / 3 / 4 / 5, a microsecond more than now each: 512 tokens over 4608 keys 32.1 / 31.0 / 31.4 / 31.6, a
+// prompt of 2048 37.1 / 35.4 / 35.2 / 36.6, 32 sequences of which two are prompts 26.8 / 26.7 / 28.2 / 28.5.
+constexpr int OV = 3;
 constexpr int MIN_SHARE = 2;                   // tiles (and OVs) of a block at least
 constexpr float LOG2E_F = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.f;
@@ -408,12 +410,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const int64_t slot = paged_slot(cta, pc.flags & 1, PAGED_TC5_ROWS);
           if (!whole && g == 0 && row_live) p.ml[slot + r] = make_float2(m_all, l_all);
-          // Through 4 KB of this warp's (chunk c of row r at c ^ (r & 7)), so that rows leave in whole lines: half a row of results at once, 32 of the
-          // fp32 sums at a time
+          // Sums go as [D / 4][rows] of four each, so that a warp's rows make whole lines; results through 4 KB of the warp's (chunk c of row r at c ^ (r & 7))
           uint8_t* const own = out_s + warp * 4096;
           const int live = rows - 32 * quarter < 32 ? rows - 32 * quarter : 32;   // rows of this warp
           const int64_t to = ((static_cast<int64_t>(pc.token) + r / p.G) * p.Hq + pc.hk * p.G + r % p.G) * D + g * (D / 2);
-          float* const part = p.acc + (slot + 32 * quarter) * D + g * (D / 2);
+          float4* const part = reinterpret_cast<float4*>(p.acc + slot * D) + r;
 #pragma unroll
           for (int q = 0; q < D / 2; q += 32) {
             float t0[32], t1[32];
@@ -426,18 +427,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 *reinterpret_cast<uint4*>(own + lane * 128 + (((q / 8 + e) ^ (r & 7)) << 4)) = pack8<T>(*reinterpret_cast<float(*)[8]>(&t0[8 * e]));
-            } else {
-              __syncwarp();   // (the 32 before have been read)
+            } else if (row_live) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(own + lane * 128 + ((e ^ (r & 7)) << 4)) = *reinterpret_cast<float4*>(&t0[4 * e]);
-              __syncwarp();
-#pragma unroll
-              for (int it = 0; it < 8; ++it) {
-                const int row = it * 4 + lane / 8, ch = lane % 8;
-                if (row < live)
-                  *reinterpret_cast<float4*>(part + static_cast<int64_t>(row) * D + q + ch * 4) = *reinterpret_cast<const float4*>(own + row * 128 + ((ch ^ (row & 7)) << 4));
-              }
+              for (int e = 0; e < 8; ++e) part[((g * (D / 2) + q) / 4 + e) * PAGED_TC5_ROWS] = *reinterpret_cast<float4*>(&t0[4 * e]);
             }
           }
           tc5::tc_fence_before();

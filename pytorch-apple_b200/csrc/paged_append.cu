@@ -4,7 +4,8 @@
 // the unfused graph that it replaces does; this one replaces nothing, and the errors would be twice as large.)
 //
 // One thread per 8 dims of both halves of a (token, head): everything it reads it has read before it writes, so queries may be
-// rotated in place.  Bound by launch latency for a decode step, by memory for a long prompt.
+// rotated in place.  64 tokens of 12 + 2 + 2 heads of 128: 2.0 us, all of it launch and one round trip to memory (0.1 us of bytes); 2048 tokens in fp16 with
+// fp32 tables: 4.4 us for 18.9 MB (2.9 us at the 6.46 TB/s of a copy), where 64-bit divisions and a slot looked up ahead of the loads made 4.8.
 #include "common.cuh"
 
 namespace b200 {

@@ -11,11 +11,15 @@
 // themselves, never on weights.
 //
 // A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once (a bulk copy per warp)
-// and then goes through a few times: for the maximum; for the sum of the weights where it is needed (about 20 instructions a token: that, and not the memory, is
-// what most of the time goes into); for the tokens that are large enough to matter. How large that is the maxima of the threads' own
-// tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are sorted by one CTA, which mostly finds everything
-// that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or weights in 16 intervals of z, then in 16 parts
-// of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is drawn from by sums over ranges.
+// and then goes through a few times: for the maximum; for the sum of the weights where it is needed; for the tokens that are large enough to matter. How
+// large that is the maxima of the threads' own tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are
+// sorted by one CTA, which mostly finds everything that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or
+// weights in 16 intervals of z, then in 16 parts of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is
+// drawn from by sums over ranges.
+//
+// 64 rows of 151 936 tokens in bf16 (19.4 MB, 3 us of memory), us: greedy 10, top-k 50 14, top-k 400 22, no filter 16, top-p 0.9 21.5, min-p 0.05 11, flat rows
+// that keep tens of thousands 115; one row 5, 11, 14, 8, 15, 7.5, 55.  Not the memory is the bound: launch and copy are 4.5 of it, every meeting of a row's CTAs is
+// 1 (there are two to six), the sum of the weights 6 (76 000 tokens per SM, an exponential and about 18 instructions each), sorting and the draw 2 to 8.
 #include <type_traits>
 
 #include "common.cuh"
