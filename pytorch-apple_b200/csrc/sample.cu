@@ -412,7 +412,7 @@ template <bool TOP> __device__ u64 row_reduce(u64 v, Shared& sh, int ctas, int& 
 
 // list[0 .. n) in descending order.  All threads; begins and ends with a barrier; list[n] up to the next multiple of 256 may be overwritten.
 // Every warp sorts 32 elements at a time by shuffles, then four runs at a time become one: an element's place is its own plus those that the other three runs
-// have ahead of it, looked for by halving.  Meanwhile element i lies at i ^ (i / 16 % 16): steps by 16 and more would all meet in one bank.  (us for 128 and 512 elements: 0.9 and 1.3, where steps over all of the list took 2.9 and 4.6.)
+// have ahead of it, looked for by halving.  Meanwhile element i lies at i ^ (i / 16 % 16): steps by 16 and more would all meet in one bank.  (us for 110 and 490 elements: 1.0 and 2.7, where steps over all of the list took 2.9 and 4.6.)
 template <int E> __device__ __forceinline__ void sort_elements(u64* list, int n) {
   const int i = threadIdx.x, lane = i & 31;
   const auto place = [](int at) { return at ^ ((at >> 4) & 15); };
