@@ -219,7 +219,7 @@ __device__ int64_t paged_pieces(const PagedParams& p, int tpt, const PagedWork& 
       if (count > PAGED_MAX_PIECES) {   // go on behind the last one taken
         const unsigned last = __ballot_sync(0xffffffffu, taken && at == PAGED_MAX_PIECES - 1);
         count = PAGED_MAX_PIECES;
-        return last ? __shfl_sync(0xffffffffu, p.whole ? start + 1 : z, __ffs(last) - 1) : base;   // (none of this round was taken: they begin at base or later)
+        return last ? __shfl_sync(0xffffffffu, p.whole ? start + 1 : z, __ffs(last) - 1) : base;   // (none of these 32 was taken: they begin at base or later)
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
     }

@@ -222,7 +222,7 @@ struct Shared {
   uint32_t bin_count[SW][32], told_count[2][MAX_CTAS][32];
   u64 cut_last;            // from the list: key << 32 | index of the last token kept
   int listed;
-  int pick[2], verdict;
+  int pick[2], settled;
   __align__(8) uint64_t full[SW];
 };
 
@@ -921,8 +921,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       }
       if (static_cast<int>(threadIdx.x) < ctas) {
         const int v = all ? 1 : 0;
-        if (ctas == 1) sh.verdict = v;
-        else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.verdict), threadIdx.x)), "r"(v) : "memory");
+        if (ctas == 1) sh.settled = v;
+        else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc5::map_to_rank(tc5::smem_addr(&sh.settled), threadIdx.x)), "r"(v) : "memory");
       }
       __syncthreads();
       if (threadIdx.x == 0) sh.listed = 0;
@@ -930,7 +930,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
       if (all) finish(n);
     }
     if (ctas > 1) tc5::cluster_sync(); else __syncthreads();
-    if (sh.verdict) return;
+    if (sh.settled) return;
   }
 
   // ---- the long way ----

@@ -279,6 +279,8 @@ CASES = {
     "draft_4": dict(seqs=[(4, 300), (4, 4), (3, 700), (1, 50), (4, 129)], heads=(16, 8), dim=64, page=32, dtype=HF),
     "draft_2_window": dict(seqs=[(2, 300), (2, 65), (1, 700), (2, 2)], window=64),
     "chunk": dict(seqs=[(100, 900)]),
+    "chunk_long_history": dict(seqs=[(9, 9000)]),   # some seventy pieces to join
+    "chunk_long_history_d64": dict(seqs=[(30, 6000), (1, 50), (2, 3000)], heads=(14, 2), dim=64, dtype=HF),
     "chunk_odd": dict(seqs=[(131, 131), (1, 900), (77, 1300), (21, 21), (22, 150), (0, 9), (63, 64)], page=48),
     "chunk_window": dict(seqs=[(131, 531), (1, 900), (300, 300), (50, 2000)], window=77),
     "chunk_window_fp16_d64": dict(seqs=[(257, 600), (1, 900), (40, 41)], window=128, heads=(14, 2), dim=64, dtype=HF, page=256),
@@ -546,6 +548,32 @@ def test_draw(native_lib, dtype, cols):
     check_draw(x, u, top_k=np.full(rows, cols // 2 + 1), top_p=p)
     check_draw(x, u, temperature=np.full(rows, 5.0), top_p=np.full(rows, 0.95))   # half of the vocabulary and more
     check_draw(x, u, temperature=np.zeros(rows))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cols", [(BF, 5000), (F32, 5000), (BF, 151936), (F32, 60000)])
+def test_draw_with_lists_around_every_size(native_lib, dtype, cols):
+    """Lists that fill a warp, a run, a round of the CTA's threads, or a token more: in one CTA per row and in several."""
+    k = [1, 2, 31, 32, 33, 63, 65, 127, 128, 129, 255, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049]
+    rows = len(k)
+    x = logits_like(rows, cols, dtype, 7 + cols)
+    u = np.random.default_rng(cols).random(rows)
+    check_draw(x, u, top_k=np.array(k))
+    check_draw(x, u, top_k=np.array(k), temperature=np.full(rows, 1.7), top_p=np.full(rows, 0.97))
+    check_draw(x.repeat(7, 1), np.tile(u, 7), top_k=np.tile(k, 7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_draw_from_the_longest_row(native_lib, dtype):
+    """4194304 like tokens and a larger one.  Token n for u (1 + N w) = 1 + (n + 1 - ..) w: where u falls among equal weights w does not depend on w's error
+    (2^-22) but by its share of one token, 1e-7."""
+    x = torch.zeros(2, 1 << 22, dtype=dtype)
+    x[:, 1234567] = 10.0
+    u, hot = np.array([0.1, 0.77]), np.full(2, 100.0)
+    check_draw(x, u, temperature=hot)
+    check_draw(x, u, temperature=hot, top_k=np.array([1000000, 3]))
+    check_draw(x, u, temperature=hot, min_p=np.array([0.5, 0.95]))
 
 
 @pytest.mark.gpu
