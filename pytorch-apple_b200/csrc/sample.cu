@@ -43,6 +43,7 @@ constexpr int CAP = 2048;                    // tokens of a list
 constexpr int BIN_BYTES = SW * BINS * 32 * 8;   // a counter per warp, bin and lane; later the lists
 constexpr int STAGE_BYTES = 152 * 1024;      // of a CTA's columns at most
 static_assert(BIN_BYTES >= 3 * CAP * 8, "the lists lie over the counters");
+static_assert(MAX_COLS / (MAX_CTAS * ST) <= 1024, "a lane's columns, where a row has all the CTAs that it can have (it has if it is not staged): Weigher::Sum");
 
 struct SampleParams {
   const void* logits;
@@ -662,6 +663,8 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
     uint32_t first = 0, end = LAST_PLACE, above = 0;   // places that are looked at, tokens before them
     u64 above_mass = 0;
     double limit = 0.;
+    const float at_least = cut == 0 ? -INFINITY : value_of(cut);   // (what top-k has left)
+    few = few && cut != 0;
 #pragma unroll 1
     for (int shift = PLACE_BITS - 4; ; shift = shift >= 4 ? shift - 4 : 0) {
       u64* const own = bins + warp * BINS * 32 + lane;
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
         }
         weight.each_set(close, z, [&](float v, int) { own[((place(weight.difference(v)) - first) >> shift) * 32] += (1ull << 52) + weight.large(v); });
       };
-      const float floor = end == LAST_PLACE ? -INFINITY : lowest(end);
+      const float floor = end == LAST_PLACE ? at_least : fmaxf(at_least, lowest(end));
       if (few) row.from(floor, count_in); else row.eights([&](const float (&z)[8], float top_, int c) {
         if (top_ >= floor) count_in(z, c);
       });

@@ -566,8 +566,8 @@ def test_draw_with_lists_around_every_size(native_lib, dtype, cols):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_draw_from_the_longest_row(native_lib, dtype):
-    """4194304 like tokens and a larger one.  Token n for u (1 + N w) = 1 + (n + 1 - ..) w: where u falls among equal weights w does not depend on w's error
-    (2^-22) but by its share of one token, 1e-7."""
+    """4194304 - 1 like tokens of weight w and a larger one of weight 1: u times the sum lies (u N w + u - 1) / w tokens behind the larger one, which an error of
+    2^-22 in w moves by 1e-7 of a token."""
     x = torch.zeros(2, 1 << 22, dtype=dtype)
     x[:, 1234567] = 10.0
     u, hot = np.array([0.1, 0.77]), np.full(2, 100.0)
