@@ -10,15 +10,15 @@
 // fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a rare token is wide).  Thresholds are found on the logits
 // themselves, never on weights.
 //
-// A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once (a bulk copy per warp)
-// and then goes through a few times: for the maximum; for the sum of the weights where it is needed; for the tokens that are large enough to matter. How
+// A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once where it fits (a bulk copy
+// per warp) and then goes through a few times: for the maximum; for the sum of the weights where it is needed; for the tokens that are large enough to matter. How
 // large that is the maxima of the threads' own tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are
 // sorted by one CTA, which mostly finds everything that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or
 // weights in 16 intervals of z, then in 16 parts of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is
 // drawn from by sums over ranges.
 //
-// 64 rows of 151 936 tokens in bf16 (19.4 MB, 3 us of memory), us: greedy 10, top-k 50 14, top-k 400 22, no filter 16, top-p 0.9 21.5, min-p 0.05 11, flat rows
-// that keep tens of thousands 115; one row 5, 11, 14, 8, 15, 7.5, 55.  Not the memory is the bound: launch and copy are 4.5 of it, every meeting of a row's CTAs is
+// 64 rows of 151 936 tokens in bf16 (19.4 MB, 3 us of memory), us: greedy 7, top-k 50 14, top-k 400 22, no filter 16, top-p 0.9 22, min-p 0.05 11, flat rows
+// that keep tens of thousands 115; one row 4, 11, 15, 8, 15, 7.5, 55; 200 rows 17, 30, 53, 45, 57.  Not the memory is the bound: launch and copy are 4.5 of it, every meeting of a row's CTAs is
 // 1 (there are two to six), the sum of the weights 6 (76 000 tokens per SM, an exponential and about 18 instructions each), sorting and the draw 2 to 8.
 #include <type_traits>
 
@@ -43,7 +43,7 @@ constexpr int CAP = 2048;                    // tokens of a list
 constexpr int BIN_BYTES = SW * BINS * 32 * 8;   // a counter per warp, bin and lane; later the lists
 constexpr int STAGE_BYTES = 152 * 1024;      // of a CTA's columns at most
 static_assert(BIN_BYTES >= 3 * CAP * 8, "the lists lie over the counters");
-static_assert(MAX_COLS / (MAX_CTAS * ST) <= 1024, "a lane's columns, where a row has all the CTAs that it can have (it has if it is not staged): Weigher::Sum");
+static_assert(MAX_COLS / (MAX_CTAS * ST) <= 1024, "a lane's columns: Weigher::Sum");
 
 struct SampleParams {
   const void* logits;
@@ -273,28 +273,33 @@ template <typename T> struct Row {
     const auto of = [](const float (&z)[8]) {
       return max_nan(max_nan(max_nan(z[0], z[1]), max_nan(z[2], z[3])), max_nan(max_nan(z[4], z[5]), max_nan(z[6], z[7])));
     };
-    if (!infinite && (copied > begin || vec)) {   // four loads under way
+    if (!infinite && (copied > begin || vec)) {   // 128, then 64 bytes of a thread under way
       const T* const at = copied > begin ? copy - begin : x;
       const int all = min(to, copied > begin ? copied : end);
-      for (; c + 3 * 256 + 8 <= all; c += 4 * 256) {
-        if constexpr (sizeof(T) == 2) {
-          uint4 w[4];
+      const auto some = [&](auto count) {
+        constexpr int N = decltype(count)::value;
+        for (; c + (N - 1) * 256 + 8 <= all; c += N * 256) {
+          if constexpr (sizeof(T) == 2) {
+            uint4 w[N];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(at + c + 256 * i);
+            for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(at + c + 256 * i);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float a, b;
-            unpack2<T>(max2<T>(max2<T>(w[i].x, w[i].y), max2<T>(w[i].z, w[i].w)), a, b);
-            f(max_nan(a, b), c + 256 * i);
+            for (int i = 0; i < N; ++i) {
+              float a, b;
+              unpack2<T>(max2<T>(max2<T>(w[i].x, w[i].y), max2<T>(w[i].z, w[i].w)), a, b);
+              f(max_nan(a, b), c + 256 * i);
+            }
+          } else {
+            float z[N][8];
+#pragma unroll
+            for (int i = 0; i < N; ++i) unpack(at + c + 256 * i, z[i]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) f(of(z[i]), c + 256 * i);
           }
-        } else {
-          float z[4][8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) unpack(at + c + 256 * i, z[i]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f(of(z[i]), c + 256 * i);
         }
-      }
+      };
+      some(std::integral_constant<int, 16 / sizeof(T)>());
+      some(std::integral_constant<int, 8 / sizeof(T)>());
     }
     for (; c < to; c += 256) {
       float z[8];
@@ -569,8 +574,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   if (!(T_ > 0.f) || none) {              // greedy: the first of the largest
     u64 at = 0;
     if (!none) {
-      row.each([&](float z, int c) {
-        if (z == m && at == 0) at = static_cast<uint32_t>(~c);
+      row.from(m, [&](const float (&z)[8], int c) {
+#pragma unroll
+        for (int e = 7; e >= 0; --e)
+          if (z[e] == m && static_cast<uint32_t>(~(c + e)) > at) at = static_cast<uint32_t>(~(c + e));
       });
       at = row_reduce<true>(at, sh, ctas, turn);
     }
@@ -904,7 +911,10 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   };
 
   // ---- the short way: the largest tokens, as many as k or as a nucleus mostly has ----
-  const bool few_k = restricted_by_k && 2 * k <= threads && k <= CAP / 2;
+  // (k of the threads have one of the tokens that reach the k-th largest maximum, so there are threads ln(threads / (threads - k)) of them where tokens come as they
+  // like: 200 rows with top-k 400, one CTA each, 53 us this way and 101 the other)
+  const bool few_k = restricted_by_k && k < threads && k <= CAP / 2 &&
+                     static_cast<float>(threads) * logf(static_cast<float>(threads) / static_cast<float>(threads - k)) <= 0.7f * CAP;
   if (few_k || (tp < 1.f && !restricted_by_k)) {
     if (!few_k) {
       typename Weigher<T>::Sum s;
@@ -1047,16 +1057,47 @@ __global__ void __launch_bounds__(ST, 1) sample_rows_kernel(const __grid_constan
   }
 }
 
-template <typename T> int launch_sample(const SampleParams& p, int64_t rows, int ctas, cudaStream_t st) {
+// Clusters of 2, 4 and 8 CTAs that a device runs at once (SMs come in groups that a cluster cannot leave: 37 of 4 do not all fit on 148)
+struct SampleWave {
+  int rows[4] = {0, 0, 0, 0};   // [log2 of the CTAs]; 0: not known yet
+};
+
+template <typename T> int launch_sample(SampleParams p, int64_t rows, cudaStream_t st) {
   constexpr int smem = BIN_BYTES + STAGE_BYTES;
-  static PerDevice<bool> configured_on;
-  bool* configured = configured_on.slot();
-  if (!configured) B200_FAIL(B200_ELAUNCH, "sample_rows_kernel: no current device");
-  if (!*configured) {
+  static PerDevice<SampleWave> wave_on;
+  SampleWave* const wave = wave_on.slot();
+  if (!wave) B200_FAIL(B200_ELAUNCH, "sample_rows_kernel: no current device");
+  if (!wave->rows[0]) {
     const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) B200_FAIL(B200_ELAUNCH, "sample_rows_kernel attribute: %s", cudaGetErrorString(e));
-    *configured = true;
+    for (int i = 3; i > 0; --i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << i, 64);
+      cfg.blockDim = dim3(ST);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 1u << i;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&wave->rows[i], sample_rows_kernel<T>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        wave->rows[i] = 0;
+      }
+    }
+    wave->rows[0] = 148;
   }
+  // As many CTAs per row as all run at once; rows of a CTA that do not fit into its shared memory are read anew in each pass, which is less than a second
+  // wave takes (us: 64 rows in fp32 with top-k 50 19 against 29, 128 in bf16 without filters 25 against 30).
+  const auto seg_of = [&](int ctas) { return ceil_div(ceil_div(static_cast<int64_t>(p.cols), ctas), 256) * 256; };
+  int log_ctas = 0;
+  while (log_ctas < 3 && p.cols > (2048 << log_ctas) && rows <= wave->rows[log_ctas + 1]) ++log_ctas;
+  // (sums of the weights stay small enough for a lane's counters: Weigher::Sum)
+  while (log_ctas < 3 && seg_of(1 << log_ctas) > 1024 * ST) ++log_ctas;
+  const int ctas = 1 << log_ctas;
+  p.seg = static_cast<int>(seg_of(ctas));
+  p.staged = p.seg * sizeof(T) <= STAGE_BYTES ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(rows));
   cfg.blockDim = dim3(ST);
@@ -1103,13 +1144,6 @@ extern "C" int b200_sample_rows(const void* logits, int64_t* out, int64_t rows, 
   SampleParams p;
   p.logits = logits; p.out = out; p.row_stride = row_stride; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.uniform = uniform; p.cols = static_cast<int>(cols);
-  // as many CTAs per row as there are SMs for, at least as many as hold the row in shared memory (longer rows are read anew in each pass)
-  const int64_t esize = dtype == B200_F32 ? 4 : 2;
-  const auto seg_of = [&](int ctas) { return ceil_div(ceil_div(cols, ctas), 256) * 256; };
-  int ctas = 1;
-  while (ctas < MAX_CTAS && cols > 2048 * ctas && (2 * ctas * rows <= 148 || seg_of(ctas) * esize > STAGE_BYTES)) ctas *= 2;
-  p.seg = static_cast<int>(seg_of(ctas));
-  p.staged = p.seg * esize <= STAGE_BYTES ? 1 : 0;
-  B200_DISPATCH_FLOAT(dtype, T, { return launch_sample<T>(p, rows, ctas, static_cast<cudaStream_t>(stream)); });
+  B200_DISPATCH_FLOAT(dtype, T, { return launch_sample<T>(p, rows, static_cast<cudaStream_t>(stream)); });
   return B200_OK;
 }
