@@ -448,7 +448,8 @@ int b200_paged_append(const b200_paged_append_args* args, void* stream);
 
 /* Attention of every sequence's new tokens over its pages (their keys and values appended before): beside
  * b200_attn_decode and b200_attn_prefill, for decoding sequences, chunks of prompts and both in one batch.
- *   sequence b: tokens q_start[b] .. q_start[b+1] - 1, at most max_q; kv_len[b] keys with them; key j lies in page
+ *   sequence b: tokens q_start[b] .. q_start[b+1] - 1, at most max_q (it chooses the kernel: with a bound that is too small the call is right, but
+ *   slower; 0 says that there are no tokens at all: nothing is launched and out is left as it was); kv_len[b] keys with them; key j lies in page
  *   page_table[b * table_stride + j / page_size].  Token i of T sees the keys up to its own position p = kv_len[b] - T + i, with
  *   window > 0 only the last `window` of them (p included).  A token without any key gives zeros.
  *   q: element strides (token, head); out [n_tokens, Hq, D]; rows behind the last sequence are left as they were.

@@ -108,7 +108,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return one();
   const Tensor &q = *tensor(a[2]), &kp = *tensor(a[3]), &vp = *tensor(a[4]), &start = *tensor(a[5]), &len = *tensor(a[6]), &table = *tensor(a[7]);
   const Tensor* given = tensor(a[11]);
-  const int64_t max_q = PyLong_AsLongLong(a[8]), window = PyLong_AsLongLong(a[10]);
+  int64_t max_q = PyLong_AsLongLong(a[8]);
+  const int64_t window = PyLong_AsLongLong(a[10]);
   const double scale = PyFloat_AsDouble(a[9]);
   if (PyErr_Occurred()) return nullptr;
   auto* const call = entry<int(const b200_attn_paged_args*, void*)>(a[0], q);
@@ -120,6 +121,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::OptionalDeviceGuard guard(q.is_cuda() ? std::optional<c10::Device>(q.device()) : std::nullopt);
   const Tensor out = given ? *given : made(q, q.sizes(), q.scalar_type());
   if (N > 0 && B > 0) {
+    // (0 tells the library that no sequence has a token, and it launches nothing: an output made here would come back as it was allocated)
+    if (max_q == 0) max_q = 1;
     // from the allocator on every call: a captured graph gets a workspace of its own, calls on other streams theirs
     const int64_t need = size(max_q, static_cast<int>(Hq), static_cast<int>(kp.size(1)), static_cast<int>(D));
     const Tensor space = made(q, {need}, at::kByte);

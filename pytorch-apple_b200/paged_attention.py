@@ -47,7 +47,8 @@ def paged_attention(q, k_pages, v_pages, q_start, kv_len, page_table, max_q, sca
     """Attention of each sequence's new tokens over its pages; returns ``[N, Hq, D]``.
 
     ``q`` ``[N, Hq, D]`` (any strides over tokens and heads); ``q_start`` int32 ``[B + 1]``: sequence b has the tokens ``q_start[b]`` up to
-    ``q_start[b + 1]``, at most ``max_q`` of them; ``kv_len`` int32 ``[B]``: its keys, the new tokens' among them; ``page_table`` int32 ``[B, n]``: its pages.
+    ``q_start[b + 1]``, at most ``max_q`` of them (it chooses the kernel: with a bound that is too small the call is right, but slower);
+    ``kv_len`` int32 ``[B]``: its keys, the new tokens' among them; ``page_table`` int32 ``[B, n]``: its pages.
     A token sees the keys up to its own, with ``window`` > 0 the last ``window`` of them.  ``scale``: 1 / sqrt(D) unless given.  Rows of ``out`` behind
     the last sequence are left as they were (as they come, where ``out`` is made here)."""
     got = native.torch_calls().paged_attention(native.entry("b200_attn_paged"), native.entry("b200_attn_paged_workspace_bytes"), q, k_pages, v_pages, q_start, kv_len,
