@@ -71,19 +71,26 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
-    """``csrc/torch_calls.cpp`` against the headers of the torch that is installed."""
-    src = CSRC / "torch_calls.cpp"
-    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime > max(src.stat().st_mtime, (INCLUDE / "b200nn.h").stat().st_mtime):
-        return CALLS_PATH
+    """``csrc/torch_calls.cpp`` against the headers of the torch that is installed.  Built again when its source, the library's header, the
+    torch or the interpreter is another one than it was built with."""
     import sysconfig
 
     import torch
 
+    from cuda_runtime import native
+
+    src = CSRC / "torch_calls.cpp"
+    built_for = native.torch_calls_built_for()
+    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime > max(src.stat().st_mtime, (INCLUDE / "b200nn.h").stat().st_mtime) and \
+            built_for.encode() in CALLS_PATH.read_bytes():
+        return CALLS_PATH
     base = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parents[1]
     includes = [base / "include", base / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], cuda / "include"]
+    CALLS_PATH.unlink(missing_ok=True)   # (where it does not compile, what was there is not to be loaded)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{p}" for p in includes), str(src), "-o", str(CALLS_PATH), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           f'-DB200_BUILT_FOR="{built_for}"', *(f"-I{p}" for p in includes), str(src), "-o", str(CALLS_PATH), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -182,4 +182,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200_torch_calls", nullptr, -1, me
 
 }  // namespace
 
+// Looked for in the file before it is loaded: torch's and the interpreter's versions
+extern "C" __attribute__((used, visibility("default"))) const char b200_torch_calls_built_for[] = B200_BUILT_FOR;
+
 PyMODINIT_FUNC PyInit_b200_torch_calls(void) { return PyModule_Create(&module); }

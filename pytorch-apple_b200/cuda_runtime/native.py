@@ -162,6 +162,15 @@ _calls = None
 _entries: dict = {}   # name -> (library, address, what must stay alive for it)
 
 
+def torch_calls_built_for() -> str:
+    """What a ``b200_torch_calls`` that can be loaded into this process carries in it (its code depends on the layout of torch's classes)."""
+    import sys
+
+    import torch
+
+    return f"b200_torch_calls for torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
 def torch_calls():
     """The module ``b200_torch_calls`` (csrc/torch_calls.cpp): entry points called with torch tensors."""
     global _calls
@@ -174,6 +183,8 @@ def torch_calls():
         path = Path(__file__).resolve().parent / "b200_torch_calls.so"
         if not path.exists():
             raise RuntimeError(f"{path} not found: build it with `python build_native.py`; there is no fallback path without it")
+        if torch_calls_built_for().encode() not in path.read_bytes():
+            raise RuntimeError(f"{path} was built for another torch than {torch.__version__}: build it again with `python build_native.py`")
         loader = importlib.machinery.ExtensionFileLoader("b200_torch_calls", str(path))
         _calls = importlib.util.module_from_spec(importlib.util.spec_from_loader("b200_torch_calls", loader))
         loader.exec_module(_calls)
