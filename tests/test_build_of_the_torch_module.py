@@ -47,3 +47,16 @@ def test_a_module_for_another_torch_is_not_loaded(monkeypatch):
         native.torch_calls()
     monkeypatch.undo()
     assert native.torch_calls().sample_rows
+
+
+@pytest.mark.parametrize("trouble", [RuntimeError("g++ failed for torch_calls.cpp"), ImportError("No module named 'torch'"), FileNotFoundError("g++")])
+def test_the_library_is_built_where_the_module_cannot_be(monkeypatch, trouble):
+    """The C ABI needs neither torch nor a host compiler for its headers; the calls with torch tensors say that their module is missing."""
+    build_native.build()   # (nothing is compiled below)
+
+    def fail(*a, **kw):
+        raise trouble
+
+    monkeypatch.setattr(build_native, "build_torch_calls", fail)
+    with pytest.warns(UserWarning, match="b200_torch_calls.so"):
+        assert build_native.build() == build_native.LIB_PATH
