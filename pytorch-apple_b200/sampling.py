@@ -38,17 +38,21 @@ class Sampler:
         self.seed = seed
         self._generators: dict[torch.device, torch.Generator] = {}
         self._on: dict[tuple, dict] = {}
+        self._last: tuple = (None, {})   # the rows that were drawn for last, and their settings
 
     def _rows(self, rows: int, device) -> dict:
-        key = (rows, device)
-        if key not in self._on:
-            made = {}
+        last = self._last   # (one thread's own: another may be drawing for another batch)
+        if last[0] != (rows, device):
             for name, t in self.settings.items():
                 if t.dim() > 1 or (t.dim() == 1 and t.shape[0] != rows):
                     raise ValueError(f"Sampler: {name} must be one number or one for each of the {rows} rows, got shape {tuple(t.shape)}")
-                made[name] = t.expand(rows).contiguous().to(device)
-            self._on[key] = made
-        return self._on[key]
+            # Kept for the next power of two and cut: a batch that grows and shrinks leaves no more than twice the largest behind.  (Nothing is given
+            # back, so no stream can still be reading what another one is given.)
+            room = rows if any(t.dim() for t in self.settings.values()) else 1 << max(rows - 1, 0).bit_length()
+            if (room, device) not in self._on:
+                self._on[room, device] = {name: t.expand(room).contiguous().to(device) for name, t in self.settings.items()}
+            last = self._last = (rows, device), {name: t[:rows] for name, t in self._on[room, device].items()}
+        return last[1]
 
     def __call__(self, logits):
         """Token ids ``[rows]`` for logits ``[rows, cols]``."""

@@ -43,3 +43,46 @@ def test_attention_whose_bound_on_the_tokens_is_none(native_lib, seqs):
     got = paged_attention(**{**a, "max_q": 0}, out=out)
     check_attention(got, a, start, table, seqs)
     assert (got[start[-1]:] == 7).all()
+
+
+# ------------------------------------------------------------------ Sampler
+def _held(x):
+    """Elements of the tensors in an object's attributes, views counted as if they were not."""
+    if isinstance(x, torch.Tensor):
+        return x.numel()
+    if isinstance(x, dict):
+        return sum(_held(v) for v in x.values())
+    return sum(_held(v) for v in x) if isinstance(x, (tuple, list)) else _held(vars(x)) if hasattr(x, "settings") else 0
+
+
+def test_sampler_does_not_keep_a_set_of_settings_for_every_batch_size(fake_native):
+    """A server's batch grows and shrinks: what a sampler holds is bounded by the largest, and every batch draws as a sampler of its own would."""
+    from sampling import Sampler
+
+    sizes = [*range(1, 65), *range(64, 0, -1), 7, 200, 7]
+    logits = gen((200, 30), torch.float32, 1)
+    sampler = Sampler(temperature=0.9, top_k=7, top_p=0.8, min_p=0.01, seed=3)
+    g = torch.Generator().manual_seed(3)
+    from sampling import sample_rows
+
+    for rows in sizes:
+        u = torch.rand(rows, generator=g)
+        full = lambda v, dt=torch.float32: torch.full((rows,), v, dtype=dt)
+        want = sample_rows(logits[:rows], u, full(0.9), full(7, torch.int32), full(0.8), full(0.01))
+        assert torch.equal(sampler(logits[:rows]), want)
+    # four settings of one number, for the powers of two up to 256, and views of the last batch
+    assert _held(sampler) <= 4 * (1 + 511 + 200)
+
+
+def test_sampler_of_one_setting_per_row_takes_batches_of_that_size_alone(fake_native):
+    from sampling import Sampler
+
+    sampler = Sampler(temperature=[0.5, 1.0, 0.0])
+    logits = gen((4, 30), torch.float32, 2)
+    assert sampler(logits[:3])[2] == logits[2].argmax()
+    for rows in (1, 2, 4):
+        with pytest.raises(ValueError, match="one for each"):
+            sampler(logits[:rows])
+    assert sampler(logits[:3])[2] == logits[2].argmax()
+    assert Sampler(temperature=[0.0])(logits[:1])[0] == logits[0].argmax()
+    assert Sampler()(logits[:0]).shape == (0,)
