@@ -174,6 +174,8 @@ class QwenSession:
         (``sampling.Sampler``) draws the token instead of taking the arg-max."""
         B, T = self.batch, self.prompt_len
         n = T if prompt_len is None else int(prompt_len)
+        if sampler is not None and not 1 <= n <= T:
+            raise ValueError(f"a token is drawn behind a prompt of 1 to {T} tokens, not of {n}")
         ids = np.ascontiguousarray(input_ids, dtype=np.int64).reshape(B, T)
         feed = {"input_ids": ids, "attention_mask": self._mask(B, T, T, 0, self.mask_dtype),
                 "position_ids": np.broadcast_to(np.arange(T, dtype=np.int64)[None], (B, T)).copy(),

@@ -86,3 +86,27 @@ def test_sampler_of_one_setting_per_row_takes_batches_of_that_size_alone(fake_na
     assert sampler(logits[:3])[2] == logits[2].argmax()
     assert Sampler(temperature=[0.0])(logits[:1])[0] == logits[0].argmax()
     assert Sampler()(logits[:0]).shape == (0,)
+
+
+# ------------------------------------------------------------------ QwenSession
+def test_session_does_not_draw_from_a_row_that_the_prompt_does_not_have(fake_native):
+    """A prompt of no tokens has no last row: counted from the end, it would be that of the padding."""
+    import model_zoo as mz
+    from ir_export import extract_ir
+    from qwen_session import QwenSession
+    from sampling import Sampler
+    from test_checkpoint_session import _tiny
+
+    cfg, sd, model = _tiny()
+    L, T, S, B = cfg.num_hidden_layers, 8, 16, 2
+    irp = extract_ir(mz.QwenPrefillWrapper(model), mz.qwen2_example_inputs(cfg, B, T, None, device="cpu"), "p")
+    ird = extract_ir(mz.QwenDecodeWrapper(model, L), mz.qwen2_example_inputs(cfg, B, 1, S, device="cpu"), "d")
+    sess = QwenSession(irp, ird, mz.state_dict_numpy(sd), L)
+    ids = torch.randint(0, cfg.vocab_size, (B, T), generator=torch.Generator().manual_seed(4)).numpy()
+    for n in (1, T):
+        assert (sess.prefill(ids, n, sampler=Sampler(temperature=0.0)) == sess.prefill(ids, n)).all()
+    for n in (0, -1, -T, T + 1):
+        sess.position = 5
+        with pytest.raises(ValueError, match="prompt"):
+            sess.prefill(ids, n, sampler=Sampler())
+        assert sess.position == 5
