@@ -208,9 +208,11 @@ class QwenSession:
         out = self._dec.execute(feed)
         self.kv = dict(zip(self._kv_in, [out[n] for n in self._kv_out]))
         self.last_logits = out[self._logits_name]
-        self.position += 1
         if sampler is not None:
-            return self._draw(sampler, self.last_logits, 0)
+            tokens = self._draw(sampler, self.last_logits, 0)
+            self.position += 1   # (a step without a token can be taken again: it writes the same cache rows)
+            return tokens
+        self.position += 1
         return self._argmax.execute({"logits": self.last_logits})["token"].to_numpy().reshape(B, 1)
 
     def generate(self, input_ids: np.ndarray, max_new_tokens: int, prompt_len: int | None = None, sampler=None) -> np.ndarray:

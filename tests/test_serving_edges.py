@@ -89,20 +89,26 @@ def test_sampler_of_one_setting_per_row_takes_batches_of_that_size_alone(fake_na
 
 
 # ------------------------------------------------------------------ QwenSession
-def test_session_does_not_draw_from_a_row_that_the_prompt_does_not_have(fake_native):
-    """A prompt of no tokens has no last row: counted from the end, it would be that of the padding."""
+def _session(T=8, S=16, B=2):
     import model_zoo as mz
     from ir_export import extract_ir
     from qwen_session import QwenSession
-    from sampling import Sampler
     from test_checkpoint_session import _tiny
 
     cfg, sd, model = _tiny()
-    L, T, S, B = cfg.num_hidden_layers, 8, 16, 2
+    L = cfg.num_hidden_layers
     irp = extract_ir(mz.QwenPrefillWrapper(model), mz.qwen2_example_inputs(cfg, B, T, None, device="cpu"), "p")
     ird = extract_ir(mz.QwenDecodeWrapper(model, L), mz.qwen2_example_inputs(cfg, B, 1, S, device="cpu"), "d")
-    sess = QwenSession(irp, ird, mz.state_dict_numpy(sd), L)
     ids = torch.randint(0, cfg.vocab_size, (B, T), generator=torch.Generator().manual_seed(4)).numpy()
+    return QwenSession(irp, ird, mz.state_dict_numpy(sd), L), ids
+
+
+def test_session_does_not_draw_from_a_row_that_the_prompt_does_not_have(fake_native):
+    """A prompt of no tokens has no last row: counted from the end, it would be that of the padding."""
+    from sampling import Sampler
+
+    T = 8
+    sess, ids = _session(T)
     for n in (1, T):
         assert (sess.prefill(ids, n, sampler=Sampler(temperature=0.0)) == sess.prefill(ids, n)).all()
     for n in (0, -1, -T, T + 1):
@@ -110,3 +116,18 @@ def test_session_does_not_draw_from_a_row_that_the_prompt_does_not_have(fake_nat
         with pytest.raises(ValueError, match="prompt"):
             sess.prefill(ids, n, sampler=Sampler())
         assert sess.position == 5
+
+
+def test_session_takes_a_step_again_whose_token_could_not_be_drawn(fake_native):
+    from sampling import Sampler
+
+    sess, ids = _session()
+    first, steps = sess.prefill(ids), []
+    for _ in range(3):
+        steps.append((sess.step(first), sess.position, sess.last_logits.to_numpy().copy()))
+    sess.prefill(ids)
+    for tok, position, logits in steps:
+        with pytest.raises(ValueError, match="one for each"):
+            sess.step(first, sampler=Sampler(top_k=[1, 2, 3]))
+        assert (sess.step(first) == tok).all() and sess.position == position
+        assert (sess.last_logits.to_numpy() == logits).all()
