@@ -1,6 +1,8 @@
 """Calls of the serving operators that the documentation allows at the edge of what it says, each against the statement in 64 bits or against the
 ordinary call."""
 
+import random
+
 import pytest
 import torch
 
@@ -131,3 +133,66 @@ def test_session_takes_a_step_again_whose_token_could_not_be_drawn(fake_native):
             sess.step(first, sampler=Sampler(top_k=[1, 2, 3]))
         assert (sess.step(first) == tok).all() and sess.position == position
         assert (sess.last_logits.to_numpy() == logits).all()
+
+
+# ------------------------------------------------------------------ attention: many sequences, starts out of range
+def _many(n, tokens, keys, seed):
+    """`n` sequences: one token each but for a few of up to `tokens`, 1 to `keys` keys, some without any."""
+    r = random.Random(seed)
+    seqs = []
+    for i in range(n):
+        T = r.randint(2, tokens) if tokens > 1 and i % 9 == 4 else 1
+        seqs.append((0, r.randint(0, keys)) if i % 31 == 7 else (T, 0) if i % 97 == 50 else (T, max(T, r.randint(1, keys))))
+    return seqs
+
+
+# How the work is dealt out: up to 32 sequences (one warp), more (all threads), more than a block has threads (256 or 352; several of each), more
+# pieces in a block than a list holds (32: the block goes on with a second list over the same rings), items whole (narrow tables) and cut (wide ones).
+MANY = {
+    "chunks_33": dict(seqs=_many(33, 60, 900, 1)),
+    "chunks_60_wide": dict(seqs=_many(60, 60, 900, 2), table_extra=40),
+    "chunks_400_fp16_d64": dict(seqs=_many(400, 70, 600, 3), heads=(14, 2), dim=64, dtype=torch.float16, page=48),
+    "chunks_400_window": dict(seqs=_many(400, 40, 700, 4), window=100, table_extra=40),
+    "decode_300_wide": dict(seqs=_many(300, 1, 400, 5), table_extra=60),
+    "decode_600_8_heads": dict(seqs=_many(600, 1, 300, 6), heads=(16, 8), dim=64),
+    "draft_600_8_heads_wide": dict(seqs=_many(600, 4, 300, 7), heads=(16, 8), dim=64, dtype=torch.float16, table_extra=130),
+    "decode_4096": dict(seqs=_many(4096, 1, 100, 8)),
+    "decode_4096_wide_window": dict(seqs=_many(4096, 1, 100, 9), table_extra=70, window=33),
+    "chunks_4096": dict(seqs=_many(4096, 25, 100, 10), heads=(6, 2)),
+    "chunks_4096_wide": dict(seqs=_many(4096, 25, 100, 11), heads=(6, 2), table_extra=40),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", MANY)
+def test_attention_of_many_sequences(native_lib, name):
+    from paged_attention import paged_attention
+
+    case = MANY[name]
+    a, start, table = build(**case, seed=len(name), extra_tokens=3)
+    N = a["q"].shape[0]
+    room = torch.full((N + 8, *a["q"].shape[1:]), 7.0, dtype=a["q"].dtype, device="cuda")
+    out = room[4:4 + N]
+    paged_attention(**a, window=case.get("window", 0), out=out)
+    torch.cuda.synchronize()
+    check_attention(out, a, start, table, case["seqs"], case.get("window", 0))
+    assert (room[:4] == 7).all() and (room[4 + start[-1]:] == 7).all()
+    first = out.clone()
+    paged_attention(**a, window=case.get("window", 0), out=out)
+    assert torch.equal(out, first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 70)], [(40, 300), (1, 70)], [(1, 5000), (2, 4000)]])
+def test_attention_cuts_starts_to_the_tokens_that_are_there(native_lib, seqs):
+    """A first token ahead of the first and a last one behind the last: results are those of the tokens in between, nothing is written beside them."""
+    from paged_attention import paged_attention
+
+    a, start, table = build(seqs, seed=3, extra_tokens=5)
+    N = a["q"].shape[0]
+    room = torch.full((N + 16, 12, 128), 7.0, dtype=BF, device="cuda")
+    a["q_start"][0], a["q_start"][2] = -4, 1 << 30
+    paged_attention(**a, out=room[8:8 + N])
+    cut = [0, start[1], N]
+    check_attention(room[8:8 + N], a, cut, table, [(start[1], seqs[0][1]), (N - start[1], seqs[1][1])])
+    assert (room[:8] == 7).all() and (room[8 + N:] == 7).all()
