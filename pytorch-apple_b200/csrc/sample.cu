@@ -5,7 +5,7 @@
 // first always), min-p what weighs at least min_p.  The token drawn is the first one, by index, at which the running sum of what is kept
 // passes u times the whole sum.
 //
-// Weights are whole numbers in units of 2^-40 (their sums over a row stay below 2^62): integer sums do not depend on the order of the additions,
+// Weights are whole numbers in units of 2^-40 (their sums over a row are at most 2^62): integer sums do not depend on the order of the additions,
 // so the same row gives the same token however it is dealt to blocks, and a sum over 150 000 tokens is as exact as its terms (in
 // fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a rare token is wide).  Thresholds are found on the logits
 // themselves, never on weights.
@@ -36,7 +36,7 @@ template <> struct Pair<__half> { using type = __half2; };
 template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 constexpr int ST = 512, SW = ST / 32;        // threads and warps of a CTA
 constexpr int MAX_CTAS = 8;                  // of a row
-constexpr int64_t MAX_COLS = 1 << 22;        // sums of weights stay below 2^62
+constexpr int64_t MAX_COLS = 1 << 22;        // sums of weights are at most 2^62
 constexpr u64 ONE = 1ull << 40;              // weight of the row's maximum
 constexpr int BINS = 16;
 constexpr int CAP = 2048;                    // tokens of a list
@@ -369,14 +369,6 @@ template <typename T> struct Row {
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     }
   }
-  template <typename F> __device__ __forceinline__ void packs(F&& f) const {
-#pragma unroll 2
-    for (int c = begin + (threadIdx.x & 31) * 8; c < end; c += 256) {
-      float v[8];
-      load(c, v);
-      f(v, c);
-    }
-  }
   template <typename F> __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 2
     for (int c = begin + (threadIdx.x & 31) * 8; c < end; c += 256) {
@@ -388,7 +380,7 @@ template <typename T> struct Row {
   }
 };
 
-__device__ __forceinline__ u64 warp_add(u64 v) {   // (v below 2^62; in three parts the warp's own instruction does it)
+__device__ __forceinline__ u64 warp_add(u64 v) {   // (v at most 2^62; in three parts the warp's own instruction does it)
   const uint32_t a = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0x3ffffffu), b = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 26) & 0x3ffffffu);
   return a + (static_cast<u64>(b) << 26) + (static_cast<u64>(__reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 52))) << 52);
 }

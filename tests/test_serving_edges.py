@@ -3,10 +3,11 @@ ordinary call."""
 
 import random
 
+import numpy as np
 import pytest
 import torch
 
-from test_paged_and_sampling import BF, _small, build, check_attention, gen, torch_calls  # noqa: F401
+from test_paged_and_sampling import BF, _small, build, check_attention, check_draw, gen, torch_calls  # noqa: F401
 
 
 # ------------------------------------------------------------------ max_q
@@ -196,3 +197,15 @@ def test_attention_cuts_starts_to_the_tokens_that_are_there(native_lib, seqs):
     cut = [0, start[1], N]
     check_attention(room[8:8 + N], a, cut, table, [(start[1], seqs[0][1]), (N - start[1], seqs[1][1])])
     assert (room[:8] == 7).all() and (room[8 + N:] == 7).all()
+
+
+# ------------------------------------------------------------------ the draw
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_draw_from_the_longest_flat_row(native_lib, dtype):
+    """4194304 equal tokens of weight 2^40 each: their sum is 2^62, and all of it is exact."""
+    x = torch.full((3, 1 << 22), -2.5, dtype=dtype)
+    u = np.array([0.0, 0.6180339, 1.0 - 2.0 ** -24])
+    check_draw(x, u)
+    check_draw(x, u, top_k=np.full(3, 3000001))
+    check_draw(x, u, top_p=np.full(3, 0.75), min_p=np.ones(3))
