@@ -457,7 +457,7 @@ int b200_paged_append(const b200_paged_append_args* args, void* stream);
  * ids outside the cache read as zeros; table entries of pages without an attended key are not looked at, and what lies in pages
  * behind kv_len or ahead of the window does not matter, whatever it is (keys and values that some token of the chunk does see
  * have to be finite: other tokens of its tile give them the weight zero).  Lengths and starts are cut to the table and to n_tokens.
- * Probabilities are rounded to the activation type for the second product; sums and accumulators are fp32.
+ * Probabilities are rounded to the activation type for the second product (as in the static-cache kernels); sums and accumulators are fp32.
  * workspace: 16-byte aligned, b200_attn_paged_workspace_bytes bytes of any content; calls that may overlap need one each.
  * The result depends on the arguments alone (pieces are joined in a fixed order, no atomics). */
 typedef struct b200_attn_paged_args {

@@ -22,6 +22,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 //
 // us: one sequence of 613 keys 8.4 (launch 2.3, lengths and pages 3, keys 2, sums 1), of 20001 keys 10.9; 64 of 512 to 4352 keys 28.5, of which 17 are the
 // keys at 6.5 TB/s, 4.3 what precedes the first copy and 4.5 the joining kernel.  A warp has 24 KB on its way, 196 KB per SM.
+//
+// Probabilities are rounded to the activation type, which the MMA takes (sums are of the unrounded ones, in fp32): against 64 bits the output is off by 0.22 % in bf16
+// (root mean square), 0.16 of which is its own rounding.  At 18 % of the issue slots the MMAs are not the bound, but two for each would lengthen the chain per block of keys.
 // ===========================================================================
 constexpr int FEW_WARPS = 8, FEW_KEYS = 16;
 // What an item costs besides its 16-key blocks, in blocks (a round of the eight warps is eight).  us at 4 / 8 / 16 / 28: 64 ragged sequences 29.6 / 29.1 / 28.6 / 28.1,
@@ -577,8 +580,11 @@ extern "C" int b200_attn_paged(const b200_attn_paged_args* args, void* stream) {
   p.ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + ml);
   p.acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + acc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Short tables: no cache is so long that a block of its own for each item would take longer than joining pieces does (4 us, and a launch
-  // on the host).  us, pieces -> whole: one sequence of 613 keys 10.7 -> 8.5, 19 with four tokens each and up to 1111 keys of 64 dims 15.5 -> 13.3.
+  // Short tables: a block of its own for each item takes hardly longer than joining pieces does, and saves a launch on the host.  By the table's width, as the lengths are on the
+  // device: a wide table over short sequences gets pieces.  us, pieces -> whole, tables as wide as the sequences are long:
+  //   1 sequence of 300 / 613 / 800 / 1024 / 2000 keys 8.7 -> 7.0, 8.8 -> 8.4, 8.8 -> 9.4, 8.8 -> 10.0, 9.0 -> 14.8; 8 of up to 1000 9.4 -> 9.9, 64 14.6 -> 15.0, 200 27.5 -> 27.1;
+  //   19 with four tokens each, 64 dims, up to 1024 / 2000 keys 14.8 -> 11.7, 18.7 -> 16.6; tiles of 128 rows: 22 tokens over 512 / 1000 keys 13.3 -> 12.2, 14.2 -> 17.0,
+  //   128 over 512 / 1000 15.1 -> 13.6, 16.0 -> 18.2, 512 over 512 / 1000 15.8 -> 14.0, 18.5 -> 18.5.
   p.whole = a.table_stride * a.page_size * D <= (rows == PAGED_TC5_ROWS ? 512 : 1024) * 128 ? 1 : 0;
   int rc = B200_ENOTSUP;
   if (tc5_enabled()) {

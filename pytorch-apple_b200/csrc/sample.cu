@@ -10,16 +10,23 @@
 // fp32 a boundary between two tokens would move by 2^-24 of the sum, more than a rare token is wide).  Thresholds are found on the logits
 // themselves, never on weights.
 //
-// A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once where it fits (a bulk copy
-// per warp) and then goes through a few times: for the maximum; for the sum of the weights where it is needed; for the tokens that are large enough to matter. How
+// A row belongs to the CTAs of a cluster, each with a contiguous range of columns that it brings into shared memory once where it fits and the row starts on a 16-byte
+// boundary (a bulk copy per warp; other rows are read from memory in every pass, element by element) and then goes through a few times: for the maximum; for the sum of the weights where it is needed; for the tokens that are large enough to matter. How
 // large that is the maxima of the threads' own tokens tell: the k-th largest of them has at least k tokens at or above it, and hardly more. Those tokens are
 // sorted by one CTA, which mostly finds everything that is kept among them and finishes alone. Where it does not (flat rows, thousands of tokens kept), counts or
 // weights in 16 intervals of z, then in 16 parts of the one in which the last token kept lies, and so on, lead to a list of tokens around it, and the row is
 // drawn from by sums over ranges.
 //
-// 64 rows of 151 936 tokens in bf16 (19.4 MB, 3 us of memory), us: greedy 7, top-k 50 14, top-k 400 22, no filter 16, top-p 0.9 22, min-p 0.05 11, flat rows
-// that keep tens of thousands 115; one row 4, 11, 15, 8, 15, 7.5, 55; 200 rows 17, 30, 53, 45, 57.  Not the memory is the bound: launch and copy are 4.5 of it, every meeting of a row's CTAs is
-// 1 (there are two to six), the sum of the weights 6 (76 000 tokens per SM, an exponential and about 18 instructions each), sorting and the draw 2 to 8.
+// us per call, twenty to a graph, rows of 151 936 tokens in bf16 (64 of them 19.4 MB, 3 us of memory; normal with a spread of 2.2 and some 300 likelier tokens), all at
+// temperature 1 but for the greedy and the flat ones (temperature 3):
+//            greedy  top-k 50  top-k 400  no filter  top-p 0.9  min-p 0.05  top-k 2000  flat, top-p 0.95
+//   1 row       4.3      11.1       14.6        8.5       14.9         7.8        25.4        54.4
+//   64 rows     6.6      14.3       22.6       16.3       22.0        11.5        70.9       115
+//   200 rows   16.6      29.6       53.2       45.1       57.4        28.1       180         394
+//   64 rows of 151 937 (seven of eight start off a 16-byte boundary): 22.8, 29.9, no filter 31.1, top-p 44.8, flat 176; of 50 257 against 50 256: 10.5 / 4.9, 18.1 / 12.9,
+//   15.3 / 10.1, 24.5 / 16.9.
+// Not the memory is the bound: launch and copy are 4.5 of it, every meeting of a row's CTAs is 1 (there are two to six), the sum of the weights 6 (76 000 tokens per SM, an
+// exponential and about 18 instructions each), sorting and the draw 2 to 8.
 #include <type_traits>
 
 #include "common.cuh"
