@@ -92,14 +92,17 @@ def build_torch_calls(force: bool = False, verbose: bool = False) -> Path:
     cuda = Path(_nvcc()).resolve().parents[1]
     includes = [base / "include", base / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], cuda / "include"]
     CALLS_PATH.unlink(missing_ok=True)   # (where it does not compile, what was there is not to be loaded)
+    made = CALLS_PATH.with_suffix(f".{os.getpid()}.so")   # (nobody finds half of it)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DB200_BUILT_FOR="{built_for}"', *(f"-I{p}" for p in includes), str(src), "-o", str(CALLS_PATH), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch",
+           f'-DB200_BUILT_FOR="{built_for}"', *(f"-I{p}" for p in includes), str(src), "-o", str(made), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
+        made.unlink(missing_ok=True)
         raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(made, CALLS_PATH)
     return CALLS_PATH
 
 

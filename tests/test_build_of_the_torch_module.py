@@ -60,3 +60,25 @@ def test_the_library_is_built_where_the_module_cannot_be(monkeypatch, trouble):
     monkeypatch.setattr(build_native, "build_torch_calls", fail)
     with pytest.warns(UserWarning, match="b200_torch_calls.so"):
         assert build_native.build() == build_native.LIB_PATH
+
+
+def test_nobody_finds_half_a_module(compiler, monkeypatch, tmp_path):
+    """While it is compiled there is none, and a failed build leaves none behind."""
+    target = tmp_path / "b200_torch_calls.so"
+    target.write_bytes(b"of another torch")
+    monkeypatch.setattr(build_native, "CALLS_PATH", target)
+    write, codes = subprocess.run, [1, 0]
+
+    def run(cmd, **kw):
+        assert not target.exists()
+        done = write(cmd, **kw)
+        assert not target.exists()
+        done.returncode = codes.pop(0)
+        return done
+
+    monkeypatch.setattr(subprocess, "run", run)
+    with pytest.raises(RuntimeError, match="failed for torch_calls.cpp"):
+        build_native.build_torch_calls()
+    assert list(tmp_path.iterdir()) == []
+    assert build_native.build_torch_calls() == target
+    assert list(tmp_path.iterdir()) == [target]
